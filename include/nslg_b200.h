@@ -363,6 +363,105 @@ int nslg_plan_decode_host(int batch, int page_size, const int32_t* slots, const 
                           int64_t bt_stride, int64_t bt_rows, int32_t* plan,
                           int64_t max_indices, uint32_t* dev_status, void* stream);
 
+/* ------------------------------------------------------------------- 8-bit KV cache
+ *
+ * The paged cache at one byte per element (no counterpart in the reference, whose pool has
+ * the activation type, kv_cache.py:382-398). One layer is four arrays:
+ *   codes_k, codes_v   e4m3 [num_pages, num_kv_heads, page_size, head_dim]
+ *   scale_k, scale_v   fp32 [num_pages, num_kv_heads]
+ * value = code * scale of its block (the page_size tokens of one page, one kv head). The
+ * append writes the smallest power of two s with amax <= 448 s (0 for a block of zeros, at
+ * least 2^-126, NaN for a block that holds a value that is not finite: all of that block
+ * then reads as NaN). The readers take any scale. Page lists are the CSR of the other
+ * entry points; page 0 needs no special contents, and a page that is handed out again
+ * needs no clearing. head_dim is a multiple of 32 up to 256; page_size 16 with head_dim 64
+ * or 128 and 16-bit activations runs on the tensor cores, the rest on CUDA cores. Pointers
+ * are 16-byte aligned (scales 4), row strides are in elements, a multiple of 16 bytes, and
+ * cover a row. */
+
+/* Rotary embedding of q and k, and k and v quantised into the pages as they are written.
+ * Sequence b has qo_len(b) = qo_indptr[b+1] - qo_indptr[b] new rows, rows q_row_start[b] + i
+ * (qo_indptr[b] + i when q_row_start is NULL) of q, k, v and q_out; row i is the token at
+ * position kv_len(b) - qo_len(b) + i of the sequence, kv_len(b) being the length of its page
+ * list, the new tokens included. That position is also its row of the cos / sin tables
+ * (fp32 [table_rows, head_dim], NULL: no rotation). The rotation is computed in fp32 (every
+ * product and the sum rounded once); q_out [num_rows, num_qo_heads, head_dim] is rounded to
+ * the activation type, k is quantised without a rounding between. q_out NULL: q is left
+ * alone. q_out may be q itself when q is contiguous. Rows of no sequence are left as they are.
+ *
+ * Where a page holds tokens of the sequence from before the call, its scale never shrinks,
+ * and where it grows their codes are rounded again for the new scale (exact but for codes
+ * that become e4m3 subnormals). A page whose first slot is written starts afresh. Writing
+ * the same rows again changes nothing. A page written by a call belongs to one sequence of
+ * that call (copy a shared page first, codes and scales).
+ *
+ * max_qo_len bounds qo_len(b). A sequence with more rows than that, more than kv_len(b) or
+ * rows outside [0, num_rows) sets NSLG_DEV_BAD_PLAN and is skipped; a page outside the pool
+ * sets NSLG_DEV_BAD_PAGE (q is still rotated); a position outside the tables sets
+ * NSLG_DEV_BAD_POSITION and the part of the page's rows the call writes stays unrotated. */
+int nslg_rope_kv8_append(int dtype, int batch, int num_qo_heads, int num_kv_heads, int head_dim,
+                         int page_size, const void* q, int64_t q_stride, const void* k,
+                         int64_t k_stride, const void* v, int64_t v_stride, int64_t num_rows,
+                         void* q_out, const float* cos_table, const float* sin_table,
+                         int64_t table_rows, void* codes_k, void* codes_v, float* scale_k,
+                         float* scale_v, int64_t num_pages, const int32_t* qo_indptr,
+                         const int32_t* q_row_start, int max_qo_len, const int32_t* kv_indptr,
+                         const int32_t* kv_indices, const int32_t* kv_last_page_len,
+                         uint32_t* dev_status, void* stream);
+
+/* Pages read back as values of the activation type `dtype`: out_k and out_v are
+ * [num_indices, page_size, num_kv_heads, head_dim], page j of the list (j < kv_indptr[batch]
+ * <= num_indices) at out[j]; slots behind a sequence's last token and pages outside the pool
+ * (NSLG_DEV_BAD_PAGE) read as zeros, the pages of out behind the list are left as they are.
+ * A finite value beyond fp16's range reads as +-65504 there. */
+int nslg_kv8_gather(int dtype, int batch, int num_kv_heads, int head_dim, int page_size,
+                    const void* codes_k, const void* codes_v, const float* scale_k,
+                    const float* scale_v, int64_t num_pages, const int32_t* kv_indptr,
+                    const int32_t* kv_indices, const int32_t* kv_last_page_len,
+                    int64_t num_indices, void* out_k, void* out_v, uint32_t* dev_status,
+                    void* stream);
+
+/* Bytes of scratch nslg_paged_decode_kv8 needs. As with nslg_paged_decode: zeroed before its
+ * first use, left with its counts at zero by every call, not to be shared by calls that may
+ * overlap on the GPU. */
+int64_t nslg_decode_kv8_workspace_bytes(int batch, int num_qo_heads, int num_kv_heads,
+                                        int head_dim);
+
+/* nslg_paged_decode over the 8-bit cache: one query row per sequence, the same sequence and
+ * head conventions, zeros for a sequence without pages. Launched with programmatic dependent
+ * launch under the rule given there (the CSR arrays may be read before the kernel before it
+ * on the stream has finished). */
+int nslg_paged_decode_kv8(int dtype, int batch, int num_qo_heads, int num_kv_heads, int head_dim,
+                          int page_size, const void* q, int64_t q_stride, void* out,
+                          int64_t out_stride, const void* codes_k, const void* codes_v,
+                          const float* scale_k, const float* scale_v, int64_t num_pages,
+                          const int32_t* kv_indptr, const int32_t* kv_indices,
+                          const int32_t* kv_last_page_len, float sm_scale, void* workspace,
+                          int64_t workspace_bytes, uint32_t* dev_status, void* stream);
+
+/* Bytes of scratch nslg_paged_prefill_kv8 needs for these sizes; num_indices is the capacity
+ * of the page list (kv_indptr[batch] <= num_indices). Needs no clearing. */
+int64_t nslg_prefill_kv8_workspace_bytes(int dtype, int batch, int num_qo_heads, int num_kv_heads,
+                                         int head_dim, int page_size, int max_qo_len,
+                                         int64_t num_indices);
+
+/* nslg_paged_prefill over the 8-bit cache: the same rows, mask and head conventions. Rows of
+ * no sequence are left as they are; a row that sees no position (qo_len(b) > kv_len(b)) is
+ * zeros. */
+int nslg_paged_prefill_kv8(int dtype, int batch, int num_qo_heads, int num_kv_heads, int head_dim,
+                           int page_size, const void* q, int64_t q_stride, int64_t q_rows,
+                           void* out, int64_t out_stride, const int32_t* qo_indptr,
+                           const int32_t* q_row_start, int max_qo_len, const void* codes_k,
+                           const void* codes_v, const float* scale_k, const float* scale_v,
+                           int64_t num_pages, const int32_t* kv_indptr, const int32_t* kv_indices,
+                           const int32_t* kv_last_page_len, int64_t num_indices, float sm_scale,
+                           int causal, void* workspace, int64_t workspace_bytes,
+                           uint32_t* dev_status, void* stream);
+
+/* The number of the graph capture that `stream` is part of, 0 when it is not capturing: a
+ * caller that keeps a workspace per stream gives each captured graph one of its own. */
+int nslg_stream_capture_id(void* stream, uint64_t* id);
+
 /* ---------------------------------------------------------------- tensor parallel */
 
 #define NSLG_IPC_HANDLE_BYTES 64   /* cudaIpcMemHandle_t                                 */

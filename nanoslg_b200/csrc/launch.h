@@ -162,4 +162,55 @@ int launch_linear_tc(int dtype, int M, int N, int K, const void* x, int64_t x_st
                      const TpPush* push, uint32_t* status, cudaStream_t stream,
                      bool swiglu = false, const LinearRope* rope = nullptr);
 
+// ---------------------------------------------------------------- 8-bit KV cache (kv8.cuh)
+// One layer of the cache and the sequences' pages in it.
+struct Kv8Cache {
+  void* codes_k;        // e4m3 [num_pages, hkv, page_size, d]
+  void* codes_v;
+  float* scale_k;       // [num_pages, hkv]
+  float* scale_v;
+  int64_t num_pages;
+  const int32_t* kv_indptr;
+  const int32_t* kv_indices;
+  const int32_t* kv_lpl;
+};
+
+struct Kv8AppendParams : Kv8Cache {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* q_out;          // [num_rows, hq, d]
+  const float* cos_t;   // null: no rotation
+  const float* sin_t;
+  const int32_t* qo_indptr;
+  const int32_t* q_row_start;
+  int64_t q_stride, k_stride, v_stride, num_rows, table_rows;
+  int batch, hq, hkv, d, page_size, group, max_qo_len;
+  int pages_per_seq;    // pages that max_qo_len tokens can touch
+  uint32_t* status;
+};
+int launch_kv8_append(int dtype, const Kv8AppendParams& p, cudaStream_t stream);
+
+struct Kv8GatherParams : Kv8Cache {
+  void* out_k;          // [num_indices, page_size, hkv, d] of the output type
+  void* out_v;
+  int64_t num_indices;
+  int batch, hkv, d, page_size;
+  uint32_t* status;
+};
+int launch_kv8_gather(int dtype, const Kv8GatherParams& p, cudaStream_t stream);
+
+struct Kv8AttnParams : Kv8Cache {
+  const void* q;
+  void* out;
+  const int32_t* qo_indptr;     // null: decode, row b is the one query of sequence b
+  const int32_t* q_row_start;
+  int64_t q_stride, out_stride, num_rows;
+  int batch, hq, hkv, d, page_size, max_qo_len, causal;
+  float sm_scale;
+  uint32_t* status;
+};
+// CUDA cores: any page size, head_dim a multiple of 32 up to 256, all three types.
+int launch_kv8_attention_simt(int dtype, const Kv8AttnParams& p, cudaStream_t stream);
+
 }  // namespace nslg

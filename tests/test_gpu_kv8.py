@@ -1,0 +1,365 @@
+"""The 8-bit KV cache on the GPU against its 64-bit definition (oracle/kv8.py).
+
+The append is compared bit for bit: scales, codes and q follow from fp32 operations whose
+rounding is fixed. Attention tolerances are derived in kv8_util.attention_bound."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import kv8_util as U
+from nanoslg_b200 import ops
+from oracle import kv8
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+
+
+@pytest.fixture(autouse=True)
+def _clean_status():
+    ops.status_word(DEV).zero_()
+    yield
+    ops.check_device_status(DEV)
+
+
+def _tables(rows, d):
+    ang = torch.outer(torch.arange(rows, dtype=torch.float64),
+                      10000.0 ** (-torch.arange(0, d, 2, dtype=torch.float64) / d))
+    ang = torch.cat([ang, ang], 1)
+    return ang.cos().float(), ang.sin().float()
+
+
+def _append(cache, oracle, tables, starts, counts, hq, dt, seed, rope, ps, left=0, spread=1.0):
+    """One append of counts[b] tokens behind starts[b], on the kernel and on the oracle; rows
+    are left padded by ``left``. Returns (q_out, expected q_out) of the real rows."""
+    hkv, d = cache[0].shape[1], cache[0].shape[3]
+    lens = [s + n for s, n in zip(starts, counts)]
+    width = max(counts) + left
+    row_start = [b * width + width - n for b, n in enumerate(counts)]
+    q = U.rows((len(lens) * width, hq, d), dt, seed, spread)
+    k = U.rows((len(lens) * width, hkv, d), dt, seed + 1, spread)
+    v = U.rows((len(lens) * width, hkv, d), dt, seed + 2, spread)
+    cos, sin = _tables(max(lens) + 1, d)
+    npg = [-(-n // ps) for n in lens]
+    ptr, idx, lpl = U.csr([t[:n] for t, n in zip(tables, npg)], lens, ps, DEV, spare=3)
+    qo = torch.tensor(np.cumsum([0] + counts), dtype=torch.int32, device=DEV)
+    got = ops.rope_kv8_append(q.to(DEV), k.to(DEV), v.to(DEV), cos.to(DEV), sin.to(DEV), *cache, qo,
+                              max(counts), ptr, idx, lpl,
+                              q_row_start=torch.tensor(row_start, dtype=torch.int32, device=DEV),
+                              rotate=rope).cpu()
+    mine, want = [], []
+    for b, (s, n) in enumerate(zip(starts, counts)):
+        r = slice(row_start[b], row_start[b] + n)
+        kf, qf = k[r].float().numpy(), q[r].float().numpy()
+        if rope:
+            c, t = cos[s:s + n].numpy(), sin[s:s + n].numpy()
+            kf, qf = kv8.rotate(kf, c, t), kv8.rotate(qf, c, t)
+        oracle.append(tables[b], s, kf, v[r].float().numpy())
+        mine.append(got[r])
+        want.append(torch.from_numpy(qf).to(dt))
+    return torch.cat(mine), torch.cat(want)
+
+
+def _assert_cache(cache, oracle, tables, lens):
+    for i, name in enumerate("kv"):
+        for t, n in zip(tables, lens):
+            t = t[:-(-n // oracle.ps)]
+            np.testing.assert_array_equal(cache[2 + i].cpu().numpy()[t], oracle.s[name][t])
+            np.testing.assert_array_equal(U.values(cache[i], cache[2 + i], t, n),
+                                          oracle.read(t, n, name))
+
+
+APPEND = [
+    # dtype, hq, hkv, d, page size, starts, counts, rope
+    (torch.bfloat16, 32, 8, 128, 16, [0, 0, 0], [1, 16, 33], True),
+    (torch.bfloat16, 32, 8, 128, 16, [5, 15, 16, 100], [1, 1, 1, 1], True),
+    (torch.float16, 8, 2, 64, 16, [3, 31, 0], [40, 1, 17], True),
+    (torch.float16, 16, 2, 128, 16, [7, 8], [1, 1], True),
+    (torch.bfloat16, 4, 4, 64, 16, [1, 2, 0], [1, 1, 1], True),
+    (torch.float32, 4, 2, 64, 16, [0, 9], [25, 3], True),
+    (torch.float32, 4, 2, 64, 16, [4, 9], [1, 1], True),
+    (torch.bfloat16, 6, 3, 96, 5, [0, 4, 12], [11, 1, 2], True),
+    (torch.float16, 5, 5, 32, 1, [0, 3], [4, 1], True),
+    (torch.bfloat16, 64, 4, 128, 16, [12, 0], [70, 2], False),
+    (torch.bfloat16, 2, 1, 256, 64, [60, 0], [9, 130], True),
+]
+
+
+@pytest.mark.parametrize("dt,hq,hkv,d,ps,starts,counts,rope", APPEND)
+def test_append_is_the_definition(dt, hq, hkv, d, ps, starts, counts, rope):
+    lens = [s + n for s, n in zip(starts, counts)]
+    pages = sum(-(-n // ps) for n in lens) + 5
+    tables = U.page_lists(lens, ps, pages, 1)
+    cache = U.random_cache(pages, hkv, ps, d, DEV, 2)           # leftovers in every page
+    cache[0].view(torch.uint8)[:, :, ps - 1] = 0x7F             # NaN codes among them
+    oracle = kv8.Cache(pages, hkv, ps, d)
+    before = [t.clone() for t in cache]
+    if any(starts):
+        first = [s if s else 1 for s in starts]                 # every page list gets a start
+        _append(cache, oracle, tables, [0] * len(lens), [min(f, n) for f, n in zip(first, lens)],
+                hq, dt, 50, rope, ps)
+    for again in range(2):                                      # the second writes the same rows
+        q, want = _append(cache, oracle, tables, starts, counts, hq, dt, 60, rope, ps, left=2)
+        assert torch.equal(q, want)
+        _assert_cache(cache, oracle, tables, lens)
+    untouched = np.setdiff1d(np.arange(pages), np.concatenate(tables))
+    for t, b in zip(cache, before):
+        assert torch.equal(t.view(torch.uint8)[untouched], b.view(torch.uint8)[untouched])
+
+
+@pytest.mark.parametrize("dt,d", [(torch.bfloat16, 128), (torch.float16, 64), (torch.float32, 64)])
+def test_append_token_by_token_grows_the_scale(dt, d):
+    """Tokens of growing size, one a call: every step re-rounds the page's older codes."""
+    cache, oracle = ops.kv8_pages(6, 16, 2, d, DEV), kv8.Cache(6, 2, 16, d)
+    table = [np.array([4, 2, 5], np.int32)]
+    for t in range(40):
+        q, want = _append(cache, oracle, table, [t], [1], 4, dt, 7 * t, True, 16, spread=2.0)
+        assert torch.equal(q, want)
+        _assert_cache(cache, oracle, table, [t + 1])
+
+
+@pytest.mark.parametrize("n", [1, 20])
+def test_append_zeros_and_values_that_are_not_finite(n):
+    hkv, d = 2, 64
+    cache = ops.kv8_pages(4, 16, hkv, d, DEV)
+    k = torch.zeros(n, hkv, d, dtype=torch.bfloat16)
+    v = U.rows((n, hkv, d), torch.bfloat16, 3)
+    v[0, 1, 5] = math.inf
+    ptr, idx, lpl = U.csr([np.array([1, 3], np.int32)[:-(-n // 16)]], [n], 16, DEV)
+    qo = torch.tensor([0, n], dtype=torch.int32, device=DEV)
+    ops.rope_kv8_append(None, k.to(DEV), v.to(DEV), None, None, *cache, qo, n, ptr, idx, lpl,
+                        rotate=False)
+    sk, sv = cache[2].cpu(), cache[3].cpu()
+    assert bool((sk[1] == 0).all()) and bool(torch.isnan(sv[1, 1])) and bool(sv[1, 0] > 0)
+    kk, vv = ops.kv8_gather(*cache, ptr, idx, lpl, torch.bfloat16)
+    assert bool((kk == 0).all())
+    assert bool(torch.isnan(vv[0, :min(n, 16), 1]).all()) and bool(torch.isfinite(vv[0, :, 0]).all())
+    if n > 16:
+        assert bool(torch.isfinite(vv[1]).all())
+    # the block stays NaN while its page lasts, and a page begun again is clean
+    if n == 1:
+        ptr2, idx2, lpl2 = U.csr([np.array([1], np.int32)], [2], 16, DEV)
+        one = torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+        fine = U.rows((1, hkv, d), torch.bfloat16, 4).to(DEV)
+        ops.rope_kv8_append(None, fine, fine, None, None, *cache, one, 1, ptr2, idx2, lpl2, rotate=False)
+        assert bool(torch.isnan(cache[3][1, 1]))
+        ops.rope_kv8_append(None, fine, fine, None, None, *cache, one, 1, ptr, idx, lpl, rotate=False)
+        assert bool(torch.isfinite(cache[3][1]).all())
+
+
+def test_append_bad_plans_are_reported_and_skipped():
+    hkv, d = 2, 64
+    cache = U.random_cache(8, hkv, 16, d, DEV, 5)
+    before = [t.clone() for t in cache]
+    x = U.rows((12, hkv, d), torch.bfloat16, 1).to(DEV)
+    cos, sin = (t.to(DEV) for t in _tables(64, d))
+
+    def run(qo, most, table, length, rows=None, tables=(cos, sin)):
+        ptr, idx, lpl = U.csr([np.array(table, np.int32)], [length], 16, DEV)
+        rs = None if rows is None else torch.tensor([rows], dtype=torch.int32, device=DEV)
+        q = torch.full_like(x, 9.0)
+        ops.rope_kv8_append(x, x, x, *tables, *cache, torch.tensor([0, qo], dtype=torch.int32, device=DEV),
+                            most, ptr, idx, lpl, q_row_start=rs, q_out=q)
+        return q
+
+    for args, what in (((12, 12, [1], 5), "plan entry"), ((12, 4, [1], 16), "plan entry"),
+                       ((4, 4, [1], 16, 10), "plan entry"), ((4, 4, [1], 16, -1), "plan entry"),
+                       ((4, 4, [8], 16), "page id"), ((4, 4, [-1], 16), "page id")):
+        q = run(*args)
+        with pytest.raises(RuntimeError, match=what):
+            ops.check_device_status(DEV)
+        assert what == "page id" or bool((q == 9.0).all())
+        for t, b in zip(cache, before):
+            assert torch.equal(t.view(torch.uint8), b.view(torch.uint8))
+    run(4, 4, [1], 16, None, (cos[:14].contiguous(), sin[:14].contiguous()))   # positions 12 to 15
+    with pytest.raises(RuntimeError, match="RoPE table"):
+        ops.check_device_status(DEV)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("hkv,d,ps,lens", [(8, 128, 16, [1, 0, 33, 512]), (2, 64, 16, [300]),
+                                           (3, 96, 5, [7, 5, 1]), (1, 256, 64, [65])])
+def test_gather_is_code_times_scale(dt, hkv, d, ps, lens):
+    pages = sum(-(-n // ps) for n in lens) + 3
+    tables = U.page_lists(lens, ps, pages, 3)
+    cache = U.random_cache(pages, hkv, ps, d, DEV, 4, power=False)
+    cache[0].view(torch.uint8)[:, :, ps - 1, 0] = 0x7F          # NaN codes, kept where in length
+    ptr, idx, lpl = U.csr(tables, lens, ps, DEV, spare=2)
+    total = sum(len(t) for t in tables)
+    out = tuple(torch.full((total + 2, ps, hkv, d), 7.0, dtype=dt, device=DEV) for _ in range(2))
+    got = ops.kv8_gather(*cache, ptr, idx, lpl, dt, out=out)
+    for i in range(2):
+        assert got[i] is out[i]
+        at = 0
+        for t, n in zip(tables, lens):
+            x = got[i][at:at + len(t)].cpu().reshape(-1, hkv, d)
+            # one product of a code and a scale, rounded to fp32 and once to dt
+            want = torch.from_numpy(U.values(cache[i], cache[2 + i], t, n)).float().to(dt)
+            torch.testing.assert_close(x[:n], want, rtol=0, atol=0, equal_nan=True)
+            assert bool((x[n:] == 0).all())
+            at += len(t)
+        assert bool((got[i][total:] == 7.0).all())
+
+
+def test_gather_saturates_finite_values_to_fp16():
+    cache = ops.kv8_pages(2, 16, 1, 32, DEV)
+    x = torch.full((1, 1, 32), 65504.0, dtype=torch.float16, device=DEV)
+    ptr, idx, lpl = U.csr([np.array([1], np.int32)], [1], 16, DEV)
+    qo = torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+    ops.rope_kv8_append(None, x, -x, None, None, *cache, qo, 1, ptr, idx, lpl, rotate=False)
+    k, v = ops.kv8_gather(*cache, ptr, idx, lpl, torch.float16)
+    assert bool((k[0, 0] == 65504.0).all()) and bool((v[0, 0] == -65504.0).all())
+    k32, _ = ops.kv8_gather(*cache, ptr, idx, lpl, torch.float32)
+    assert bool((k32[0, 0] == 65536.0).all())
+
+
+def _check_attention(out, q, cache, tables, lens, counts, row_start, sm_scale, p_half, causal=True):
+    out = out.cpu()
+    for b, (t, n, c) in enumerate(zip(tables, lens, counts)):
+        r = slice(row_start[b], row_start[b] + c)
+        k, v = (U.values(cache[i], cache[2 + i], t, n) for i in range(2))
+        qd = q[r].cpu().double().numpy()
+        want = kv8.attention(qd, k, v, sm_scale, causal)
+        bound = U.attention_bound(qd, k, v, sm_scale, want, out.dtype, p_half, causal)
+        err = np.abs(out[r].double().numpy() - want)
+        assert not np.isnan(err).any(), (b, n)
+        assert (err <= bound).all(), (b, n, float((err / bound).max()))
+
+
+DECODE = [
+    # dtype, hq, hkv, d, page size, lens
+    (torch.bfloat16, 32, 8, 128, 16, [1, 15, 16, 17, 100, 1000]),
+    (torch.float16, 32, 8, 128, 16, [513]),
+    (torch.float16, 16, 2, 128, 16, [0, 33, 0, 700, 0]),
+    (torch.bfloat16, 4, 1, 128, 16, [2, 31, 32, 600]),
+    (torch.bfloat16, 16, 1, 128, 16, [77, 1200]),
+    (torch.bfloat16, 64, 8, 128, 16, [40, 513]),
+    (torch.float16, 8, 8, 128, 16, [19, 260]),
+    (torch.bfloat16, 8, 2, 64, 16, [9, 300, 1024]),
+    (torch.float16, 12, 3, 64, 16, [5, 160, 64]),
+    (torch.bfloat16, 10, 5, 128, 16, [129, 48, 3]),
+    (torch.bfloat16, 34, 2, 128, 16, [70, 5]),
+    (torch.float32, 4, 2, 64, 16, [1, 50, 33]),
+    (torch.float32, 32, 8, 128, 16, [130]),
+    (torch.bfloat16, 6, 3, 96, 5, [12, 1]),
+    (torch.float16, 2, 1, 256, 64, [65]),
+]
+
+
+def _p_half(dt):
+    # the products of 16-bit types take probabilities of the type or of fp16
+    return U.HALF[dt] if dt != torch.float32 else 0.0
+
+
+@pytest.mark.parametrize("dt,hq,hkv,d,ps,lens", DECODE)
+def test_decode_is_the_definition(dt, hq, hkv, d, ps, lens):
+    pages = sum(-(-n // ps) for n in lens) + 3
+    tables = U.page_lists(lens, ps, pages, 11)
+    cache = U.random_cache(pages, hkv, ps, d, DEV, 12, power=d != 64)
+    for t, n in zip(tables, lens):
+        if n % ps:                                  # slots behind the last token hold NaN codes
+            for pool in cache[:2]:
+                pool.view(torch.uint8)[int(t[-1]), :, n % ps:] = 0x7F
+    wide = U.rows((len(lens), hq + 2, d), dt, 13).to(DEV)
+    q = wide[:, 1:-1]                               # a strided view
+    sm = 1 / math.sqrt(d)
+    plan = U.csr(tables, lens, ps, DEV, spare=1)
+    out = ops.paged_decode_kv8(q, *cache, *plan, sm)
+    _check_attention(out, q, cache, tables, lens, [1] * len(lens), list(range(len(lens))), sm,
+                     _p_half(dt))
+    again = torch.full((len(lens), hq + 1, d), 3.0, dtype=dt, device=DEV)
+    ops.paged_decode_kv8(q, *cache, *plan, sm, out=again[:, :hq])
+    assert torch.equal(again[:, :hq], out) and bool((again[:, hq] == 3.0).all())
+
+
+PREFILL = [
+    # dtype, hq, hkv, d, page size, lens, new rows, causal, left padding
+    (torch.bfloat16, 32, 8, 128, 16, [33, 17, 64], [33, 1, 20], True, 0),
+    (torch.bfloat16, 32, 8, 128, 16, [300], [5], True, 0),
+    (torch.float16, 32, 8, 128, 16, [700, 40, 0], [3, 4, 0], True, 3),
+    (torch.float16, 8, 2, 128, 16, [100, 260], [100, 130], True, 0),
+    (torch.bfloat16, 8, 8, 128, 16, [65, 10], [60, 10], False, 1),
+    (torch.bfloat16, 4, 2, 64, 16, [50, 31], [50, 2], True, 0),
+    (torch.float16, 16, 2, 64, 16, [129], [100], True, 2),
+    (torch.float16, 12, 2, 128, 16, [40], [12], True, 0),
+    (torch.bfloat16, 34, 2, 128, 16, [20], [6], True, 0),
+    (torch.float32, 4, 2, 64, 16, [32, 20], [32, 1], True, 0),
+    (torch.bfloat16, 6, 3, 96, 5, [12, 6], [5, 6], True, 1),
+]
+
+
+@pytest.mark.parametrize("dt,hq,hkv,d,ps,lens,counts,causal,left", PREFILL)
+def test_prefill_is_the_definition(dt, hq, hkv, d, ps, lens, counts, causal, left):
+    pages = sum(-(-n // ps) for n in lens) + 3
+    tables = U.page_lists(lens, ps, pages, 21)
+    cache = U.random_cache(pages, hkv, ps, d, DEV, 22)
+    for t, n in zip(tables, lens):
+        if n % ps:
+            for pool in cache[:2]:
+                pool.view(torch.uint8)[int(t[-1]), :, n % ps:] = 0x7F
+    width = max(counts) + left
+    row_start = ([b * width + width - c for b, c in enumerate(counts)] if left
+                 else [int(x) for x in np.cumsum([0] + counts)[:-1]])
+    nrows = len(lens) * width if left else sum(counts)
+    q = U.rows((nrows, hq, d), dt, 23).to(DEV)
+    out = torch.full_like(q, 5.0)
+    sm = 1 / math.sqrt(d)
+    plan = U.csr(tables, lens, ps, DEV, spare=1)
+    qo = torch.tensor(np.cumsum([0] + counts), dtype=torch.int32, device=DEV)
+    rs = torch.tensor(row_start, dtype=torch.int32, device=DEV) if left else None
+    ops.paged_prefill_kv8(q, qo, max(counts), *cache, *plan, sm, causal=causal, q_row_start=rs, out=out)
+    _check_attention(out, q, cache, tables, lens, counts, row_start, sm, _p_half(dt), causal)
+    real = torch.zeros(nrows, dtype=torch.bool)
+    for s, c in zip(row_start, counts):
+        real[s:s + c] = True
+    assert bool((out[~real.to(DEV)] == 5.0).all())
+
+
+@pytest.mark.parametrize("dt,d", [(torch.bfloat16, 128), (torch.float16, 64), (torch.float32, 64)])
+def test_prefill_rows_that_see_nothing_are_zeros(dt, d):
+    """More rows than positions (row i sits at kv_len - qo_len + i < 0), and rows of a
+    sequence without pages."""
+    hq, hkv, ps = 8, 2, 16
+    cache = U.random_cache(8, hkv, ps, d, DEV, 2)
+    lens, counts = [3, 0, 20], [5, 4, 2]
+    tables = U.page_lists(lens, ps, 8, 1)
+    q = U.rows((sum(counts), hq, d), dt, 3).to(DEV)
+    qo = torch.tensor(np.cumsum([0] + counts), dtype=torch.int32, device=DEV)
+    out = torch.full_like(q, 5.0)
+    sm = 1 / math.sqrt(d)
+    ops.paged_prefill_kv8(q, qo, 5, *cache, *U.csr(tables, lens, ps, DEV), sm, out=out)
+    _check_attention(out, q, cache, tables, lens, counts, [0, 5, 9], sm, _p_half(dt))
+    assert bool((out[:2] == 0).all()) and bool((out[5:9] == 0).all())
+
+
+def test_attention_bad_pages_are_reported():
+    hq, hkv, d = 8, 2, 128
+    for dt in (torch.bfloat16, torch.float32):
+        cache = U.random_cache(4, hkv, 16, d, DEV, 2)
+        q = U.rows((3, hq, d), dt, 3).to(DEV)
+        ptr, idx, lpl = U.csr([np.array([1, 99], np.int32)], [20], 16, DEV)
+        ops.paged_decode_kv8(q[:1], *cache, ptr, idx, lpl, 0.1)
+        with pytest.raises(RuntimeError, match="page id"):
+            ops.check_device_status(DEV)
+        qo = torch.tensor([0, 3], dtype=torch.int32, device=DEV)
+        ops.paged_prefill_kv8(q, qo, 3, *cache, ptr, idx, lpl, 0.1)
+        with pytest.raises(RuntimeError, match="page id"):
+            ops.check_device_status(DEV)
+        ops.kv8_gather(*cache, ptr, idx, lpl, dt)
+        with pytest.raises(RuntimeError, match="page id"):
+            ops.check_device_status(DEV)
+
+
+def test_a_block_that_is_not_finite_reads_as_nan():
+    hq, hkv, d = 8, 2, 128
+    for dt in (torch.bfloat16, torch.float32):
+        cache = U.random_cache(4, hkv, 16, d, DEV, 2)
+        plan = U.csr([np.array([1, 2], np.int32)], [30], 16, DEV)
+        q = U.rows((1, hq, d), dt, 3).to(DEV)
+        for i in (2, 3):
+            keep = cache[i][2, 1].clone()
+            cache[i][2, 1] = math.nan
+            out = ops.paged_decode_kv8(q, *cache, *plan, 0.1)
+            assert bool(torch.isnan(out[0, 4:]).all()) and bool(torch.isfinite(out[0, :4]).all())
+            cache[i][2, 1] = keep

@@ -1,0 +1,151 @@
+"""The 8-bit cache without a GPU: the oracle's rounding and scales, and what the entry
+points refuse."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from nanoslg_b200 import _native as N
+from nanoslg_b200 import build, ops
+from oracle import kv8
+
+
+@pytest.fixture(scope="module")
+def lib():
+    build.build()
+    return N.lib()
+
+
+def test_oracle_rounding_is_e4m3():
+    every = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).double().numpy()
+    finite = np.sort(every[np.isfinite(every)])
+    np.testing.assert_array_equal(kv8.e4m3(finite), finite)
+    # neighbours' middles: a tie goes to the even code, anything off it to the nearer one
+    lo, hi = finite[:-1], finite[1:]
+    mid = (lo + hi) / 2
+    want = torch.from_numpy(mid).to(torch.float8_e4m3fn).double().numpy()
+    np.testing.assert_array_equal(kv8.e4m3(mid), want)
+    np.testing.assert_array_equal(np.abs(kv8.e4m3(np.nextafter(mid, hi)) - hi).max(), 0)
+    np.testing.assert_array_equal(np.abs(kv8.e4m3(np.nextafter(mid, lo)) - lo).max(), 0)
+
+
+@pytest.mark.parametrize("amax,scale", [(0.0, 0.0), (448.0, 1.0), (448.0001, 2.0), (224.0, 0.5),
+                                        (1.0, 2.0 ** -8), (1.75, 2.0 ** -8), (1.7501, 2.0 ** -7),
+                                        (3.4e38, 2.0 ** 120), (1e-45, 2.0 ** -126),
+                                        (math.inf, math.nan), (math.nan, math.nan)])
+def test_oracle_scale(amax, scale):
+    got = kv8.scale_of(amax)
+    assert (math.isnan(got) and math.isnan(scale)) or got == scale
+
+
+def test_oracle_append_does_not_depend_on_the_cut_but_for_subnormals():
+    rng = np.random.default_rng(0)
+    k = rng.standard_normal((40, 2, 32)) * np.exp2(rng.integers(-1, 2, (40, 2, 1)))
+    whole, single = (kv8.Cache(4, 2, 16, 32) for _ in range(2))
+    whole.append([3, 1, 2], 0, k, k)
+    for t in range(40):
+        single.append([3, 1, 2], t, k[t:t + 1], k[t:t + 1])
+    np.testing.assert_array_equal(whole.s["k"], single.s["k"])
+    a, b = whole.read([3, 1, 2], 40, "k"), single.read([3, 1, 2], 40, "k")
+    s = np.repeat(whole.s["k"][[3, 1, 2]], 16, 0)[:40, :, None]
+    normal = np.abs(k) >= s * 2.0 ** -6
+    np.testing.assert_array_equal(a[normal], b[normal])
+    assert (np.abs(a - b) <= s * 2.0 ** -9)[~normal].all()
+
+
+def _attend(lib, dtype=N.DTYPE_BF16, batch=1, hq=8, hkv=2, d=128, ps=16, q=16, qs=1024, out=16,
+            pool=16, scale=16, pages=4, plan=16, sm=0.1, name="nslg_paged_decode_kv8"):
+    vp = ctypes.c_void_p
+    return lib.nslg_paged_decode_kv8(dtype, batch, hq, hkv, d, ps, vp(q), qs, vp(out), qs, vp(pool),
+                                     vp(pool), vp(scale), vp(scale), pages, vp(plan), vp(plan),
+                                     vp(plan), sm, None, 0, None, None)
+
+
+@pytest.mark.parametrize("bad,what", [
+    (dict(dtype=7), b"dtype"), (dict(batch=-1), b"batch"), (dict(hkv=0), b"num_kv_heads"),
+    (dict(hq=9), b"num_qo_heads"), (dict(d=40), b"head_dim"), (dict(d=288), b"head_dim"),
+    (dict(ps=0), b"page_size"), (dict(pages=0), b"num_pages"), (dict(pool=0), b"null cache"),
+    (dict(scale=0), b"null cache"), (dict(plan=0), b"page list"), (dict(pool=24), b"aligned"),
+    (dict(q=0), b"null"), (dict(out=0), b"null"), (dict(q=18), b"aligned"), (dict(qs=1020), b"stride"),
+    (dict(qs=512), b"stride"), (dict(sm=0.0), b"sm_scale"), (dict(sm=math.nan), b"sm_scale")])
+def test_attention_refusals(lib, bad, what):
+    assert _attend(lib, **bad) in (N.ERR_ARG, N.ERR_UNSUPPORTED)
+    assert what in lib.nslg_last_error()
+
+
+def test_empty_calls_do_nothing(lib):
+    assert _attend(lib, batch=0, q=0, out=0, pool=0) == N.OK
+    z = [None] * 2
+    assert lib.nslg_kv8_gather(N.DTYPE_F32, 0, 2, 64, 16, *z, *z, 4, *z, None, 8, *z, None, None) == N.OK
+    assert lib.nslg_rope_kv8_append(N.DTYPE_F32, 1, 2, 2, 64, 16, None, 0, None, 0, None, 0, 0, None,
+                                    None, None, 0, None, None, None, None, 4, None, None, 0, None,
+                                    None, None, None, None) == N.OK
+
+
+@pytest.mark.parametrize("bad,what", [
+    (dict(cos=0), b"cos and sin"), (dict(rows=0), b"cos and sin"), (dict(k=0), b"null"),
+    (dict(q=0), b"q_out given without q"), (dict(qo=0), b"null"), (dict(most=-1), b"max_qo_len"),
+    (dict(ks=100), b"k rows"), (dict(v=8), b"v rows"), (dict(cos=20), b"tables")])
+def test_append_refusals(lib, bad, what):
+    a = dict(q=16, k=16, v=16, ks=256, cos=16, rows=5, qo=16, most=4) | bad
+    vp = ctypes.c_void_p
+    rc = lib.nslg_rope_kv8_append(N.DTYPE_BF16, 1, 8, 2, 128, 16, vp(a["q"]), 1024, vp(a["k"]), a["ks"],
+                                  vp(a["v"]), 256, 4, vp(16), vp(a["cos"]), vp(16), a["rows"], vp(16),
+                                  vp(16), vp(16), vp(16), 4, vp(a["qo"]), None, a["most"], vp(16),
+                                  vp(16), vp(16), None, None)
+    assert rc == N.ERR_ARG and what in lib.nslg_last_error()
+
+
+def test_gather_and_prefill_refusals(lib):
+    vp = ctypes.c_void_p
+    p = vp(16)
+    rc = lib.nslg_kv8_gather(N.DTYPE_BF16, 1, 2, 128, 16, p, p, p, p, 4, p, p, p, 8, None, p, None, None)
+    assert rc == N.ERR_ARG and b"null" in lib.nslg_last_error()
+    rc = lib.nslg_kv8_gather(N.DTYPE_BF16, 1, 2, 128, 16, p, p, p, p, 4, p, p, p, -1, p, p, None, None)
+    assert rc == N.ERR_ARG and b"num_indices" in lib.nslg_last_error()
+    rc = lib.nslg_paged_prefill_kv8(N.DTYPE_BF16, 1, 8, 2, 128, 16, p, 1024, 0, p, 1024, p, None, 4, p,
+                                    p, p, p, 4, p, p, p, 8, 0.1, 1, None, 0, None, None)
+    assert rc == N.ERR_ARG and b"q_rows" in lib.nslg_last_error()
+    rc = lib.nslg_paged_prefill_kv8(N.DTYPE_BF16, 1, 8, 2, 128, 16, p, 1024, 4, p, 1024, None, None, 4,
+                                    p, p, p, p, 4, p, p, p, 8, 0.1, 1, None, 0, None, None)
+    assert rc == N.ERR_ARG and b"null" in lib.nslg_last_error()
+
+
+def test_ops_refuse_cpu_tensors_and_wrong_layouts():
+    pool = ops.kv8_pages(4, 16, 2, 64, "cpu")
+    assert pool[0].shape == (4, 2, 16, 64) and pool[2].shape == (4, 2)
+    i = torch.zeros(2, dtype=torch.int32)
+    q = torch.zeros(1, 4, 64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.paged_decode_kv8(q, *pool, i, i, i, 0.1)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.paged_prefill_kv8(q, i, 1, *pool, i, i, i, 0.1)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.kv8_gather(*pool, i, i, i, torch.bfloat16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.rope_kv8_append(None, q, q, None, None, *pool, i, 1, i, i, i, rotate=False)
+    cpu = torch.device("cpu")
+
+    def check(a=pool[0], b=pool[1], c=pool[2], d=pool[3], ptr=i, idx=i, lpl=i):
+        return ops._kv8_cache(cpu, a, b, c, d, ptr, idx, lpl)
+    assert check() == (4, 2, 16, 64, 1)
+    with pytest.raises(TypeError, match="float8"):
+        check(a=pool[0].float())
+    with pytest.raises(ValueError, match="alike"):
+        check(b=pool[1][:3])
+    with pytest.raises(ValueError, match="contiguous"):
+        check(a=pool[0].transpose(2, 3), b=pool[1].transpose(2, 3))
+    with pytest.raises(ValueError, match="scales"):
+        check(c=pool[2].double())
+    with pytest.raises(ValueError, match="scales"):
+        check(d=pool[3][:, :1])
+    with pytest.raises(ValueError, match="int32"):
+        check(idx=i.long())
+    with pytest.raises(ValueError, match="entries"):
+        check(ptr=torch.zeros(4, dtype=torch.int32))
+    with pytest.raises(ValueError, match="kv heads"):
+        ops._kv8_rows(torch.zeros(1, 3, 64), "q", 2, 64)
+    with pytest.raises(ValueError, match="kv heads"):
+        ops._kv8_rows(torch.zeros(1, 4, 32), "q", 2, 64)
