@@ -115,59 +115,102 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8App
     uint8_t* codes = static_cast<uint8_t*>(kv == 0 ? p.codes_k : p.codes_v) +
                      blk * p.page_size * d;
     if (tid == 0) (kv == 0 ? p.scale_k : p.scale_v)[blk] = now[kv];
+    // a block that is not finite: every code 0, its NaN is the scale
+    const bool nan = now[kv] != now[kv];
     if (older > 0 && !(now[kv] == was[kv])) {
       const float ratio = was[kv] * scale_inverse(now[kv]);
       uint16_t* c2 = reinterpret_cast<uint16_t*>(codes);
-      for (int i = tid; i < older * d / 2; i += kAppendThreads) c2[i] = e4m3x2_rescale(c2[i], ratio);
+      for (int i = tid; i < older * d / 2; i += kAppendThreads) c2[i] = nan ? 0 : e4m3x2_rescale(c2[i], ratio);
     }
     const float inv = scale_inverse(now[kv]);
     uint16_t* dst = reinterpret_cast<uint16_t*>(codes + static_cast<int64_t>(older) * d);
     for (int i = tid; i < nt * d / 2; i += kAppendThreads) {
       const int t = i / (d / 2), e = i % (d / 2) * 2;
-      dst[i] = e4m3x2_from_f32(value(kv, t, e) * inv, value(kv, t, e + 1) * inv);
+      dst[i] = nan ? 0 : e4m3x2_from_f32(value(kv, t, e) * inv, value(kv, t, e + 1) * inv);
     }
   }
 }
 
 // Reading back: one block per listed page, [page_size, hkv, d] values of type T in list
 // order; slots behind the sequence's last token are zeros. Rows of pages behind the last
-// listed one are left as they are.
+// listed one are left as they are. A thread takes 16 codes of one head row: 16-byte loads,
+// 16-byte stores, consecutive threads along the output. Bound by its bytes (one read and two
+// or four written per element).
+//
+// kStage: the pages staged for the 16-bit prefill kernel, which reads them through an
+// identity page list (`ids`). There the value of a masked position still meets a probability
+// of 0 in a product, so the NaN of a V block is moved to its K block, whose scores are masked
+// by selection; and rows that see no position, which that kernel does not visit, are zeroed.
 constexpr int kGatherThreads = 256;
 
 template <typename T>
+__device__ __forceinline__ void store16(T* dst, const uint4& c, float sc) {
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  constexpr int kPer = 16 / sizeof(T);           // elements per 16-byte store
+  alignas(16) T v[16];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 f = f32x2_from_e4m3x2(static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1))));
+    v[2 * i] = from_cache<T>(f.x * sc);
+    v[2 * i + 1] = from_cache<T>(f.y * sc);
+  }
+#pragma unroll
+  for (int i = 0; i < 16; i += kPer)
+    *reinterpret_cast<uint4*>(dst + i) = *reinterpret_cast<const uint4*>(v + i);
+}
+
+template <typename T, bool kStage>
 __global__ void __launch_bounds__(kGatherThreads) kv8_gather_kernel(const Kv8GatherParams p) {
   pdl_wait();
   pdl_trigger();
   __shared__ int s_fill;
   const int64_t j = blockIdx.x;
   const int tid = threadIdx.x;
+  if constexpr (kStage) {
+    for (int64_t b = j; b < p.batch; b += gridDim.x) {
+      const int q0 = p.qo_indptr[b], len = p.qo_indptr[b + 1] - q0;
+      const int np = p.kv_indptr[b + 1] - p.kv_indptr[b];
+      const int kv_len = np > 0 ? (np - 1) * p.page_size + p.kv_lpl[b] : 0;
+      const int none = kv_len == 0 ? len : p.causal ? len - kv_len : 0;
+      const int64_t row0 = p.q_row_start != nullptr ? p.q_row_start[b] : q0;
+      if (none <= 0 || len > p.max_qo_len || row0 < 0 || row0 + len > p.num_rows) continue;
+      const int words = p.hq * p.d * static_cast<int>(sizeof(T)) / 16;
+      for (int64_t i = tid; i < static_cast<int64_t>(none) * words; i += kGatherThreads)
+        reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (row0 + i / words) * p.out_stride)[i % words] =
+            make_uint4(0u, 0u, 0u, 0u);
+    }
+    if (tid == 0) p.ids[j] = static_cast<int32_t>(j);
+  }
   if (j >= p.kv_indptr[p.batch]) return;
-  for (int b = tid; b < p.batch; b += kGatherThreads)
-    if (p.kv_indptr[b] <= j && j < p.kv_indptr[b + 1])
-      s_fill = j == p.kv_indptr[b + 1] - 1 ? p.kv_lpl[b] : p.page_size;
+  const int64_t page = p.kv_indices[j];
+  for (int b = tid; b < p.batch; b += kGatherThreads) {
+    const int lo = p.kv_indptr[b], hi = p.kv_indptr[b + 1];
+    if (lo <= j && j < hi) s_fill = j == hi - 1 ? p.kv_lpl[b] : p.page_size;
+  }
   __syncthreads();
   const int fill = s_fill;
-  int64_t page = p.kv_indices[j];
   const bool bad = page < 0 || page >= p.num_pages;
   if (bad && tid == 0) report(p.status, NSLG_DEV_BAD_PAGE);
-  const int d2 = p.d / 2, per_head = p.page_size * d2, n = p.hkv * per_head;
+  const int chunks = p.d / 16, per_slot = p.hkv * chunks, n = p.page_size * per_slot;
+  const int64_t blk0 = page * p.hkv;
   for (int i = tid; i < n; i += kGatherThreads) {
-    const int h = i / per_head, s = i % per_head / d2, e = i % d2;
-    const int64_t dst = ((j * p.page_size + s) * p.hkv + h) * p.d + 2 * e;
-    for (int kv = 0; kv < 2; ++kv) {
-      float2 v = make_float2(0.f, 0.f);
-      if (!bad && s < fill) {
-        const int64_t blk = page * p.hkv + h;
-        const float sc = (kv == 0 ? p.scale_k : p.scale_v)[blk];
-        v = f32x2_from_e4m3x2(static_cast<const uint16_t*>(kv == 0 ? p.codes_k : p.codes_v)
-                                  [(blk * p.page_size + s) * d2 + e]);
-        v.x *= sc;
-        v.y *= sc;
+    const int s = i / per_slot, r = i - s * per_slot, h = r / chunks, c = r - h * chunks;
+    uint4 ck = make_uint4(0u, 0u, 0u, 0u), cv = ck;
+    float sk = 0.f, sv = 0.f;
+    if (!bad && s < fill) {
+      const int64_t off = ((blk0 + h) * p.page_size + s) * p.d + c * 16;
+      ck = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.codes_k) + off);
+      cv = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.codes_v) + off);
+      sk = p.scale_k[blk0 + h];
+      sv = p.scale_v[blk0 + h];
+      if (kStage && sv != sv) {
+        sk = sv;
+        sv = 0.f;
       }
-      T* out = static_cast<T*>(kv == 0 ? p.out_k : p.out_v) + dst;
-      out[0] = from_cache<T>(v.x);
-      out[1] = from_cache<T>(v.y);
     }
+    const int64_t dst = (j * n + i) * 16;
+    store16(static_cast<T*>(p.out_k) + dst, ck, sk);
+    store16(static_cast<T*>(p.out_v) + dst, cv, sv);
   }
 }
 
@@ -189,10 +232,17 @@ int launch_kv8_append(int dtype, const Kv8AppendParams& p, cudaStream_t stream) 
 int launch_kv8_gather(int dtype, const Kv8GatherParams& p, cudaStream_t stream) {
   const dim3 grid(static_cast<unsigned>(p.num_indices)), block(kGatherThreads);
   if (dtype == NSLG_DTYPE_BF16)
-    return launch_pdl("kv8_gather", kv8_gather_kernel<__nv_bfloat16>, grid, block, 0, stream, p);
+    return launch_pdl("kv8_gather", kv8_gather_kernel<__nv_bfloat16, false>, grid, block, 0, stream, p);
   if (dtype == NSLG_DTYPE_F16)
-    return launch_pdl("kv8_gather", kv8_gather_kernel<__half>, grid, block, 0, stream, p);
-  return launch_pdl("kv8_gather", kv8_gather_kernel<float>, grid, block, 0, stream, p);
+    return launch_pdl("kv8_gather", kv8_gather_kernel<__half, false>, grid, block, 0, stream, p);
+  return launch_pdl("kv8_gather", kv8_gather_kernel<float, false>, grid, block, 0, stream, p);
+}
+
+int launch_kv8_stage(int dtype, const Kv8GatherParams& p, cudaStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(p.num_indices)), block(kGatherThreads);
+  if (dtype == NSLG_DTYPE_BF16)
+    return launch_pdl("kv8_stage", kv8_gather_kernel<__nv_bfloat16, true>, grid, block, 0, stream, p);
+  return launch_pdl("kv8_stage", kv8_gather_kernel<__half, true>, grid, block, 0, stream, p);
 }
 
 }  // namespace nslg

@@ -1,0 +1,707 @@
+// Split-KV attention over the 8-bit paged cache for decode steps and for a few new rows on
+// a long context: page_size 16, head_dim 64 or 128, 16-bit activations, any head counts.
+//
+// What bounds it: the bytes of the cache, one per element, read once. So every SM streams
+// an equal share of them whatever the sequences' lengths, and the arithmetic per byte is
+// kept below what an SM can issue in the time its share of the bandwidth takes.
+//
+// Work split. A unit is one page of one kv head: 16 tokens, K and V blocks of 16 * head_dim
+// bytes each, contiguous, with one scale each. A "virtual sequence" is (sequence, kv head,
+// tile of 16 query rows), its rows being the (new token, query head of the group) pairs that
+// read this kv head. The units of all virtual sequences form one flat list (U = pages x kv
+// heads x tiles), and CTA c of n takes [U c / n, U (c + 1) / n), each of its 8 warps an equal
+// contiguous part of that, n = min(#SMs, U / 8). It is computed on the device from kv_indptr:
+// no host-side plan, replayable in a CUDA graph. Splitting by kv head (not only by pages)
+// spreads one short sequence over as many warps as it has units, and keeps a partial to one
+// group's rows, so a batch costs about one partial per CTA boundary.
+//
+// A warp is a pipeline of its own: lane i & 31 holds the page id and the scales of unit i,
+// issues the two TMA loads (2 KiB each at head_dim 128, 128-byte swizzle, no multicast) into
+// one of the warp's `stages` slots, and refills a slot as soon as the warp has read it, so
+// there is no producer warp and no barrier between warps before the end.
+//
+// Mathematics of a unit, for the 16 rows of the tile:
+//   x = (q . code_k) * (scale_k * sm_scale * log2 e)      two m16n8 tiles, mma f16 -> fp32
+//   p = 2^(x - m)        m: running reference, raised only when x passes it by 8 (p <= 2^8)
+//   o = o + scale_v * (p . code_v);  l = l + sum p
+// Codes become f16 exactly (one cvt per two). q of bf16 becomes f16 exactly too: each row is
+// first multiplied by the power of two that brings its largest magnitude to [2^14, 2^15)
+// (elements 2^-38 below it vanish). p is rounded to f16, 2^-11 relative, whatever the
+// activation type. The products of a page are scaled as fp32 sums, so the scales of
+// neighbouring pages may differ by any factor.
+// Operand layouts: the order of head_dim inside a k step of q.K is free as long as q and K
+// agree, so K fragments are plain ldmatrix words (4 codes = dims 4t .. 4t + 3 of a 16-dim
+// chunk) and q is loaded to match. V's columns come from ldmatrix.trans of 16-bit units (two
+// dims of one token); one byte permute pairs the tokens, and the two products of a chunk
+// hold its even and its odd dims.
+// A block whose scale is NaN reads as NaN: its NaN is put on the scores (masked like them),
+// so a row that sees nothing of the block is not touched. Codes behind a sequence's last
+// token may be anything, NaN codes too: they are cleared in V and masked in the scores.
+//
+// Joining. A virtual sequence inside one warp's part is written straight to `out`. Pieces of
+// the warps of one CTA meet in shared memory. One that spans CTAs leaves a partial (o, m, l)
+// per CTA in the workspace; the CTA that arrives last, by a count per first CTA, joins them in
+// CTA order and puts the count back to zero. No CTA waits for another, and the sums do not
+// depend on who is last.
+#include <cuda.h>
+
+#include <string>
+
+#include "kv8.cuh"
+#include "launch.h"
+
+namespace nslg {
+namespace {
+
+constexpr int kPS = 16;
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+constexpr int kMaxStages = 8;
+constexpr int kMaxSmem = 232448;      // 227 KiB
+constexpr int kSmemBatch = 2048;      // batches up to this size keep the page list's bounds in smem
+constexpr float kHeadroom = 8.f;      // log2 of the largest probability before m is raised
+
+struct TcParams : Kv8AttnParams {
+  float* part_o;        // [2 * grid][rows][D]
+  float* part_ml;       // [2 * grid][rows][2]
+  uint32_t* arrive;     // [grid]
+  int group, tiles, rows, stages, grid, smem_csr;
+  float scale_log2;
+};
+
+// Rows of one virtual sequence's tile in q and out, and what they see.
+struct Tile {
+  int b, h, r0;           // sequence, kv head, first (token, head) pair of the tile
+  int qo_len, kv_len;
+  int64_t row0;           // row of the sequence's first new token
+};
+
+__device__ __forceinline__ int cta_of(int64_t u, int64_t total, int n) {
+  return static_cast<int>((static_cast<int64_t>(n) * (u + 1) - 1) / total);
+}
+
+// The sequence that holds flat page x.
+__device__ __forceinline__ int seq_of(const int32_t* indptr, int batch, int64_t x) {
+  int lo = 1, hi = batch;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (indptr[mid] > x) hi = mid; else lo = mid + 1;
+  }
+  return lo - 1;
+}
+
+// New rows of sequence b (0 where the plan does not fit the row tensors).
+__device__ __forceinline__ int new_rows(const TcParams& p, int b, int64_t* row0) {
+  if (p.qo_indptr == nullptr) {
+    *row0 = b;
+    return 1;
+  }
+  const int q0 = p.qo_indptr[b];
+  const int len = p.qo_indptr[b + 1] - q0;
+  *row0 = p.q_row_start != nullptr ? p.q_row_start[b] : q0;
+  if (len <= 0) return 0;
+  if (len > p.max_qo_len || *row0 < 0 || *row0 + len > p.num_rows) {
+    report(p.status, NSLG_DEV_BAD_PLAN);
+    return 0;
+  }
+  return len;
+}
+
+__device__ __forceinline__ void tma_load_2d(void* dst, const void* tmap, uint64_t* bar, int c0,
+                                            int c1, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      ".L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;" ::"r"(smem_u32(dst)),
+      "l"(tmap), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "l"(policy)
+      : "memory");
+}
+
+// Sequences without pages: their rows are zeros. CTA c takes sequences c, c + grid, ...
+template <typename T>
+__device__ void zero_empty(const TcParams& p, const int32_t* indptr) {
+  const int words = p.hq * p.d / 8;
+  for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+    if (indptr[b] != indptr[b + 1]) continue;
+    int64_t row0;
+    const int len = new_rows(p, b, &row0);
+    for (int i = 0; i < len; ++i) {
+      uint4* o = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (row0 + i) * p.out_stride);
+      for (int e = threadIdx.x; e < words; e += kThreads) o[e] = make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+}
+
+// Byte offset of 16-byte chunk c of token t inside a block's tile: the block is rows of 128
+// bytes (two tokens a row at head_dim 64), TMA's 128-byte swizzle.
+template <int D>
+__device__ __forceinline__ uint32_t tile_offset(int t, int c) {
+  if (D == 128) return t * 128 + ((c ^ (t & 7)) << 4);
+  const int row = t >> 1, cc = (t & 1) * 4 + c;
+  return row * 128 + ((cc ^ (row & 7)) << 4);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_k,
+                       const __grid_constant__ CUtensorMap tmap_v, const TcParams p) {
+  constexpr int KS = D / 16;             // 16-dim chunks: k steps of q.K, column pairs of p.V
+  constexpr int kBlock = kPS * D;        // bytes of one K (or V) block
+  constexpr int kSlot = 2 * kBlock;
+  constexpr int kBoxRows = kBlock / 128;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ int s_vid[2 * kWarps];      // virtual sequence of each warp's head / tail piece
+  __shared__ int s_piece[2 * kWarps + 1], s_group[2 * kWarps + 1];
+  __shared__ int s_ngroups, s_last[2];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int stages = p.stages;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int piece_floats = p.rows * (D + 2);
+  uint8_t* ring = smem + static_cast<size_t>(warp) * stages * kSlot;
+  float* heads = reinterpret_cast<float*>(smem + static_cast<size_t>(kWarps) * stages * kSlot);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(
+      heads + ((static_cast<size_t>(kWarps) * piece_floats + 1) & ~static_cast<size_t>(1)));
+  uint64_t* full = bars + warp * stages;
+
+  const int32_t* indptr = p.kv_indptr;
+  const int32_t* lpl = p.kv_lpl;
+  if (p.smem_csr) {
+    int32_t* s_ip = reinterpret_cast<int32_t*>(bars + kWarps * stages);
+    int32_t* s_lpl = s_ip + p.batch + 1;
+    for (int i = threadIdx.x; i <= p.batch; i += kThreads) s_ip[i] = p.kv_indptr[i];
+    for (int i = threadIdx.x; i < p.batch; i += kThreads) s_lpl[i] = p.kv_lpl[i];
+    indptr = s_ip;
+    lpl = s_lpl;
+  }
+  if (lane < stages) mbar_init(&full[lane], 1);
+  fence_barrier_init();
+  if (threadIdx.x < 2 * kWarps) s_vid[threadIdx.x] = -1;
+  __syncthreads();
+
+  const int hm = p.hkv * p.tiles;        // virtual sequences per sequence
+  const int64_t total = static_cast<int64_t>(indptr[p.batch]) * hm;
+  const int64_t want = (total + kWarps - 1) / kWarps;
+  const int n = static_cast<int>(want < p.grid ? want : p.grid);
+  const int c = blockIdx.x;
+  if (c >= n) {
+    pdl_wait();
+    pdl_trigger();
+    zero_empty<T>(p, indptr);
+    return;
+  }
+  const int64_t u0 = total * c / n, u1 = total * (c + 1) / n;
+  const int64_t ua = u0 + (u1 - u0) * warp / kWarps;
+  const int64_t ub = u0 + (u1 - u0) * (warp + 1) / kWarps;
+  const int units = static_cast<int>(ub - ua);
+
+  // ---- metadata of 32 units at a time, one per lane
+  struct Meta {
+    int page, vid, j;
+    float sk, sv;
+  };
+  auto locate = [&](int i, Meta& m) {    // page list only: may run before the PDL wait
+    m.page = -1;
+    m.vid = -1;
+    m.j = 0;
+    if (i < units) {
+      const int64_t u = ua + i;
+      const int b = seq_of(indptr, p.batch, u / hm);
+      const int first = indptr[b], np = indptr[b + 1] - first;
+      const int64_t loc = u - static_cast<int64_t>(first) * hm;
+      const int vs = static_cast<int>(loc / np);
+      m.vid = b * hm + vs;
+      m.j = static_cast<int>(loc - static_cast<int64_t>(vs) * np);
+      m.page = p.kv_indices[first + m.j];
+      if (m.page < 0 || m.page >= p.num_pages) {
+        report(p.status, NSLG_DEV_BAD_PAGE);
+        m.page = -1;
+      }
+    }
+  };
+  auto head_of = [&](int vid) { return vid % hm / p.tiles; };
+  auto load_scales = [&](Meta& m) {
+    m.sk = m.sv = 0.f;
+    if (m.page >= 0) {
+      const int64_t blk = static_cast<int64_t>(m.page) * p.hkv + head_of(m.vid);
+      m.sk = p.scale_k[blk];
+      m.sv = p.scale_v[blk];
+      if (m.sv != m.sv) {                // NaN rides on the scores
+        m.sk = m.sv;
+        m.sv = 0.f;
+      }
+    }
+  };
+  const uint64_t policy = p.tiles > 1 ? l2_policy_evict_last() : l2_policy_evict_first();
+  auto issue = [&](const Meta& m, int i) {   // by the lane that holds unit i
+    const int s = i % stages;
+    const int page = m.page < 0 ? 0 : m.page;   // a bad page: page 0's codes, scale 0
+    const int row = (page * p.hkv + head_of(m.vid)) * kBoxRows;
+    mbar_arrive_expect_tx(&full[s], kSlot);
+    tma_load_2d(ring + s * kSlot, &tmap_k, &full[s], 0, row, policy);
+    tma_load_2d(ring + s * kSlot + kBlock, &tmap_v, &full[s], 0, row, policy);
+  };
+
+  Meta cur, nxt;
+  locate(lane, nxt);
+  pdl_wait();      // the kernel before may have written q, the codes and the scales
+  pdl_trigger();
+  if (lane < stages && lane < units) issue(nxt, lane);
+  load_scales(nxt);
+  zero_empty<T>(p, indptr);
+
+  const int g = lane >> 2, tq = lane & 3;
+  const int mi = lane >> 3, lr = lane & 7;
+  // ldmatrix row addresses: K matrices (tokens 0-7 | 8-15) x (chunk, chunk + 1)
+  const int ltok = (mi & 1) * 8 + lr, lch = mi >> 1;
+
+  uint32_t qa[KS][4];
+  float o[2 * KS][4];
+  float m0 = -INFINITY, m1 = -INFINITY, nb0 = 0.f, nb1 = 0.f, l0 = 0.f, l1 = 0.f;
+  float f0 = 0.f, f1 = 0.f;              // sm_scale * log2 e / the row's power of two
+  int vid = -1;
+  Tile t{};
+  int pos0 = 0, pos1 = 0;                // last position seen by rows g and g + 8
+  bool ok = true;
+
+  auto begin = [&](int v) {
+    vid = v;
+    t.b = v / hm;
+    const int vs = v % hm;
+    t.h = vs / p.tiles;
+    t.r0 = vs % p.tiles * 16;
+    t.qo_len = new_rows(p, t.b, &t.row0);
+    t.kv_len = (indptr[t.b + 1] - indptr[t.b] - 1) * kPS + lpl[t.b];
+    float sc[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int pair = t.r0 + g + 8 * r;
+      const int tok = pair / p.group;
+      const bool live = g + 8 * r < p.rows && tok < t.qo_len;
+      const T* src = static_cast<const T*>(p.q) + (t.row0 + tok) * p.q_stride +
+                     static_cast<int64_t>(t.h * p.group + pair % p.group) * D + 4 * tq;
+      uint2 raw[KS];
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+        raw[k] = live ? *reinterpret_cast<const uint2*>(src + 16 * k) : make_uint2(0u, 0u);
+      // a row of no sequence sees everything: it is never written, and no page is an edge for it
+      const int lim = !live ? 0x7fffffff : p.causal ? t.kv_len - t.qo_len + tok : t.kv_len - 1;
+      if (r) pos1 = lim; else pos0 = lim;
+      sc[r] = 1.f;
+      if constexpr (Mma16<T>::kFormat == 1) {      // bf16 -> f16 by a power of two
+        uint32_t top = 0u;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          top = max(max(top, (raw[k].x & 0x7FFFu)), (raw[k].x >> 16) & 0x7FFFu);
+          top = max(max(top, (raw[k].y & 0x7FFFu)), (raw[k].y >> 16) & 0x7FFFu);
+        }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // magnitude in [2^(e - 127), 2^(e - 126)): times 2^(141 - e) is in [2^14, 2^15)
+        const int e = static_cast<int>(top >> 7);
+        float up = 1.f;
+        if (e > 14 && e < 255) {       // smaller rows, zeros, infinities and NaN: as they are
+          up = __uint_as_float(static_cast<uint32_t>(min(268 - e, 254)) << 23);
+          sc[r] = 1.f / up;
+        }
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const uint32_t w[2] = {raw[k].x, raw[k].y};
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            qa[k][2 * i + r] = pack_f16x2(__uint_as_float(w[i] << 16) * up,
+                                          __uint_as_float(w[i] & 0xFFFF0000u) * up);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          qa[k][r] = raw[k].x;
+          qa[k][2 + r] = raw[k].y;
+        }
+      }
+    }
+    f0 = p.scale_log2 * sc[0];
+    f1 = p.scale_log2 * sc[1];
+#pragma unroll
+    for (int k = 0; k < 2 * KS; ++k) o[k][0] = o[k][1] = o[k][2] = o[k][3] = 0.f;
+    m0 = m1 = -INFINITY;
+    nb0 = nb1 = l0 = l1 = 0.f;
+  };
+
+  auto seg_begin = [&](int v) {
+    const int b = v / hm;
+    const int first = indptr[b], np = indptr[b + 1] - first;
+    return static_cast<int64_t>(first) * hm + static_cast<int64_t>(v % hm) * np;
+  };
+  auto out_row = [&](int v, int r) -> T* {   // row r of the tile in out, null where there is none
+    const int b = v / hm, vs = v % hm;
+    const int pair = vs % p.tiles * 16 + r, tok = pair / p.group;
+    int64_t row0;
+    if (tok >= new_rows(p, b, &row0)) return nullptr;
+    return static_cast<T*>(p.out) + (row0 + tok) * p.out_stride +
+           static_cast<int64_t>(vs / p.tiles * p.group + pair % p.group) * D;
+  };
+
+  // The warp's state of virtual sequence `vid`, finished: to out, or as a piece.
+  auto finish = [&]() {
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+    const int64_t beg = seg_begin(vid);
+    const int64_t end = beg + (indptr[t.b + 1] - indptr[t.b]);
+    const bool whole = beg >= ua && end <= ub;
+    const bool tail = end > ub;
+    float* piece = tail ? reinterpret_cast<float*>(ring) : heads + warp * piece_floats;
+    if (!whole && lane == 0) s_vid[2 * warp + (tail ? 1 : 0)] = vid;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int row = g + 8 * r;
+      if (row >= p.rows) continue;
+      const float l = r ? l1 : l0;
+      if (whole) {
+        T* dst = out_row(vid, row);
+        if (dst == nullptr) continue;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+          *reinterpret_cast<uint2*>(dst + 16 * k + 4 * tq) =
+              make_uint2(Mma16<T>::pack(o[2 * k][2 * r] * inv, o[2 * k + 1][2 * r] * inv),
+                         Mma16<T>::pack(o[2 * k][2 * r + 1] * inv, o[2 * k + 1][2 * r + 1] * inv));
+      } else {
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+          *reinterpret_cast<float2*>(piece + row * D + 16 * k + 4 * tq) =
+              make_float2(o[2 * k][2 * r], o[2 * k + 1][2 * r]),
+          *reinterpret_cast<float2*>(piece + row * D + 16 * k + 4 * tq + 2) =
+              make_float2(o[2 * k][2 * r + 1], o[2 * k + 1][2 * r + 1]);
+        if (tq == 0) {
+          piece[p.rows * D + 2 * row] = r ? m1 : m0;
+          piece[p.rows * D + 2 * row + 1] = l;
+        }
+      }
+    }
+  };
+
+  int slot = 0;
+  uint32_t phase = 0;
+  for (int base = 0; base < units && ok; base += 32) {
+    cur = nxt;
+    locate(base + 32 + lane, nxt);
+    load_scales(nxt);
+    const int stop = min(32, units - base);
+    for (int i = 0; i < stop; ++i) {
+      const int v = __shfl_sync(0xffffffffu, cur.vid, i);
+      if (v != vid) {
+        if (vid >= 0) finish();
+        begin(v);
+      }
+      const float sk = __shfl_sync(0xffffffffu, cur.sk, i);
+      const float sv = __shfl_sync(0xffffffffu, cur.sv, i);
+      const int tok0 = __shfl_sync(0xffffffffu, cur.j, i) * kPS;
+      ok = __all_sync(0xffffffffu, mbar_wait(&full[slot], phase));
+      if (!ok) {
+        if (lane == 0) report(p.status, NSLG_DEV_WAIT_TIMEOUT);
+        // issue nothing more; wait (bounded) for the loads in flight before leaving
+        for (int k = 1; k < stages; ++k) {
+          const int s = (slot + k) % stages;
+          if (base + i + k < units) (void)mbar_wait(&full[s], s > slot ? phase : phase ^ 1);
+        }
+        break;
+      }
+      const uint32_t kb = smem_u32(ring + slot * kSlot), vb = kb + kBlock;
+      // ---- scores of the page's 16 tokens
+      float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int k = 0; k < KS; k += 2) {
+        uint32_t w[4];
+        ldmatrix_x4(kb + tile_offset<D>(ltok, k + lch), w[0], w[1], w[2], w[3]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          mma_f16_16816(s[e & 1], qa[k + (e >> 1)], f16x2_from_e4m3x2(static_cast<uint16_t>(w[e])),
+                        f16x2_from_e4m3x2(static_cast<uint16_t>(w[e] >> 16)));
+      }
+      const float a0 = f0 * sk, a1 = f1 * sk;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        s[e][0] *= a0;
+        s[e][1] *= a0;
+        s[e][2] *= a1;
+        s[e][3] *= a1;
+      }
+      // a page some row does not see whole, or that ends the sequence
+      const int held = t.kv_len - tok0;
+      const bool edge = !__all_sync(0xffffffffu, min(pos0, pos1) >= tok0 + kPS - 1) || held < kPS;
+      if (edge) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int tok = tok0 + (e >> 1) * 8 + tq * 2 + (e & 1);
+          if (tok > pos0) s[e >> 1][e & 1] = -INFINITY;
+          if (tok > pos1) s[e >> 1][2 + (e & 1)] = -INFINITY;
+        }
+      }
+      // ---- the running reference, raised when a score passes it by kHeadroom
+      float x0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+      float x1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
+      if (__any_sync(0xffffffffu, x0 > m0 + kHeadroom || x1 > m1 + kHeadroom)) {
+        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
+        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
+        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
+        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
+        const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+        const float c0 = n0 == -INFINITY ? 1.f : fast_exp2(m0 - n0);
+        const float c1 = n1 == -INFINITY ? 1.f : fast_exp2(m1 - n1);
+        m0 = n0;
+        m1 = n1;
+        nb0 = n0 == -INFINITY ? 0.f : -n0;
+        nb1 = n1 == -INFINITY ? 0.f : -n1;
+        l0 *= c0;
+        l1 *= c1;
+#pragma unroll
+        for (int k = 0; k < 2 * KS; ++k) {
+          o[k][0] *= c0;
+          o[k][1] *= c0;
+          o[k][2] *= c1;
+          o[k][3] *= c1;
+        }
+      }
+      uint32_t pa[4];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float p0 = fast_exp2(s[e][0] + nb0), p1 = fast_exp2(s[e][1] + nb0);
+        const float p2 = fast_exp2(s[e][2] + nb1), p3 = fast_exp2(s[e][3] + nb1);
+        l0 += p0 + p1;
+        l1 += p2 + p3;
+        pa[2 * e] = pack_f16x2(p0, p1);
+        pa[2 * e + 1] = pack_f16x2(p2, p3);
+      }
+      // ---- o += scale_v * (p . V), two 16-dim chunks a step
+      uint32_t clear[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
+      if (held < kPS) {     // codes behind the last token count as 0
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          clear[e] = (tq * 2 + 8 * e < held ? 0x00FF00FFu : 0u) |
+                     (tq * 2 + 8 * e + 1 < held ? 0xFF00FF00u : 0u);
+      }
+#pragma unroll
+      for (int k = 0; k < KS; k += 2) {
+        uint32_t w[4];
+        ldmatrix_x4_trans(vb + tile_offset<D>(ltok, k + lch), w[0], w[1], w[2], w[3]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = __byte_perm(w[e], 0u, 0x3120) & clear[e & 1];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float even[4] = {0.f, 0.f, 0.f, 0.f}, odd[4] = {0.f, 0.f, 0.f, 0.f};
+          mma_f16_16816(even, pa, f16x2_from_e4m3x2(static_cast<uint16_t>(w[2 * e])),
+                        f16x2_from_e4m3x2(static_cast<uint16_t>(w[2 * e + 1])));
+          mma_f16_16816(odd, pa, f16x2_from_e4m3x2(static_cast<uint16_t>(w[2 * e] >> 16)),
+                        f16x2_from_e4m3x2(static_cast<uint16_t>(w[2 * e + 1] >> 16)));
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            o[2 * (k + e)][x] = fmaf(even[x], sv, o[2 * (k + e)][x]);
+            o[2 * (k + e) + 1][x] = fmaf(odd[x], sv, o[2 * (k + e) + 1][x]);
+          }
+        }
+      }
+      __syncwarp();        // the slot has been read by every lane
+      const int ahead = i + stages;
+      if (base + ahead < units && lane == (ahead & 31)) issue(ahead < 32 ? cur : nxt, base + ahead);
+      if (++slot == stages) {
+        slot = 0;
+        phase ^= 1;
+      }
+    }
+  }
+  // after a wait that gave up: the pieces are garbage (the status says so), but the joining
+  // below keeps its control flow, so the counts return to zero
+  if (vid >= 0) finish();
+  __syncthreads();
+
+  // ---- the pieces of this CTA, in unit order, grouped by virtual sequence
+  if (warp == 0) {
+    const int v = lane < 2 * kWarps ? s_vid[lane] : -1;
+    const uint32_t have = __ballot_sync(0xffffffffu, v >= 0);
+    const int at = __popc(have & ((1u << lane) - 1u));
+    if (v >= 0) s_piece[at] = lane;
+    __syncwarp();
+    const int cnt = __popc(have);
+    const bool starts = lane < cnt && (lane == 0 || s_vid[s_piece[lane]] != s_vid[s_piece[lane - 1]]);
+    const uint32_t st = __ballot_sync(0xffffffffu, starts);
+    if (starts) s_group[__popc(st & ((1u << lane) - 1u))] = lane;
+    if (lane == 0) {
+      s_group[__popc(st)] = cnt;
+      s_ngroups = __popc(st);
+      s_last[0] = s_last[1] = 0;
+    }
+  }
+  __syncthreads();
+  const int ngroups = s_ngroups;
+  if (ngroups == 0) return;
+  constexpr int DQ = D / 4;
+  auto piece_at = [&](int k) -> const float* {
+    const int id = s_piece[k], w = id >> 1;
+    return (id & 1) ? reinterpret_cast<const float*>(smem + static_cast<size_t>(w) * stages * kSlot)
+                    : heads + w * piece_floats;
+  };
+  for (int e = threadIdx.x; e < ngroups * p.rows * DQ; e += kThreads) {
+    const int gr = e / (p.rows * DQ), row = e / DQ % p.rows, dq = e % DQ;
+    const int k0 = s_group[gr], k1 = s_group[gr + 1];
+    float m = -INFINITY;
+    for (int k = k0; k < k1; ++k) m = fmaxf(m, piece_at(k)[p.rows * D + 2 * row]);
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = k0; k < k1; ++k) {
+      const float* pc = piece_at(k);
+      const float w = fast_exp2(pc[p.rows * D + 2 * row] - base);
+      const float2 a = *reinterpret_cast<const float2*>(pc + row * D + 4 * dq);
+      const float2 b = *reinterpret_cast<const float2*>(pc + row * D + 4 * dq + 2);
+      l = fmaf(w, pc[p.rows * D + 2 * row + 1], l);
+      acc.x = fmaf(w, a.x, acc.x);
+      acc.y = fmaf(w, a.y, acc.y);
+      acc.z = fmaf(w, b.x, acc.z);
+      acc.w = fmaf(w, b.y, acc.w);
+    }
+    const int v = s_vid[s_piece[k0]];
+    const int64_t beg = seg_begin(v);
+    const int b = v / hm;
+    const int64_t end = beg + (indptr[b + 1] - indptr[b]);
+    if (beg >= u0 && end <= u1) {
+      T* dst = out_row(v, row);
+      if (dst == nullptr) continue;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      *reinterpret_cast<uint2*>(dst + 4 * dq) = make_uint2(
+          Mma16<T>::pack(acc.x * inv, acc.y * inv), Mma16<T>::pack(acc.z * inv, acc.w * inv));
+    } else {
+      const int64_t r = (2ll * c + (beg >= u0 ? 1 : 0)) * p.rows + row;
+      *reinterpret_cast<float4*>(p.part_o + r * D + 4 * dq) = acc;
+      if (dq == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * r) = make_float2(m, l);
+    }
+  }
+  __syncthreads();
+
+  // ---- virtual sequences that span CTAs: the first and the last group can be one
+  int jv[2], cf[2], cnt[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int v = s_vid[s_piece[k == 0 ? 0 : s_group[ngroups - 1]]];
+    const int64_t beg = seg_begin(v);
+    const int64_t end = beg + (indptr[v / hm + 1] - indptr[v / hm]);
+    // k == 0: one that began before this CTA; k == 1: one that begins here and goes on
+    const bool joins = k == 0 ? beg < u0 : (beg >= u0 && end > u1);
+    jv[k] = joins ? v : -1;
+    cf[k] = joins ? cta_of(beg, total, n) : 0;
+    cnt[k] = joins ? cta_of(end - 1, total, n) - cf[k] + 1 : 0;
+    if (joins && threadIdx.x == 32 * k) {
+      const uint32_t prev = atom_add_acq_rel_u32(&p.arrive[cf[k]], 1u);
+      if (prev + 1u == static_cast<uint32_t>(cnt[k])) {
+        atomicExch(&p.arrive[cf[k]], 0u);
+        s_last[k] = 1;
+      }
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    if (!s_last[k]) continue;
+    for (int e = threadIdx.x; e < p.rows * DQ; e += kThreads) {
+      const int row = e / DQ, dq = e % DQ;
+      // partial i: CTA cf + i, the slot of one that begins there for the first, else of one
+      // that began before
+      auto slot_row = [&](int i) { return (2ll * (cf[k] + i) + (i == 0 ? 1 : 0)) * p.rows + row; };
+      float m = -INFINITY;
+#pragma unroll 8
+      for (int i = 0; i < cnt[k]; ++i) m = fmaxf(m, __ldcg(p.part_ml + 2 * slot_row(i)));
+      const float base = m == -INFINITY ? 0.f : m;
+      float l = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+      for (int i = 0; i < cnt[k]; ++i) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + 2 * slot_row(i)));
+        const float4 a = __ldcg(reinterpret_cast<const float4*>(p.part_o + slot_row(i) * D + 4 * dq));
+        const float w = fast_exp2(ml.x - base);
+        l = fmaf(w, ml.y, l);
+        acc.x = fmaf(w, a.x, acc.x);
+        acc.y = fmaf(w, a.y, acc.y);
+        acc.z = fmaf(w, a.z, acc.z);
+        acc.w = fmaf(w, a.w, acc.w);
+      }
+      T* dst = out_row(jv[k], row);
+      if (dst == nullptr) continue;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      *reinterpret_cast<uint2*>(dst + 4 * dq) = make_uint2(
+          Mma16<T>::pack(acc.x * inv, acc.y * inv), Mma16<T>::pack(acc.z * inv, acc.w * inv));
+    }
+  }
+}
+
+int64_t arrive_bytes(int grid) { return (static_cast<int64_t>(grid) * 4 + 255) / 256 * 256; }
+
+int tile_rows(int group, int max_qo_len) {
+  const int64_t pairs = static_cast<int64_t>(group) * max_qo_len;
+  return pairs < 16 ? static_cast<int>(pairs) : 16;
+}
+
+template <typename T, int D>
+int launch_typed(TcParams p, cudaStream_t stream) {
+  CUtensorMap tk, tv;
+  const uint64_t rows = static_cast<uint64_t>(p.num_pages) * p.hkv * kPS * D / 128;
+  int rc = encode_tiled_2d_bytes(&tk, p.codes_k, 128, rows, kPS * D / 128);
+  if (rc == NSLG_OK) rc = encode_tiled_2d_bytes(&tv, p.codes_v, 128, rows, kPS * D / 128);
+  if (rc != NSLG_OK) return rc;
+  constexpr size_t kSlot = 2 * kPS * D;
+  p.smem_csr = p.batch <= kSmemBatch ? 1 : 0;
+  const size_t heads = (static_cast<size_t>(kWarps) * p.rows * (D + 2) + 1) / 2 * 8;
+  const size_t csr = p.smem_csr ? static_cast<size_t>(2 * p.batch + 1) * 4 : 0;
+  const size_t fixed = 1024 + heads + csr + kWarps * kMaxStages * 8 + 1024;  // + the static arrays
+  int stages = static_cast<int>((kMaxSmem - fixed) / (kWarps * kSlot));
+  if (stages > kMaxStages) stages = kMaxStages;
+  if (stages < 3)      // a warp's tail piece takes three slots of its ring
+    return set_error(NSLG_ERR_UNSUPPORTED, "kv8 attention: no room for the pipeline");
+  p.stages = stages;
+  const size_t smem = 1024 + heads + csr + static_cast<size_t>(kWarps) * stages * (kSlot + 8);
+  auto kern = kv8_attn_tc_kernel<T, D>;
+  const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               static_cast<int>(smem));
+  if (err != cudaSuccess) return set_error(NSLG_ERR_CUDA, cudaGetErrorString(err));
+  return launch_pdl("kv8_attn_tc", kern, dim3(p.grid), dim3(kThreads), smem, stream, tk, tv, p);
+}
+
+}  // namespace
+
+bool kv8_attn_tc_supported(int dtype, const Kv8AttnParams& p) {
+  if (dtype != NSLG_DTYPE_BF16 && dtype != NSLG_DTYPE_F16) return false;
+  if (p.page_size != kPS || (p.d != 64 && p.d != 128)) return false;
+  const int64_t tiles = (static_cast<int64_t>(p.hq / p.hkv) * p.max_qo_len + 15) / 16;
+  // TMA row coordinates and the virtual sequences' numbers are 32-bit
+  return p.num_pages * p.hkv * kPS < (int64_t{1} << 31) &&
+         static_cast<int64_t>(p.batch) * p.hkv * tiles < (int64_t{1} << 31);
+}
+
+int64_t kv8_attn_tc_workspace_bytes(int group, int max_qo_len, int d) {
+  const int grid = sm_count();
+  return arrive_bytes(grid) + 2ll * grid * tile_rows(group, max_qo_len) * (d + 2) * 4 + 256;
+}
+
+int launch_kv8_attention_tc(int dtype, const Kv8AttnParams& a, void* workspace,
+                            int64_t workspace_bytes, cudaStream_t stream) {
+  TcParams p{};
+  static_cast<Kv8AttnParams&>(p) = a;
+  p.group = a.hq / a.hkv;
+  const int64_t need = kv8_attn_tc_workspace_bytes(p.group, a.max_qo_len, a.d);
+  if (workspace == nullptr || workspace_bytes < need)
+    return set_error(NSLG_ERR_WORKSPACE, "kv8 attention: the workspace needs " + std::to_string(need) + " bytes");
+  p.grid = sm_count();
+  p.rows = tile_rows(p.group, a.max_qo_len);
+  p.tiles = static_cast<int>((static_cast<int64_t>(p.group) * a.max_qo_len + 15) / 16);
+  p.scale_log2 = a.sm_scale * 1.4426950408889634f;
+  const uintptr_t ws = (reinterpret_cast<uintptr_t>(workspace) + 255) & ~static_cast<uintptr_t>(255);
+  p.arrive = reinterpret_cast<uint32_t*>(ws);
+  p.part_o = reinterpret_cast<float*>(ws + arrive_bytes(p.grid));
+  p.part_ml = p.part_o + 2ll * p.grid * p.rows * a.d;
+  if (dtype == NSLG_DTYPE_F16)
+    return a.d == 128 ? launch_typed<__half, 128>(p, stream) : launch_typed<__half, 64>(p, stream);
+  return a.d == 128 ? launch_typed<__nv_bfloat16, 128>(p, stream)
+                    : launch_typed<__nv_bfloat16, 64>(p, stream);
+}
+
+}  // namespace nslg

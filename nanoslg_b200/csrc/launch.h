@@ -56,6 +56,11 @@ int encode_tiled_3d_bf16(CUtensorMap* out, const void* base, uint64_t d0, uint64
                          uint64_t d2, uint64_t stride1_bytes, uint64_t stride2_bytes,
                          uint32_t box0, uint32_t box1, uint32_t box2);
 
+// 2-D map of contiguous rows of row_bytes (at most 128) bytes, 128-byte swizzle, boxes of
+// box_rows whole rows.
+int encode_tiled_2d_bytes(CUtensorMap* out, const void* base, uint64_t row_bytes, uint64_t rows,
+                          uint32_t box_rows);
+
 // Cached map of one pool layer [pages, 16, hkv, d] with a [16 tok x 1 head x 64 dim] box.
 int pool_tensor_map(const void* pool, int64_t pages, int hkv, int d, CUtensorMap* out);
 // Same pool with a [16 tok x hkv heads x 64 dim] box landing as [head][token][64] in smem
@@ -197,8 +202,17 @@ struct Kv8GatherParams : Kv8Cache {
   int64_t num_indices;
   int batch, hkv, d, page_size;
   uint32_t* status;
+  // staging for the prefill kernel only: the identity page list, and the rows of `out` that
+  // see no position
+  int32_t* ids;
+  void* out;
+  const int32_t* qo_indptr;
+  const int32_t* q_row_start;
+  int64_t out_stride, num_rows;
+  int hq, max_qo_len, causal;
 };
 int launch_kv8_gather(int dtype, const Kv8GatherParams& p, cudaStream_t stream);
+int launch_kv8_stage(int dtype, const Kv8GatherParams& p, cudaStream_t stream);
 
 struct Kv8AttnParams : Kv8Cache {
   const void* q;
@@ -212,5 +226,11 @@ struct Kv8AttnParams : Kv8Cache {
 };
 // CUDA cores: any page size, head_dim a multiple of 32 up to 256, all three types.
 int launch_kv8_attention_simt(int dtype, const Kv8AttnParams& p, cudaStream_t stream);
+
+// Tensor cores, split over the cache (kv8_attn_tc.cu): decode, and a few rows a sequence.
+bool kv8_attn_tc_supported(int dtype, const Kv8AttnParams& p);
+int64_t kv8_attn_tc_workspace_bytes(int group, int max_qo_len, int d);
+int launch_kv8_attention_tc(int dtype, const Kv8AttnParams& p, void* workspace,
+                            int64_t workspace_bytes, cudaStream_t stream);
 
 }  // namespace nslg

@@ -65,6 +65,23 @@ int encode_tiled_3d_bf16(CUtensorMap* out, const void* base, uint64_t d0, uint64
   return NSLG_OK;
 }
 
+int encode_tiled_2d_bytes(CUtensorMap* out, const void* base, uint64_t row_bytes, uint64_t rows,
+                          uint32_t box_rows) {
+  EncodeTiledFn enc = encode_fn();
+  if (enc == nullptr) return set_error(NSLG_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const cuuint64_t dims[2] = {row_bytes, rows};
+  const cuuint64_t strides[1] = {row_bytes};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(row_bytes), box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims,
+                         strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return set_error(NSLG_ERR_CUDA, "cuTensorMapEncodeTiled failed: " + std::to_string(r));
+  return NSLG_OK;
+}
+
 int cached_pool_map(const void* pool, int64_t pages, int hkv, int d, int all_heads,
                     CUtensorMap* out) {
   std::lock_guard<std::mutex> lock(g_map_mu);

@@ -689,12 +689,15 @@ def paged_prefill_kv8(q, qo_indptr, max_qo_len, pool_k, pool_v, scale_k, scale_v
     if nrows == 0 or batch == 0 or max_qo_len == 0:
         return out
     n = kv_indices.numel()
-    wsb = N.lib().nslg_prefill_kv8_workspace_bytes(dt, batch, hq, hkv, d, ps, int(max_qo_len), n)
-    ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+    lib, stream, most = N.lib(), _stream(q), int(max_qo_len)
+    ws = _STATE.stream_workspace(dev, stream,
+                                 lib.nslg_prefill_kv8_workspace_bytes(hq, hkv, d, most))
+    stb = lib.nslg_prefill_kv8_staging_bytes(dt, hq, hkv, d, ps, most, n)
+    staging = torch.empty(stb, dtype=torch.uint8, device=dev) if stb else None
     _kv8_call(dev, "nslg_paged_prefill_kv8", dt, batch, hq, hkv, d, ps, q.data_ptr(), qs, nrows,
-              out.data_ptr(), os_, qo_indptr.data_ptr(), _ptr(q_row_start), int(max_qo_len),
+              out.data_ptr(), os_, qo_indptr.data_ptr(), _ptr(q_row_start), most,
               pool_k.data_ptr(), pool_v.data_ptr(), scale_k.data_ptr(), scale_v.data_ptr(),
               num_pages, kv_indptr.data_ptr(), kv_indices.data_ptr(),
               kv_last_page_len.data_ptr(), n, float(sm_scale), 1 if causal else 0,
-              ws.data_ptr(), wsb, status_word(dev).data_ptr(), _stream(q))
+              ws.data_ptr(), ws.numel(), _ptr(staging), stb, status_word(dev).data_ptr(), stream)
     return out
