@@ -7,10 +7,10 @@
 //
 // Work split. A unit is one page of one kv head: 16 tokens, K and V blocks of 16 * head_dim
 // bytes each, contiguous, with one scale each. A "virtual sequence" is (sequence, kv head,
-// tile of 16 query rows), its rows being the (new token, query head of the group) pairs that
+// tile of 8 NT query rows), its rows being the (new token, query head of the group) pairs that
 // read this kv head. The units of all virtual sequences form one flat list (U = pages x kv
-// heads x tiles), and CTA c of n takes [U c / n, U (c + 1) / n), each of its 8 warps an equal
-// contiguous part of that, n = min(#SMs, U / 8). It is computed on the device from kv_indptr:
+// heads x tiles), and CTA c of n takes [U c / n, U (c + 1) / n), each of its W warps an
+// equal contiguous part of that, n = min(#SMs, U / W). It is computed on the device from kv_indptr:
 // no host-side plan, replayable in a CUDA graph. Splitting by kv head (not only by pages)
 // spreads one short sequence over as many warps as it has units, and keeps a partial to one
 // group's rows, so a batch costs about one partial per CTA boundary.
@@ -20,20 +20,25 @@
 // one of the warp's `stages` slots, and refills a slot as soon as the warp has read it, so
 // there is no producer warp and no barrier between warps before the end.
 //
-// Mathematics of a unit, for the 16 rows of the tile:
-//   x = (q . code_k) * (scale_k * sm_scale * log2 e)      two m16n8 tiles, mma f16 -> fp32
+// Mathematics of a unit, transposed so that a short group wastes little of an mma: the 16
+// tokens (of K) and 16-dim chunks (of V) are the rows of m16n8k16 products, the query rows
+// their 8 columns (one or two column tiles, NT):
+//   x^T = code_k . q^T  (16 tokens x 8 NT rows), times scale_k * sm_scale * log2 e
 //   p = 2^(x - m)        m: running reference, raised only when x passes it by 8 (p <= 2^8)
-//   o = o + scale_v * (p . code_v);  l = l + sum p
+//   o^T = o^T + scale_v * (code_v^T . p^T);  l = l + sum p
+// Against rows-first products (16 query rows, 4 of them in use at a group of 4) this halves
+// the products, the accumulators (32 registers instead of 64 at head_dim 128, so 16 warps
+// fit an SM instead of 8) and the exponentials.
 // Codes become f16 exactly (one cvt per two). q of bf16 becomes f16 exactly too: each row is
 // first multiplied by the power of two that brings its largest magnitude to [2^14, 2^15)
 // (elements 2^-38 below it vanish). p is rounded to f16, 2^-11 relative, whatever the
 // activation type. The products of a page are scaled as fp32 sums, so the scales of
 // neighbouring pages may differ by any factor.
-// Operand layouts: the order of head_dim inside a k step of q.K is free as long as q and K
+// Operand layouts: the order of head_dim inside a k step of K.q is free as long as q and K
 // agree, so K fragments are plain ldmatrix words (4 codes = dims 4t .. 4t + 3 of a 16-dim
-// chunk) and q is loaded to match. V's columns come from ldmatrix.trans of 16-bit units (two
-// dims of one token); one byte permute pairs the tokens, and the two products of a chunk
-// hold its even and its odd dims.
+// chunk) and q is loaded to match. V^T comes from ldmatrix.trans of 16-bit units (two dims
+// of one token); one byte permute pairs the tokens, and row g / g + 8 of the chunk's product
+// is dim 2g / 2g + 1. p^T is the scores' fragment transposed by movmatrix.
 // A block whose scale is NaN reads as NaN: its NaN is put on the scores (masked like them),
 // so a row that sees nothing of the block is not touched. Codes behind a sequence's last
 // token may be anything, NaN codes too: they are cleared in V and masked in the scores.
@@ -53,9 +58,10 @@
 namespace nslg {
 namespace {
 
+#ifndef NSLG_W1
+#define NSLG_W1 12
+#endif
 constexpr int kPS = 16;
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
 constexpr int kMaxStages = 8;
 constexpr int kMaxSmem = 232448;      // 227 KiB
 constexpr int kSmemBatch = 2048;      // batches up to this size keep the page list's bounds in smem
@@ -68,6 +74,22 @@ struct TcParams : Kv8AttnParams {
   int group, tiles, rows, stages, grid, smem_csr;
   float scale_log2;
 };
+
+// W warps a CTA: 16 where the state of 8 query rows a warp fits 128 registers a thread, 8 for
+// the 16 rows of two column tiles.
+template <int NT>
+struct Shape {
+  static constexpr int kWarps = NT == 1 ? NSLG_W1 : 8;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kRows = 8 * NT;
+};
+
+// The 8 x 8 matrix of 16-bit elements held two a lane (row lane / 4), transposed.
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
 
 // Rows of one virtual sequence's tile in q and out, and what they see.
 struct Tile {
@@ -117,7 +139,7 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const void* tmap, uint64_
 }
 
 // Sequences without pages: their rows are zeros. CTA c takes sequences c, c + grid, ...
-template <typename T>
+template <typename T, int kThreads>
 __device__ void zero_empty(const TcParams& p, const int32_t* indptr) {
   const int words = p.hq * p.d / 8;
   for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
@@ -140,11 +162,12 @@ __device__ __forceinline__ uint32_t tile_offset(int t, int c) {
   return row * 128 + ((cc ^ (row & 7)) << 4);
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 1)
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
     kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_k,
                        const __grid_constant__ CUtensorMap tmap_v, const TcParams p) {
-  constexpr int KS = D / 16;             // 16-dim chunks: k steps of q.K, column pairs of p.V
+  constexpr int kWarps = Shape<NT>::kWarps, kThreads = Shape<NT>::kThreads;
+  constexpr int KS = D / 16;             // 16-dim chunks: k steps of K.q, row tiles of V^T.p^T
   constexpr int kBlock = kPS * D;        // bytes of one K (or V) block
   constexpr int kSlot = 2 * kBlock;
   constexpr int kBoxRows = kBlock / 128;
@@ -186,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (c >= n) {
     pdl_wait();
     pdl_trigger();
-    zero_empty<T>(p, indptr);
+    zero_empty<T, kThreads>(p, indptr);
     return;
   }
   const int64_t u0 = total * c / n, u1 = total * (c + 1) / n;
@@ -247,20 +270,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_trigger();
   if (lane < stages && lane < units) issue(nxt, lane);
   load_scales(nxt);
-  zero_empty<T>(p, indptr);
+  zero_empty<T, kThreads>(p, indptr);
 
   const int g = lane >> 2, tq = lane & 3;
   const int mi = lane >> 3, lr = lane & 7;
   // ldmatrix row addresses: K matrices (tokens 0-7 | 8-15) x (chunk, chunk + 1)
   const int ltok = (mi & 1) * 8 + lr, lch = mi >> 1;
 
-  uint32_t qa[KS][4];
-  float o[2 * KS][4];
-  float m0 = -INFINITY, m1 = -INFINITY, nb0 = 0.f, nb1 = 0.f, l0 = 0.f, l1 = 0.f;
-  float f0 = 0.f, f1 = 0.f;              // sm_scale * log2 e / the row's power of two
+  uint32_t qb[NT][KS][2];                // q^T fragments: row g of column tile nt
+  float o[NT][KS][4];                    // rows 2tq, 2tq + 1 (c 0/1), dims 2g (0, 1), 2g + 1 (2, 3)
+  float m[NT][2], nb[NT][2], l[NT][2], f[NT][2];   // of rows 2tq, 2tq + 1
+  int pos[NT][2];                        // last position they see
+  int low = 0;                           // ... the least of all the tile's rows
   int vid = -1;
   Tile t{};
-  int pos0 = 0, pos1 = 0;                // last position seen by rows g and g + 8
   bool ok = true;
 
   auto begin = [&](int v) {
@@ -268,15 +291,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     t.b = v / hm;
     const int vs = v % hm;
     t.h = vs / p.tiles;
-    t.r0 = vs % p.tiles * 16;
+    t.r0 = vs % p.tiles * Shape<NT>::kRows;
     t.qo_len = new_rows(p, t.b, &t.row0);
     t.kv_len = (indptr[t.b + 1] - indptr[t.b] - 1) * kPS + lpl[t.b];
-    float sc[2];
+    low = 0x7fffffff;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int pair = t.r0 + g + 8 * r;
+    for (int nt = 0; nt < NT; ++nt) {
+      const int pair = t.r0 + nt * 8 + g;
       const int tok = pair / p.group;
-      const bool live = g + 8 * r < p.rows && tok < t.qo_len;
+      const bool live = nt * 8 + g < p.rows && tok < t.qo_len;
       const T* src = static_cast<const T*>(p.q) + (t.row0 + tok) * p.q_stride +
                      static_cast<int64_t>(t.h * p.group + pair % p.group) * D + 4 * tq;
       uint2 raw[KS];
@@ -285,8 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         raw[k] = live ? *reinterpret_cast<const uint2*>(src + 16 * k) : make_uint2(0u, 0u);
       // a row of no sequence sees everything: it is never written, and no page is an edge for it
       const int lim = !live ? 0x7fffffff : p.causal ? t.kv_len - t.qo_len + tok : t.kv_len - 1;
-      if (r) pos1 = lim; else pos0 = lim;
-      sc[r] = 1.f;
+      float sc = p.scale_log2;
       if constexpr (Mma16<T>::kFormat == 1) {      // bf16 -> f16 by a power of two
         uint32_t top = 0u;
 #pragma unroll
@@ -300,31 +322,34 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int e = static_cast<int>(top >> 7);
         float up = 1.f;
         if (e > 14 && e < 255) {       // smaller rows, zeros, infinities and NaN: as they are
-          up = __uint_as_float(static_cast<uint32_t>(min(268 - e, 254)) << 23);
-          sc[r] = 1.f / up;
+          up = __uint_as_float(static_cast<uint32_t>(268 - e) << 23);
+          sc *= 1.f / up;
         }
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          const uint32_t w[2] = {raw[k].x, raw[k].y};
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            qa[k][2 * i + r] = pack_f16x2(__uint_as_float(w[i] << 16) * up,
-                                          __uint_as_float(w[i] & 0xFFFF0000u) * up);
+          qb[nt][k][0] = pack_f16x2(__uint_as_float(raw[k].x << 16) * up,
+                                    __uint_as_float(raw[k].x & 0xFFFF0000u) * up);
+          qb[nt][k][1] = pack_f16x2(__uint_as_float(raw[k].y << 16) * up,
+                                    __uint_as_float(raw[k].y & 0xFFFF0000u) * up);
         }
       } else {
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          qa[k][r] = raw[k].x;
-          qa[k][2 + r] = raw[k].y;
+          qb[nt][k][0] = raw[k].x;
+          qb[nt][k][1] = raw[k].y;
         }
       }
-    }
-    f0 = p.scale_log2 * sc[0];
-    f1 = p.scale_log2 * sc[1];
 #pragma unroll
-    for (int k = 0; k < 2 * KS; ++k) o[k][0] = o[k][1] = o[k][2] = o[k][3] = 0.f;
-    m0 = m1 = -INFINITY;
-    nb0 = nb1 = l0 = l1 = 0.f;
+      for (int e = 0; e < 2; ++e) {    // row r's values are in the lanes 4r .. 4r + 3
+        f[nt][e] = __shfl_sync(0xffffffffu, sc, (2 * tq + e) * 4);
+        pos[nt][e] = __shfl_sync(0xffffffffu, lim, (2 * tq + e) * 4);
+        m[nt][e] = -INFINITY;
+        nb[nt][e] = l[nt][e] = 0.f;
+      }
+      low = min(low, __reduce_min_sync(0xffffffffu, lim));
+#pragma unroll
+      for (int k = 0; k < KS; ++k) o[nt][k][0] = o[nt][k][1] = o[nt][k][2] = o[nt][k][3] = 0.f;
+    }
   };
 
   auto seg_begin = [&](int v) {
@@ -334,7 +359,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   auto out_row = [&](int v, int r) -> T* {   // row r of the tile in out, null where there is none
     const int b = v / hm, vs = v % hm;
-    const int pair = vs % p.tiles * 16 + r, tok = pair / p.group;
+    const int pair = vs % p.tiles * Shape<NT>::kRows + r, tok = pair / p.group;
     int64_t row0;
     if (tok >= new_rows(p, b, &row0)) return nullptr;
     return static_cast<T*>(p.out) + (row0 + tok) * p.out_stride +
@@ -343,10 +368,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // The warp's state of virtual sequence `vid`, finished: to out, or as a piece.
   auto finish = [&]() {
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
     const int64_t beg = seg_begin(vid);
     const int64_t end = beg + (indptr[t.b + 1] - indptr[t.b]);
     const bool whole = beg >= ua && end <= ub;
@@ -354,32 +375,34 @@ __global__ void __launch_bounds__(kThreads, 1)
     float* piece = tail ? reinterpret_cast<float*>(ring) : heads + warp * piece_floats;
     if (!whole && lane == 0) s_vid[2 * warp + (tail ? 1 : 0)] = vid;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = g + 8 * r;
-      if (row >= p.rows) continue;
-      const float l = r ? l1 : l0;
-      if (whole) {
-        T* dst = out_row(vid, row);
-        if (dst == nullptr) continue;
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int k = 0; k < KS; ++k)
-          *reinterpret_cast<uint2*>(dst + 16 * k + 4 * tq) =
-              make_uint2(Mma16<T>::pack(o[2 * k][2 * r] * inv, o[2 * k + 1][2 * r] * inv),
-                         Mma16<T>::pack(o[2 * k][2 * r + 1] * inv, o[2 * k + 1][2 * r + 1] * inv));
-      } else {
+      for (int e = 0; e < 2; ++e) {
+        float ls = l[nt][e];
+        ls += __shfl_xor_sync(0xffffffffu, ls, 4);
+        ls += __shfl_xor_sync(0xffffffffu, ls, 8);
+        ls += __shfl_xor_sync(0xffffffffu, ls, 16);
+        const int row = nt * 8 + 2 * tq + e;
+        if (row >= p.rows) continue;
+        if (whole) {
+          T* dst = out_row(vid, row);
+          if (dst == nullptr) continue;
+          const float inv = ls == 0.f ? 0.f : 1.f / ls;
 #pragma unroll
-        for (int k = 0; k < KS; ++k)
-          *reinterpret_cast<float2*>(piece + row * D + 16 * k + 4 * tq) =
-              make_float2(o[2 * k][2 * r], o[2 * k + 1][2 * r]),
-          *reinterpret_cast<float2*>(piece + row * D + 16 * k + 4 * tq + 2) =
-              make_float2(o[2 * k][2 * r + 1], o[2 * k + 1][2 * r + 1]);
-        if (tq == 0) {
-          piece[p.rows * D + 2 * row] = r ? m1 : m0;
-          piece[p.rows * D + 2 * row + 1] = l;
+          for (int k = 0; k < KS; ++k)
+            *reinterpret_cast<uint32_t*>(dst + 16 * k + 2 * g) =
+                Mma16<T>::pack(o[nt][k][e] * inv, o[nt][k][2 + e] * inv);
+        } else {
+#pragma unroll
+          for (int k = 0; k < KS; ++k)
+            *reinterpret_cast<float2*>(piece + row * D + 16 * k + 2 * g) =
+                make_float2(o[nt][k][e], o[nt][k][2 + e]);
+          if (g == 0) {
+            piece[p.rows * D + 2 * row] = m[nt][e];
+            piece[p.rows * D + 2 * row + 1] = ls;
+          }
         }
       }
-    }
   };
 
   int slot = 0;
@@ -410,71 +433,71 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const uint32_t kb = smem_u32(ring + slot * kSlot), vb = kb + kBlock;
       // ---- scores of the page's 16 tokens
-      float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      float s[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
 #pragma unroll
       for (int k = 0; k < KS; k += 2) {
         uint32_t w[4];
         ldmatrix_x4(kb + tile_offset<D>(ltok, k + lch), w[0], w[1], w[2], w[3]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          mma_f16_16816(s[e & 1], qa[k + (e >> 1)], f16x2_from_e4m3x2(static_cast<uint16_t>(w[e])),
-                        f16x2_from_e4m3x2(static_cast<uint16_t>(w[e] >> 16)));
-      }
-      const float a0 = f0 * sk, a1 = f1 * sk;
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t a[4] = {f16x2_from_e4m3x2(static_cast<uint16_t>(w[2 * e])),
+                                 f16x2_from_e4m3x2(static_cast<uint16_t>(w[2 * e + 1])),
+                                 f16x2_from_e4m3x2(static_cast<uint16_t>(w[2 * e] >> 16)),
+                                 f16x2_from_e4m3x2(static_cast<uint16_t>(w[2 * e + 1] >> 16))};
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        s[e][0] *= a0;
-        s[e][1] *= a0;
-        s[e][2] *= a1;
-        s[e][3] *= a1;
+          for (int nt = 0; nt < NT; ++nt)
+            mma_f16_16816(s[nt], a, qb[nt][k + e][0], qb[nt][k + e][1]);
+        }
       }
       // a page some row does not see whole, or that ends the sequence
       const int held = t.kv_len - tok0;
-      const bool edge = !__all_sync(0xffffffffu, min(pos0, pos1) >= tok0 + kPS - 1) || held < kPS;
-      if (edge) {
+      const bool edge = low < tok0 + kPS - 1 || held < kPS;
+      bool raise = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int tok = tok0 + (e >> 1) * 8 + tq * 2 + (e & 1);
-          if (tok > pos0) s[e >> 1][e & 1] = -INFINITY;
-          if (tok > pos1) s[e >> 1][2 + (e & 1)] = -INFINITY;
+          s[nt][e] *= f[nt][e & 1] * sk;
+          if (edge && tok0 + (e >> 1) * 8 + g > pos[nt][e & 1]) s[nt][e] = -INFINITY;
+          raise |= s[nt][e] > m[nt][e & 1] + kHeadroom;
         }
       }
       // ---- the running reference, raised when a score passes it by kHeadroom
-      float x0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
-      float x1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
-      if (__any_sync(0xffffffffu, x0 > m0 + kHeadroom || x1 > m1 + kHeadroom)) {
-        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
-        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
-        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
-        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
-        const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
-        const float c0 = n0 == -INFINITY ? 1.f : fast_exp2(m0 - n0);
-        const float c1 = n1 == -INFINITY ? 1.f : fast_exp2(m1 - n1);
-        m0 = n0;
-        m1 = n1;
-        nb0 = n0 == -INFINITY ? 0.f : -n0;
-        nb1 = n1 == -INFINITY ? 0.f : -n1;
-        l0 *= c0;
-        l1 *= c1;
+      if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
-        for (int k = 0; k < 2 * KS; ++k) {
-          o[k][0] *= c0;
-          o[k][1] *= c0;
-          o[k][2] *= c1;
-          o[k][3] *= c1;
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x = fmaxf(s[nt][e], s[nt][2 + e]);
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            const float mn = fmaxf(m[nt][e], x);
+            const float cf = mn == -INFINITY ? 1.f : fast_exp2(m[nt][e] - mn);
+            m[nt][e] = mn;
+            nb[nt][e] = mn == -INFINITY ? 0.f : -mn;
+            l[nt][e] *= cf;
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+              o[nt][k][e] *= cf;
+              o[nt][k][2 + e] *= cf;
+            }
+          }
+      }
+      uint32_t pb[NT][2];      // p^T: tokens 0-7, 8-15
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float p0 = fast_exp2(s[nt][2 * e] + nb[nt][0]);
+          const float p1 = fast_exp2(s[nt][2 * e + 1] + nb[nt][1]);
+          l[nt][0] += p0;
+          l[nt][1] += p1;
+          pb[nt][e] = movmatrix_trans(pack_f16x2(p0, p1));
         }
-      }
-      uint32_t pa[4];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float p0 = fast_exp2(s[e][0] + nb0), p1 = fast_exp2(s[e][1] + nb0);
-        const float p2 = fast_exp2(s[e][2] + nb1), p3 = fast_exp2(s[e][3] + nb1);
-        l0 += p0 + p1;
-        l1 += p2 + p3;
-        pa[2 * e] = pack_f16x2(p0, p1);
-        pa[2 * e + 1] = pack_f16x2(p2, p3);
-      }
-      // ---- o += scale_v * (p . V), two 16-dim chunks a step
+      // ---- o^T += scale_v * (V^T . p^T)
       uint32_t clear[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
       if (held < kPS) {     // codes behind the last token count as 0
 #pragma unroll
@@ -490,15 +513,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int e = 0; e < 4; ++e) w[e] = __byte_perm(w[e], 0u, 0x3120) & clear[e & 1];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float even[4] = {0.f, 0.f, 0.f, 0.f}, odd[4] = {0.f, 0.f, 0.f, 0.f};
-          mma_f16_16816(even, pa, f16x2_from_e4m3x2(static_cast<uint16_t>(w[2 * e])),
-                        f16x2_from_e4m3x2(static_cast<uint16_t>(w[2 * e + 1])));
-          mma_f16_16816(odd, pa, f16x2_from_e4m3x2(static_cast<uint16_t>(w[2 * e] >> 16)),
-                        f16x2_from_e4m3x2(static_cast<uint16_t>(w[2 * e + 1] >> 16)));
+          const uint32_t a[4] = {f16x2_from_e4m3x2(static_cast<uint16_t>(w[2 * e])),
+                                 f16x2_from_e4m3x2(static_cast<uint16_t>(w[2 * e] >> 16)),
+                                 f16x2_from_e4m3x2(static_cast<uint16_t>(w[2 * e + 1])),
+                                 f16x2_from_e4m3x2(static_cast<uint16_t>(w[2 * e + 1] >> 16))};
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            o[2 * (k + e)][x] = fmaf(even[x], sv, o[2 * (k + e)][x]);
-            o[2 * (k + e) + 1][x] = fmaf(odd[x], sv, o[2 * (k + e) + 1][x]);
+          for (int nt = 0; nt < NT; ++nt) {
+            float pv[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_f16_16816(pv, a, pb[nt][0], pb[nt][1]);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[nt][k + e][x] = fmaf(pv[x], sv, o[nt][k + e][x]);
           }
         }
       }
@@ -641,8 +665,9 @@ int tile_rows(int group, int max_qo_len) {
   return pairs < 16 ? static_cast<int>(pairs) : 16;
 }
 
-template <typename T, int D>
+template <typename T, int D, int NT>
 int launch_typed(TcParams p, cudaStream_t stream) {
+  constexpr int kWarps = Shape<NT>::kWarps, kThreads = Shape<NT>::kThreads;
   CUtensorMap tk, tv;
   const uint64_t rows = static_cast<uint64_t>(p.num_pages) * p.hkv * kPS * D / 128;
   int rc = encode_tiled_2d_bytes(&tk, p.codes_k, 128, rows, kPS * D / 128);
@@ -655,15 +680,23 @@ int launch_typed(TcParams p, cudaStream_t stream) {
   const size_t fixed = 1024 + heads + csr + kWarps * kMaxStages * 8 + 1024;  // + the static arrays
   int stages = static_cast<int>((kMaxSmem - fixed) / (kWarps * kSlot));
   if (stages > kMaxStages) stages = kMaxStages;
-  if (stages < 3)      // a warp's tail piece takes three slots of its ring
+  if (static_cast<size_t>(stages) * kSlot < static_cast<size_t>(p.rows) * (D + 2) * 4)
+    // a warp's tail piece is put into its part of the ring
     return set_error(NSLG_ERR_UNSUPPORTED, "kv8 attention: no room for the pipeline");
   p.stages = stages;
   const size_t smem = 1024 + heads + csr + static_cast<size_t>(kWarps) * stages * (kSlot + 8);
-  auto kern = kv8_attn_tc_kernel<T, D>;
+  auto kern = kv8_attn_tc_kernel<T, D, NT>;
   const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                static_cast<int>(smem));
   if (err != cudaSuccess) return set_error(NSLG_ERR_CUDA, cudaGetErrorString(err));
   return launch_pdl("kv8_attn_tc", kern, dim3(p.grid), dim3(kThreads), smem, stream, tk, tv, p);
+}
+
+template <typename T>
+int launch_dim(const TcParams& p, cudaStream_t stream) {
+  if (p.rows <= 8)
+    return p.d == 128 ? launch_typed<T, 128, 1>(p, stream) : launch_typed<T, 64, 1>(p, stream);
+  return p.d == 128 ? launch_typed<T, 128, 2>(p, stream) : launch_typed<T, 64, 2>(p, stream);
 }
 
 }  // namespace
@@ -698,10 +731,8 @@ int launch_kv8_attention_tc(int dtype, const Kv8AttnParams& a, void* workspace,
   p.arrive = reinterpret_cast<uint32_t*>(ws);
   p.part_o = reinterpret_cast<float*>(ws + arrive_bytes(p.grid));
   p.part_ml = p.part_o + 2ll * p.grid * p.rows * a.d;
-  if (dtype == NSLG_DTYPE_F16)
-    return a.d == 128 ? launch_typed<__half, 128>(p, stream) : launch_typed<__half, 64>(p, stream);
-  return a.d == 128 ? launch_typed<__nv_bfloat16, 128>(p, stream)
-                    : launch_typed<__nv_bfloat16, 64>(p, stream);
+  if (dtype == NSLG_DTYPE_F16) return launch_dim<__half>(p, stream);
+  return launch_dim<__nv_bfloat16>(p, stream);
 }
 
 }  // namespace nslg
