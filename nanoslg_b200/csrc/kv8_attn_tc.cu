@@ -63,6 +63,7 @@ namespace {
 #endif
 constexpr int kPS = 16;
 constexpr int kMaxStages = 8;
+constexpr int kStaticSmem = 2048;     // at least the kernel's __shared__ arrays
 constexpr int kMaxSmem = 232448;      // 227 KiB
 constexpr int kSmemBatch = 2048;      // batches up to this size keep the page list's bounds in smem
 constexpr float kHeadroom = 8.f;      // log2 of the largest probability before m is raised
@@ -98,12 +99,19 @@ struct Tile {
   int64_t row0;           // row of the sequence's first new token
 };
 
-__device__ __forceinline__ int cta_of(int64_t u, int64_t total, int n) {
-  return static_cast<int>((static_cast<int64_t>(n) * (u + 1) - 1) / total);
-}
+// [0, total) in n contiguous parts, the first total % n of them one longer.
+struct Split {
+  int q, r;
+  __device__ __forceinline__ Split(int total, int n) : q(total / n), r(total % n) {}
+  __device__ __forceinline__ int begin(int c) const { return q * c + min(c, r); }
+  __device__ __forceinline__ int part_of(int u) const {
+    const int cut = r * (q + 1);
+    return u < cut ? u / (q + 1) : r + (u - cut) / q;
+  }
+};
 
 // The sequence that holds flat page x.
-__device__ __forceinline__ int seq_of(const int32_t* indptr, int batch, int64_t x) {
+__device__ __forceinline__ int seq_of(const int32_t* indptr, int batch, int x) {
   int lo = 1, hi = batch;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
@@ -139,6 +147,51 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const void* tmap, uint64_
 }
 
 // Sequences without pages: their rows are zeros. CTA c takes sequences c, c + grid, ...
+// Joined pieces of one row: sums relative to the running maximum m of their references.
+struct Sum {
+  float m = -INFINITY, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  // the first min(N, count) of N pieces (x = m, l; a = four values); the others are repeats
+  template <int N>
+  __device__ __forceinline__ void add(const float2 (&x)[N], const float4 (&a)[N], int count) {
+    float mn = m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) mn = fmaxf(mn, x[i].x);
+    const float base = mn == -INFINITY ? 0.f : mn;
+    const float old = fast_exp2(m - base);       // 0 for m = -inf: nothing has been added yet
+    m = mn;
+    l *= old;
+    acc.x *= old;
+    acc.y *= old;
+    acc.z *= old;
+    acc.w *= old;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (i < count) {
+        const float w = fast_exp2(x[i].x - base);
+        l = fmaf(w, x[i].y, l);
+        acc.x = fmaf(w, a[i].x, acc.x);
+        acc.y = fmaf(w, a[i].y, acc.y);
+        acc.z = fmaf(w, a[i].z, acc.z);
+        acc.w = fmaf(w, a[i].w, acc.w);
+      }
+    }
+  }
+};
+
+// Where the rows of a virtual sequence's tile go: new row (r0 + r) / group of its sequence,
+// query head head0 + (r0 + r) % group.
+struct Group {
+  int b, head0, r0, len, part;
+  int64_t row0;
+};
+
+// A virtual sequence that spans CTAs cf .. cf + cnt - 1 (vid -1: none).
+struct Join {
+  int vid, cf, cnt;
+  Group to;
+};
+
 template <typename T, int kThreads>
 __device__ void zero_empty(const TcParams& p, const int32_t* indptr) {
   const int words = p.hq * p.d / 8;
@@ -173,17 +226,21 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
   constexpr int kBoxRows = kBlock / 128;
   extern __shared__ uint8_t smem_raw[];
   __shared__ int s_vid[2 * kWarps];      // virtual sequence of each warp's head / tail piece
-  __shared__ int s_piece[2 * kWarps + 1], s_group[2 * kWarps + 1];
+  __shared__ int s_piece[2 * kWarps];    // pieces in unit order: offset in floats from `smem`
+  __shared__ int s_group[2 * kWarps + 1];
+  __shared__ Group s_info[2 * kWarps];
+  __shared__ Join s_join[2];
   __shared__ int s_ngroups, s_last[2];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int stages = p.stages;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int piece_floats = p.rows * (D + 2);
+  constexpr int kPR = D + 8;             // row stride of a piece: its stores hit every bank
+  const int piece_floats = (p.rows * (kPR + 2) + 3) & ~3;
   uint8_t* ring = smem + static_cast<size_t>(warp) * stages * kSlot;
   float* heads = reinterpret_cast<float*>(smem + static_cast<size_t>(kWarps) * stages * kSlot);
   uint64_t* bars = reinterpret_cast<uint64_t*>(
-      heads + ((static_cast<size_t>(kWarps) * piece_floats + 1) & ~static_cast<size_t>(1)));
+      heads + static_cast<size_t>(kWarps) * piece_floats);
   uint64_t* full = bars + warp * stages;
 
   const int32_t* indptr = p.kv_indptr;
@@ -202,74 +259,71 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
   __syncthreads();
 
   const int hm = p.hkv * p.tiles;        // virtual sequences per sequence
-  const int64_t total = static_cast<int64_t>(indptr[p.batch]) * hm;
-  const int64_t want = (total + kWarps - 1) / kWarps;
-  const int n = static_cast<int>(want < p.grid ? want : p.grid);
+  const int64_t all = static_cast<int64_t>(indptr[p.batch]) * hm;
+  const bool fits = all >= 0 && all < (int64_t{1} << 31) - kWarps;
+  const int total = fits ? static_cast<int>(all) : 0;
+  const int n = min((total + kWarps - 1) / kWarps, p.grid);
   const int c = blockIdx.x;
   if (c >= n) {
     pdl_wait();
     pdl_trigger();
+    if (!fits && threadIdx.x == 0) report(p.status, NSLG_DEV_BAD_PLAN);
     zero_empty<T, kThreads>(p, indptr);
     return;
   }
-  const int64_t u0 = total * c / n, u1 = total * (c + 1) / n;
-  const int64_t ua = u0 + (u1 - u0) * warp / kWarps;
-  const int64_t ub = u0 + (u1 - u0) * (warp + 1) / kWarps;
-  const int units = static_cast<int>(ub - ua);
+  const Split ctas(total, n);
+  const int u0 = ctas.begin(c), u1 = ctas.begin(c + 1);
+  const Split parts(u1 - u0, kWarps);
+  const int ua = u0 + parts.begin(warp), ub = u0 + parts.begin(warp + 1);
+  const int units = ub - ua;
 
   // ---- metadata of 32 units at a time, one per lane
   struct Meta {
-    int page, vid, j;
+    int blk, vid, j;       // block (page * kv heads + head; -1: a bad page), sequence, page of it
     float sk, sv;
   };
-  auto locate = [&](int i, Meta& m) {    // page list only: may run before the PDL wait
-    m.page = -1;
+  auto locate = [&](int u, int& vid, int& first) {   // unit u: its sequence and page list entry
+    const int b = seq_of(indptr, p.batch, u / hm);
+    first = indptr[b];
+    const int np = indptr[b + 1] - first;
+    const int loc = u - first * hm;
+    const int vs = loc / np;
+    vid = b * hm + vs;
+    return loc - vs * np;
+  };
+  auto look_up = [&](int i, Meta& m) {    // page list only: may run before the PDL wait
+    m.blk = -1;
     m.vid = -1;
     m.j = 0;
     if (i < units) {
-      const int64_t u = ua + i;
-      const int b = seq_of(indptr, p.batch, u / hm);
-      const int first = indptr[b], np = indptr[b + 1] - first;
-      const int64_t loc = u - static_cast<int64_t>(first) * hm;
-      const int vs = static_cast<int>(loc / np);
-      m.vid = b * hm + vs;
-      m.j = static_cast<int>(loc - static_cast<int64_t>(vs) * np);
-      m.page = p.kv_indices[first + m.j];
-      if (m.page < 0 || m.page >= p.num_pages) {
+      int first;
+      m.j = locate(ua + i, m.vid, first);
+      const int page = p.kv_indices[first + m.j];
+      if (page < 0 || page >= p.num_pages)
         report(p.status, NSLG_DEV_BAD_PAGE);
-        m.page = -1;
-      }
+      else
+        m.blk = page * p.hkv + m.vid % hm / p.tiles;
     }
   };
-  auto head_of = [&](int vid) { return vid % hm / p.tiles; };
   auto load_scales = [&](Meta& m) {
-    m.sk = m.sv = 0.f;
-    if (m.page >= 0) {
-      const int64_t blk = static_cast<int64_t>(m.page) * p.hkv + head_of(m.vid);
-      m.sk = p.scale_k[blk];
-      m.sv = p.scale_v[blk];
-      if (m.sv != m.sv) {                // NaN rides on the scores
-        m.sk = m.sv;
-        m.sv = 0.f;
-      }
-    }
+    m.sk = m.blk >= 0 ? p.scale_k[m.blk] : 0.f;
+    m.sv = m.blk >= 0 ? p.scale_v[m.blk] : 0.f;
   };
   const uint64_t policy = p.tiles > 1 ? l2_policy_evict_last() : l2_policy_evict_first();
   auto issue = [&](const Meta& m, int i) {   // by the lane that holds unit i
     const int s = i % stages;
-    const int page = m.page < 0 ? 0 : m.page;   // a bad page: page 0's codes, scale 0
-    const int row = (page * p.hkv + head_of(m.vid)) * kBoxRows;
+    const int row = max(m.blk, 0) * kBoxRows;   // a bad page: page 0's codes, scale 0
     mbar_arrive_expect_tx(&full[s], kSlot);
     tma_load_2d(ring + s * kSlot, &tmap_k, &full[s], 0, row, policy);
     tma_load_2d(ring + s * kSlot + kBlock, &tmap_v, &full[s], 0, row, policy);
   };
 
   Meta cur, nxt;
-  locate(lane, nxt);
+  look_up(lane, nxt);
   pdl_wait();      // the kernel before may have written q, the codes and the scales
   pdl_trigger();
+  load_scales(nxt);   // before the bulk loads, which would queue in front of them
   if (lane < stages && lane < units) issue(nxt, lane);
-  load_scales(nxt);
   zero_empty<T, kThreads>(p, indptr);
 
   const int g = lane >> 2, tq = lane & 3;
@@ -352,28 +406,56 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
     }
   };
 
-  auto seg_begin = [&](int v) {
+  auto segment = [&](int v, int& beg, int& end) {   // units of virtual sequence v
     const int b = v / hm;
     const int first = indptr[b], np = indptr[b + 1] - first;
-    return static_cast<int64_t>(first) * hm + static_cast<int64_t>(v % hm) * np;
+    beg = first * hm + (v - b * hm) * np;
+    end = beg + np;
   };
-  auto out_row = [&](int v, int r) -> T* {   // row r of the tile in out, null where there is none
-    const int b = v / hm, vs = v % hm;
-    const int pair = vs % p.tiles * Shape<NT>::kRows + r, tok = pair / p.group;
-    int64_t row0;
-    if (tok >= new_rows(p, b, &row0)) return nullptr;
-    return static_cast<T*>(p.out) + (row0 + tok) * p.out_stride +
-           static_cast<int64_t>(vs / p.tiles * p.group + pair % p.group) * D;
+  auto group_of = [&](int v) {           // where the rows of virtual sequence v go
+    Group gi;
+    gi.b = v / hm;
+    const int vs = v - gi.b * hm, h = vs / p.tiles;
+    gi.head0 = h * p.group;
+    gi.r0 = (vs - h * p.tiles) * Shape<NT>::kRows;
+    gi.len = new_rows(p, gi.b, &gi.row0);
+    return gi;
   };
+  auto out_row = [&](const Group& gi, int r) -> T* {   // row r of the tile, null: none
+    const int pair = gi.r0 + r, tok = pair / p.group;
+    if (tok >= gi.len) return nullptr;
+    return static_cast<T*>(p.out) + (gi.row0 + tok) * p.out_stride +
+           static_cast<int64_t>(gi.head0 + pair - tok * p.group) * D;
+  };
+
+  // The virtual sequences this CTA shares with others, worked out while the first loads are
+  // under way: [0] one that began in an earlier CTA, [1] one that begins here and goes on.
+  if (warp < 2 && lane == 0) {
+    Join jn;
+    int first;
+    locate(warp == 0 ? u0 : u1 - 1, jn.vid, first);
+    int beg, end;
+    segment(jn.vid, beg, end);
+    if (warp == 0 ? beg < u0 : (beg >= u0 && end > u1)) {
+      jn.cf = ctas.part_of(beg);
+      jn.cnt = ctas.part_of(end - 1) - jn.cf + 1;
+      jn.to = group_of(jn.vid);
+    } else {
+      jn.vid = -1;
+    }
+    s_join[warp] = jn;
+  }
 
   // The warp's state of virtual sequence `vid`, finished: to out, or as a piece.
   auto finish = [&]() {
-    const int64_t beg = seg_begin(vid);
-    const int64_t end = beg + (indptr[t.b + 1] - indptr[t.b]);
+    int beg, end;
+    segment(vid, beg, end);
     const bool whole = beg >= ua && end <= ub;
     const bool tail = end > ub;
     float* piece = tail ? reinterpret_cast<float*>(ring) : heads + warp * piece_floats;
     if (!whole && lane == 0) s_vid[2 * warp + (tail ? 1 : 0)] = vid;
+    Group to{};
+    if (whole) to = group_of(vid);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -385,7 +467,7 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
         const int row = nt * 8 + 2 * tq + e;
         if (row >= p.rows) continue;
         if (whole) {
-          T* dst = out_row(vid, row);
+          T* dst = out_row(to, row);
           if (dst == nullptr) continue;
           const float inv = ls == 0.f ? 0.f : 1.f / ls;
 #pragma unroll
@@ -395,11 +477,11 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
         } else {
 #pragma unroll
           for (int k = 0; k < KS; ++k)
-            *reinterpret_cast<float2*>(piece + row * D + 16 * k + 2 * g) =
+            *reinterpret_cast<float2*>(piece + row * kPR + 16 * k + 2 * g) =
                 make_float2(o[nt][k][e], o[nt][k][2 + e]);
           if (g == 0) {
-            piece[p.rows * D + 2 * row] = m[nt][e];
-            piece[p.rows * D + 2 * row + 1] = ls;
+            piece[p.rows * kPR + 2 * row] = m[nt][e];
+            piece[p.rows * kPR + 2 * row + 1] = ls;
           }
         }
       }
@@ -409,7 +491,7 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
   uint32_t phase = 0;
   for (int base = 0; base < units && ok; base += 32) {
     cur = nxt;
-    locate(base + 32 + lane, nxt);
+    look_up(base + 32 + lane, nxt);
     load_scales(nxt);
     const int stop = min(32, units - base);
     for (int i = 0; i < stop; ++i) {
@@ -418,8 +500,12 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
         if (vid >= 0) finish();
         begin(v);
       }
-      const float sk = __shfl_sync(0xffffffffu, cur.sk, i);
-      const float sv = __shfl_sync(0xffffffffu, cur.sv, i);
+      float sk = __shfl_sync(0xffffffffu, cur.sk, i);
+      float sv = __shfl_sync(0xffffffffu, cur.sv, i);
+      if (sv != sv) {        // NaN rides on the scores
+        sk = sv;
+        sv = 0.f;
+      }
       const int tok0 = __shfl_sync(0xffffffffu, cur.j, i) * kPS;
       ok = __all_sync(0xffffffffu, mbar_wait(&full[slot], phase));
       if (!ok) {
@@ -544,16 +630,30 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
   if (warp == 0) {
     const int v = lane < 2 * kWarps ? s_vid[lane] : -1;
     const uint32_t have = __ballot_sync(0xffffffffu, v >= 0);
-    const int at = __popc(have & ((1u << lane) - 1u));
-    if (v >= 0) s_piece[at] = lane;
-    __syncwarp();
-    const int cnt = __popc(have);
-    const bool starts = lane < cnt && (lane == 0 || s_vid[s_piece[lane]] != s_vid[s_piece[lane - 1]]);
+    const uint32_t before = have & ((1u << lane) - 1u);
+    // the piece before this one, if it is of the same sequence, is not a start
+    const int prev = __shfl_sync(0xffffffffu, v, before != 0u ? 31 - __clz(before) : 0);
+    const bool starts = v >= 0 && (before == 0u || prev != v);
     const uint32_t st = __ballot_sync(0xffffffffu, starts);
-    if (starts) s_group[__popc(st & ((1u << lane) - 1u))] = lane;
+    if (v >= 0) {
+      const int w = lane >> 1;
+      s_piece[__popc(before)] =
+          (lane & 1) ? w * stages * (kSlot / 4) : kWarps * stages * (kSlot / 4) + w * piece_floats;
+    }
+    if (starts) {
+      const int gr = __popc(st & ((1u << lane) - 1u));
+      s_group[gr] = __popc(before);
+      Group gi = group_of(v);
+      int beg, end;
+      segment(v, beg, end);
+      // whole in this CTA: to out; else to the partial of the one that began before (2c) or
+      // begins here (2c + 1)
+      gi.part = beg >= u0 && end <= u1 ? -1 : 2 * c + (beg >= u0 ? 1 : 0);
+      s_info[gr] = gi;
+    }
     if (lane == 0) {
-      s_group[__popc(st)] = cnt;
       s_ngroups = __popc(st);
+      s_group[__popc(st)] = __popc(have);
       s_last[0] = s_last[1] = 0;
     }
   }
@@ -561,99 +661,75 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
   const int ngroups = s_ngroups;
   if (ngroups == 0) return;
   constexpr int DQ = D / 4;
-  auto piece_at = [&](int k) -> const float* {
-    const int id = s_piece[k], w = id >> 1;
-    return (id & 1) ? reinterpret_cast<const float*>(smem + static_cast<size_t>(w) * stages * kSlot)
-                    : heads + w * piece_floats;
+  const float* pieces = reinterpret_cast<const float*>(smem);
+  const int ml = p.rows * kPR;           // (m, l) of a piece's rows lie behind its values
+  auto store_out = [&](T* dst, const float4& a, float l) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    *reinterpret_cast<uint2*>(dst) =
+        make_uint2(Mma16<T>::pack(a.x * inv, a.y * inv), Mma16<T>::pack(a.z * inv, a.w * inv));
   };
-  for (int e = threadIdx.x; e < ngroups * p.rows * DQ; e += kThreads) {
-    const int gr = e / (p.rows * DQ), row = e / DQ % p.rows, dq = e % DQ;
+  const int per_group = p.rows * DQ;
+  for (int e = threadIdx.x; e < ngroups * per_group; e += kThreads) {
+    const int gr = e / per_group, row = (e - gr * per_group) / DQ, dq = e % DQ;
     const int k0 = s_group[gr], k1 = s_group[gr + 1];
-    float m = -INFINITY;
-    for (int k = k0; k < k1; ++k) m = fmaxf(m, piece_at(k)[p.rows * D + 2 * row]);
-    const float base = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = k0; k < k1; ++k) {
-      const float* pc = piece_at(k);
-      const float w = fast_exp2(pc[p.rows * D + 2 * row] - base);
-      const float2 a = *reinterpret_cast<const float2*>(pc + row * D + 4 * dq);
-      const float2 b = *reinterpret_cast<const float2*>(pc + row * D + 4 * dq + 2);
-      l = fmaf(w, pc[p.rows * D + 2 * row + 1], l);
-      acc.x = fmaf(w, a.x, acc.x);
-      acc.y = fmaf(w, a.y, acc.y);
-      acc.z = fmaf(w, b.x, acc.z);
-      acc.w = fmaf(w, b.y, acc.w);
+    Sum sum;
+    for (int k = k0; k < k1; k += 4) {
+      float2 x[4];
+      float4 a[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float* pc = pieces + s_piece[min(k + i, k1 - 1)];
+        x[i] = *reinterpret_cast<const float2*>(pc + ml + 2 * row);
+        a[i] = *reinterpret_cast<const float4*>(pc + row * kPR + 4 * dq);
+      }
+      sum.add<4>(x, a, k1 - k);
     }
-    const int v = s_vid[s_piece[k0]];
-    const int64_t beg = seg_begin(v);
-    const int b = v / hm;
-    const int64_t end = beg + (indptr[b + 1] - indptr[b]);
-    if (beg >= u0 && end <= u1) {
-      T* dst = out_row(v, row);
-      if (dst == nullptr) continue;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      *reinterpret_cast<uint2*>(dst + 4 * dq) = make_uint2(
-          Mma16<T>::pack(acc.x * inv, acc.y * inv), Mma16<T>::pack(acc.z * inv, acc.w * inv));
+    const Group& gi = s_info[gr];
+    if (gi.part < 0) {
+      T* dst = out_row(gi, row);
+      if (dst != nullptr) store_out(dst + 4 * dq, sum.acc, sum.l);
     } else {
-      const int64_t r = (2ll * c + (beg >= u0 ? 1 : 0)) * p.rows + row;
-      *reinterpret_cast<float4*>(p.part_o + r * D + 4 * dq) = acc;
-      if (dq == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * r) = make_float2(m, l);
+      const int64_t r = static_cast<int64_t>(gi.part) * p.rows + row;
+      *reinterpret_cast<float4*>(p.part_o + r * D + 4 * dq) = sum.acc;
+      if (dq == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * r) = make_float2(sum.m, sum.l);
     }
   }
   __syncthreads();
 
-  // ---- virtual sequences that span CTAs: the first and the last group can be one
-  int jv[2], cf[2], cnt[2];
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int v = s_vid[s_piece[k == 0 ? 0 : s_group[ngroups - 1]]];
-    const int64_t beg = seg_begin(v);
-    const int64_t end = beg + (indptr[v / hm + 1] - indptr[v / hm]);
-    // k == 0: one that began before this CTA; k == 1: one that begins here and goes on
-    const bool joins = k == 0 ? beg < u0 : (beg >= u0 && end > u1);
-    jv[k] = joins ? v : -1;
-    cf[k] = joins ? cta_of(beg, total, n) : 0;
-    cnt[k] = joins ? cta_of(end - 1, total, n) - cf[k] + 1 : 0;
-    if (joins && threadIdx.x == 32 * k) {
-      const uint32_t prev = atom_add_acq_rel_u32(&p.arrive[cf[k]], 1u);
-      if (prev + 1u == static_cast<uint32_t>(cnt[k])) {
-        atomicExch(&p.arrive[cf[k]], 0u);
-        s_last[k] = 1;
-      }
+  // ---- virtual sequences that span CTAs
+  if (warp < 2 && lane == 0 && s_join[warp].vid >= 0) {
+    uint32_t* count = &p.arrive[s_join[warp].cf];
+    const uint32_t prev = atom_add_acq_rel_u32(count, 1u);
+    if (prev + 1u == static_cast<uint32_t>(s_join[warp].cnt)) {
+      atomicExch(count, 0u);
+      s_last[warp] = 1;
     }
   }
   __syncthreads();
-#pragma unroll
   for (int k = 0; k < 2; ++k) {
     if (!s_last[k]) continue;
-    for (int e = threadIdx.x; e < p.rows * DQ; e += kThreads) {
+    const Join& jn = s_join[k];
+    const int cnt = jn.cnt;
+    for (int e = threadIdx.x; e < per_group; e += kThreads) {
       const int row = e / DQ, dq = e % DQ;
-      // partial i: CTA cf + i, the slot of one that begins there for the first, else of one
-      // that began before
-      auto slot_row = [&](int i) { return (2ll * (cf[k] + i) + (i == 0 ? 1 : 0)) * p.rows + row; };
-      float m = -INFINITY;
-#pragma unroll 8
-      for (int i = 0; i < cnt[k]; ++i) m = fmaxf(m, __ldcg(p.part_ml + 2 * slot_row(i)));
-      const float base = m == -INFINITY ? 0.f : m;
-      float l = 0.f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-      for (int i = 0; i < cnt[k]; ++i) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + 2 * slot_row(i)));
-        const float4 a = __ldcg(reinterpret_cast<const float4*>(p.part_o + slot_row(i) * D + 4 * dq));
-        const float w = fast_exp2(ml.x - base);
-        l = fmaf(w, ml.y, l);
-        acc.x = fmaf(w, a.x, acc.x);
-        acc.y = fmaf(w, a.y, acc.y);
-        acc.z = fmaf(w, a.z, acc.z);
-        acc.w = fmaf(w, a.w, acc.w);
+      Sum sum;
+      // kBatch partials at a time, every load of a batch in flight at once. Partial i is CTA
+      // cf + i's: the one that begins there for the first, the one that began before else.
+      constexpr int kBatch = 8;
+      for (int i0 = 0; i0 < cnt; i0 += kBatch) {
+        float2 x[kBatch];
+        float4 a[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int at = min(i0 + i, cnt - 1);
+          const int64_t r = (2ll * (jn.cf + at) + (at == 0 ? 1 : 0)) * p.rows + row;
+          x[i] = __ldcg(reinterpret_cast<const float2*>(p.part_ml + 2 * r));
+          a[i] = __ldcg(reinterpret_cast<const float4*>(p.part_o + r * D + 4 * dq));
+        }
+        sum.add<kBatch>(x, a, cnt - i0);
       }
-      T* dst = out_row(jv[k], row);
-      if (dst == nullptr) continue;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      *reinterpret_cast<uint2*>(dst + 4 * dq) = make_uint2(
-          Mma16<T>::pack(acc.x * inv, acc.y * inv), Mma16<T>::pack(acc.z * inv, acc.w * inv));
+      T* dst = out_row(jn.to, row);
+      if (dst != nullptr) store_out(dst + 4 * dq, sum.acc, sum.l);
     }
   }
 }
@@ -675,12 +751,13 @@ int launch_typed(TcParams p, cudaStream_t stream) {
   if (rc != NSLG_OK) return rc;
   constexpr size_t kSlot = 2 * kPS * D;
   p.smem_csr = p.batch <= kSmemBatch ? 1 : 0;
-  const size_t heads = (static_cast<size_t>(kWarps) * p.rows * (D + 2) + 1) / 2 * 8;
+  const size_t piece = static_cast<size_t>((p.rows * (D + 10) + 3) & ~3) * 4;
+  const size_t heads = kWarps * piece;
   const size_t csr = p.smem_csr ? static_cast<size_t>(2 * p.batch + 1) * 4 : 0;
-  const size_t fixed = 1024 + heads + csr + kWarps * kMaxStages * 8 + 1024;  // + the static arrays
+  const size_t fixed = 1024 + heads + csr + kWarps * kMaxStages * 8 + kStaticSmem;
   int stages = static_cast<int>((kMaxSmem - fixed) / (kWarps * kSlot));
   if (stages > kMaxStages) stages = kMaxStages;
-  if (static_cast<size_t>(stages) * kSlot < static_cast<size_t>(p.rows) * (D + 2) * 4)
+  if (static_cast<size_t>(stages) * kSlot < piece)
     // a warp's tail piece is put into its part of the ring
     return set_error(NSLG_ERR_UNSUPPORTED, "kv8 attention: no room for the pipeline");
   p.stages = stages;

@@ -192,6 +192,7 @@ struct Kv8AppendParams : Kv8Cache {
   int64_t q_stride, k_stride, v_stride, num_rows, table_rows;
   int batch, hq, hkv, d, page_size, group, max_qo_len;
   int pages_per_seq;    // pages that max_qo_len tokens can touch
+  int heads_per_block;  // set by the launch
   uint32_t* status;
 };
 int launch_kv8_append(int dtype, const Kv8AppendParams& p, cudaStream_t stream);
