@@ -32,6 +32,16 @@ from . import _native as N
 from . import ops
 
 
+def parse_kv_dtype(kv_dtype):
+    """A cache element type as a config names it: None / "auto" (the activation type) -> None,
+    "fp8" / "fp8_e4m3" / torch.float8_e4m3fn -> torch.float8_e4m3fn."""
+    if kv_dtype in (None, "auto"):
+        return None
+    if kv_dtype in ("fp8", "fp8_e4m3", ops.KV8_DTYPE):
+        return ops.KV8_DTYPE
+    raise ValueError(f"unknown kv cache dtype {kv_dtype!r}")
+
+
 @dataclass
 class KVCacheConfig:
     """Cache sizing (kv_cache.py:59-145). ``backend`` is kept for config compatibility;
@@ -49,15 +59,28 @@ class KVCacheConfig:
     device: torch.device = None
     enable_prefix_caching: bool = True
     backend: str = "b200"
+    # what the pages hold: None = ``dtype``, torch.float8_e4m3fn = the 8-bit cache (e4m3 codes
+    # and one scale per page and kv head; about twice the tokens in the same memory)
+    kv_dtype: Optional[torch.dtype] = None
 
     def __post_init__(self):
+        self.kv_dtype = parse_kv_dtype(self.kv_dtype)
+        if self.kv8 and (self.head_dim % 32 or self.head_dim > 256):
+            raise ValueError("the 8-bit cache needs a head_dim that is a multiple of 32, at most "
+                             f"256, got {self.head_dim}")
         if self.backend not in ("auto", "b200", "flashinfer", "contiguous"):
             raise ValueError(f"unknown kv backend {self.backend!r}")
         self.backend = "b200"
         if self.max_pages <= 0:
             self.max_pages = self._auto_pages()
 
+    @property
+    def kv8(self) -> bool:
+        return self.kv_dtype is not None
+
     def _elem_bytes(self) -> int:
+        if self.kv8:
+            return 1
         return {torch.float16: 2, torch.bfloat16: 2, torch.float32: 4}.get(self.dtype, 2)
 
     def _auto_pages(self) -> int:
@@ -73,6 +96,8 @@ class KVCacheConfig:
         budget = int(max(0, free - headroom) * self.memory_fraction)
         per_page = (2 * self.num_layers * self.page_size * self.num_kv_heads
                     * self.head_dim * self._elem_bytes())
+        if self.kv8:
+            per_page += 2 * self.num_layers * self.num_kv_heads * 4      # the scales
         return max(64, min(budget // max(per_page, 1), 65536))
 
     @classmethod
@@ -155,7 +180,9 @@ class KVCacheManager(ABC):
 
 class PagePool:
     """K/V pages ``[num_layers, max_pages, page_size, num_kv_heads, head_dim]``; page 0 is
-    the permanent null page (kv_cache.py:382-442).
+    the permanent null page (kv_cache.py:382-442). With ``cfg.kv_dtype`` the pages hold e4m3
+    codes, ``[num_layers, max_pages, num_kv_heads, page_size, head_dim]``, and ``k_scale`` /
+    ``v_scale`` ``[num_layers, max_pages, num_kv_heads]`` their scales.
 
     Page ids come from ``set.pop()`` on a free set built and updated exactly as the
     reference does, so the same call sequence hands out the same ids.  The reference
@@ -166,9 +193,17 @@ class PagePool:
 
     def __init__(self, cfg: KVCacheConfig):
         self.cfg = cfg
+        self.k_scale = self.v_scale = None
         shape = (cfg.num_layers, cfg.max_pages, cfg.page_size, cfg.num_kv_heads, cfg.head_dim)
-        self.k = torch.zeros(shape, dtype=cfg.dtype, device=cfg.device)
-        self.v = torch.zeros(shape, dtype=cfg.dtype, device=cfg.device)
+        dt = cfg.dtype
+        if cfg.kv8:
+            # the 8-bit cache keeps each (page, kv head) block contiguous, with one scale
+            shape = (cfg.num_layers, cfg.max_pages, cfg.num_kv_heads, cfg.page_size, cfg.head_dim)
+            dt = cfg.kv_dtype
+            self.k_scale = torch.zeros(shape[:3], dtype=torch.float32, device=cfg.device)
+            self.v_scale = torch.zeros(shape[:3], dtype=torch.float32, device=cfg.device)
+        self.k = torch.zeros(shape, dtype=dt, device=cfg.device)
+        self.v = torch.zeros(shape, dtype=dt, device=cfg.device)
         self.ref_count = [0] * cfg.max_pages
         # numpy, so a decode step updates the pages of a whole batch in one indexed op
         self.tokens_used = np.zeros(cfg.max_pages, dtype=np.int32)
@@ -182,6 +217,9 @@ class PagePool:
         self.v_layers = [self.v[i] for i in range(cfg.num_layers)]
         self.layer_ptrs = [(a.data_ptr(), b.data_ptr())
                            for a, b in zip(self.k_layers, self.v_layers)]
+        # 8-bit cache: (codes of K, of V, scales of K, of V) per layer, as the kv8 ops take them
+        self.kv8_layers = ([(self.k[i], self.v[i], self.k_scale[i], self.v_scale[i])
+                            for i in range(cfg.num_layers)] if cfg.kv8 else None)
 
     def alloc(self, n=1) -> Optional[List[int]]:
         with self._lock:
@@ -226,6 +264,12 @@ class PagePool:
         if not ids:
             return
         idx = torch.tensor(ids, dtype=torch.long).to(self.k.device, non_blocking=True)
+        if self.kv8_layers is not None:
+            self.k.view(torch.uint8).index_fill_(1, idx, 0)
+            self.v.view(torch.uint8).index_fill_(1, idx, 0)
+            self.k_scale.index_fill_(1, idx, 0)
+            self.v_scale.index_fill_(1, idx, 0)
+            return
         self.k.index_fill_(1, idx, 0)
         self.v.index_fill_(1, idx, 0)
 
@@ -254,6 +298,9 @@ class PagePool:
         self.flush_zero()
         self.k[:, d].copy_(self.k[:, pid])
         self.v[:, d].copy_(self.v[:, pid])
+        if self.kv8_layers is not None:
+            self.k_scale[:, d].copy_(self.k_scale[:, pid])
+            self.v_scale[:, d].copy_(self.v_scale[:, pid])
         self.tokens_used[d] = self.tokens_used[pid]
         return d
 
@@ -824,6 +871,9 @@ class B200CacheContext(CacheContext):
     def attend(self, layer_idx, q, k_new, v_new, n_heads, n_kv_heads):
         """q, k_new already rotated (the ABC contract, models.py:99-105)."""
         self._check_width(q)
+        if self.cache.pool.kv8_layers is not None:
+            self._append_kv8(layer_idx, None, k_new, v_new, None, None)
+            return self._attention_kv8(layer_idx, q)
         if self._is_decode:
             out = self._decode_direct(layer_idx, q, k_new, v_new)
             if out is not None:
@@ -839,6 +889,9 @@ class B200CacheContext(CacheContext):
         self._check_width(q)
         pool = self.cache.pool
         B, S, hq, d = q.shape
+        if pool.kv8_layers is not None:
+            q_rot = self._append_kv8(layer_idx, q, k_new, v_new, cos, sin)
+            return self._attention_kv8(layer_idx, q_rot.view(B, S, hq, d))
         q_rot = ops.rope_kv_append(q, k_new, v_new, self._pos_i32, cos, sin, self._write_loc,
                                    pool.k_layers[layer_idx], pool.v_layers[layer_idx])
         return self._attention(layer_idx, q_rot.view(B, S, hq, d))
@@ -849,7 +902,7 @@ class B200CacheContext(CacheContext):
         weight), then attention -- what the projections followed by ``attend_rope`` do.
         Returns None (nothing launched) where that kernel does not take the operands;
         the caller then projects and calls ``attend_rope``."""
-        if not self._is_decode or x.dim() != 3:
+        if not self._is_decode or x.dim() != 3 or self.cache.pool.kv8_layers is not None:
             return None
         B, S, _ = x.shape
         if B != self.batch_size or S != self._iw:
@@ -897,6 +950,23 @@ class B200CacheContext(CacheContext):
         if rc:
             raise N.NativeError("nslg_append_paged_decode", rc, lib.nslg_last_error().decode())
         return out
+
+    def _append_kv8(self, layer_idx, q, k, v, cos, sin):
+        """New rows into the 8-bit pages, rotated when cos / sin are given (with q)."""
+        return ops.rope_kv8_append(q, k, v, cos, sin, *self.cache.pool.kv8_layers[layer_idx],
+                                   self.qo_indptr, max(self.new_token_counts, default=0),
+                                   self.kv_indptr, self.kv_indices, self.kv_last_page_len,
+                                   q_row_start=self.q_row_start, rotate=cos is not None)
+
+    def _attention_kv8(self, layer_idx, q):
+        B, S, hq, d = q.shape
+        layer = self.cache.pool.kv8_layers[layer_idx]
+        seqs = (self.kv_indptr, self.kv_indices, self.kv_last_page_len)
+        if self._is_decode and S == 1:
+            return ops.paged_decode_kv8(q[:, 0], *layer, *seqs, self._sm_scale).view(B, 1, hq * d)
+        out = ops.paged_prefill_kv8(q, self.qo_indptr, max(self.new_token_counts, default=0),
+                                    *layer, *seqs, self._sm_scale, q_row_start=self.q_row_start)
+        return out.view(B, S, hq * d)
 
     def _check_width(self, q):
         if q.shape[0] != self.batch_size or q.shape[1] != self._iw:
@@ -1279,6 +1349,9 @@ class B200PagedKVCache(KVCacheManager):
             st.block_table.extend(self._alloc(need - len(st.block_table)))
 
     def begin_forward(self, seq_ids, ntoks, offsets=None):
+        if self.cfg.kv8 and len(set(seq_ids)) != len(seq_ids):
+            # two writers of one page: its scale would depend on which came first
+            raise ValueError("a sequence can be in a forward over the 8-bit cache only once")
         if (self.device_plan and 0 < len(seq_ids) <= 4096 and not any(offsets or ())
                 and (ntoks.count(1) == len(ntoks) if isinstance(ntoks, list)
                      else all(n == 1 for n in ntoks))):
@@ -1370,7 +1443,8 @@ class B200PagedKVCache(KVCacheManager):
 def create_cache_manager(hf_config, parallel_config, device, dtype, model_config,
                          max_batch_size=4) -> KVCacheManager:
     """Factory with the reference's signature (kv_cache.py:780-804); always the B200
-    paged backend."""
+    paged backend. ``model_config.kv_cache_dtype`` ("auto", or "fp8" for the 8-bit cache)
+    chooses what the pages hold."""
     dev = torch.device(device) if device is not None else None
     if dev is not None and dev.type == "cuda":
         torch.cuda.synchronize(dev)
@@ -1385,5 +1459,6 @@ def create_cache_manager(hf_config, parallel_config, device, dtype, model_config
         dtype=dtype,
         enable_prefix_caching=getattr(model_config, "enable_prefix_caching", True),
         backend=getattr(model_config, "kv_backend", "auto"),
+        kv_dtype=getattr(model_config, "kv_cache_dtype", None),
     )
     return B200PagedKVCache(kv_cfg)

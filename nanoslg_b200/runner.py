@@ -49,7 +49,7 @@ class LlamaRunner:
 
     def __init__(self, hf_config, device, dtype=torch.bfloat16, tp_size=1, rank=0,
                  max_kv_pages=0, page_size=16, prefix_caching=True, seed=0, pp_size=1,
-                 peer_allreduce=True, peer_max_rows=256):
+                 peer_allreduce=True, peer_max_rows=256, kv_cache_dtype=None):
         self.device = torch.device(device)
         self.dtype = dtype
         world = tp_size * pp_size
@@ -85,7 +85,8 @@ class LlamaRunner:
                                       peer_max_rows, hf_config.hidden_size, dtype)
             models.enable_peer_allreduce(self.model, self.peer)
         mc = SimpleNamespace(page_size=page_size, max_kv_pages=max_kv_pages,
-                             enable_prefix_caching=prefix_caching)
+                             enable_prefix_caching=prefix_caching,
+                             kv_cache_dtype=kv_cache_dtype)
         self.cache = create_cache_manager(hf_config, self.pcfg, self.device, dtype, mc,
                                           max_batch_size=0)
         self.seq_ids = []

@@ -149,3 +149,53 @@ def test_ops_refuse_cpu_tensors_and_wrong_layouts():
         ops._kv8_rows(torch.zeros(1, 3, 64), "q", 2, 64)
     with pytest.raises(ValueError, match="kv heads"):
         ops._kv8_rows(torch.zeros(1, 4, 32), "q", 2, 64)
+
+
+def test_manager_bookkeeping_does_not_depend_on_the_cache_type():
+    """Pages, plans and copy on write of an 8-bit pool on the CPU: the ids of a 16-bit one, and
+    a copied page takes its scales along."""
+    from nanoslg_b200.kv_cache import B200PagedKVCache, KVCacheConfig
+    mgrs = [B200PagedKVCache(KVCacheConfig(num_layers=2, num_kv_heads=2, num_qo_heads=4, head_dim=32,
+                                           page_size=4, max_pages=40, dtype=torch.bfloat16, kv_dtype=t))
+            for t in (None, "fp8")]
+    assert mgrs[0].pool.kv8_layers is None
+    assert mgrs[1].pool.k.shape == (2, 40, 2, 4, 32) and mgrs[1].pool.k.dtype == torch.float8_e4m3fn
+    plans = []
+    for m in mgrs:
+        m.allocate_sequence("a", list(range(11)))
+        m.begin_forward(["a"], [11])
+        m.seqs["a"].num_tokens = 11
+        m.release_sequence("a")
+        n = m.allocate_sequence("b", list(range(11)))
+        m.seqs["b"].num_tokens = n - 1
+        page = m.seqs["b"].block_table[1]
+        if m.pool.kv8_layers:
+            m.pool.k_scale[:, page] = 3.0
+            m.pool.v_scale[:, page] = 5.0
+            m.pool.k.view(torch.uint8)[:, page] = 7
+        ctx = m.begin_forward(["b"], [2])
+        assert m.seqs["b"].block_table[1] != page
+        plans.append((list(m.seqs["b"].block_table), ctx.kv_indptr.tolist(), ctx.kv_indices.tolist(),
+                      ctx.kv_last_page_len.tolist(), ctx.qo_indptr.tolist(), ctx.q_row_start.tolist()))
+    assert plans[0] == plans[1]
+    new = mgrs[1].seqs["b"].block_table[1]
+    assert bool((mgrs[1].pool.k_scale[:, new] == 3.0).all()) and bool((mgrs[1].pool.v_scale[:, new] == 5.0).all())
+    assert bool((mgrs[1].pool.k.view(torch.uint8)[:, new] == 7).all())
+
+
+@pytest.mark.parametrize("kv_dtype,ok", [(None, True), ("auto", True), ("fp8", True), ("fp8_e4m3", True),
+                                         (torch.float8_e4m3fn, True), ("int8", False),
+                                         (torch.float8_e5m2, False)])
+def test_kv_dtype_names(kv_dtype, ok):
+    from nanoslg_b200.kv_cache import KVCacheConfig
+
+    def make(d=64):
+        return KVCacheConfig(num_layers=1, num_kv_heads=1, num_qo_heads=1, head_dim=d, kv_dtype=kv_dtype)
+    if not ok:
+        with pytest.raises(ValueError, match="kv cache dtype"):
+            make()
+        return
+    assert make().kv8 == (kv_dtype not in (None, "auto"))
+    if make().kv8:
+        with pytest.raises(ValueError, match="head_dim"):
+            make(d=80)
