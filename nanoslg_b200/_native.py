@@ -5,10 +5,12 @@ from ``nanoslg_b200/lib/libnslg_b200.so``.  There is no fallback: when the libra
 missing every op raises.  Loading needs no GPU; calling a kernel does.
 """
 import ctypes
+import importlib.util
 import os
 import threading
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libnslg_b200.so")
+KV8_PATH = os.path.join(os.path.dirname(LIB_PATH), "_kv8.so")
 
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
@@ -99,6 +101,7 @@ TP_MAX_WORLD = 8
 TP_COUNTER_BYTES = 1024
 
 _lib = None
+_kv8 = None
 _lock = threading.Lock()
 
 
@@ -128,6 +131,25 @@ def lib():
                 fn.argtypes = args
             _lib = h
     return _lib
+
+
+def kv8():
+    """The torch side of the 8-bit cache's ops (csrc/kv8_torch.cpp), loaded once."""
+    global _kv8
+    if _kv8 is None:
+        from . import ops
+        lib()
+        with _lock:
+            if _kv8 is None:
+                if not os.path.exists(KV8_PATH):
+                    raise RuntimeError(f"nanoslg_b200 extension not found at {KV8_PATH}; "
+                                       "build it with `python -m nanoslg_b200.build`")
+                spec = importlib.util.spec_from_file_location("_kv8", KV8_PATH)
+                m = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(m)
+                m.setup(lambda i: ops.status_word(f"cuda:{i}").data_ptr(), NativeError)
+                _kv8 = m
+    return _kv8
 
 
 def call(name, *args):

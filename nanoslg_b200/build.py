@@ -3,6 +3,7 @@
 Each ``csrc/*.cu`` file is compiled by nvcc into ``_build/`` (in parallel, skipped
 when up to date) and the objects are linked into one shared library that exports the
 C ABI of ``include/nslg_b200.h``.  nvcc cross-compiles, so this runs without a GPU.
+``csrc/kv8_torch.cpp``, the torch side of the 8-bit cache's ops, becomes ``lib/_kv8.so``.
 
     python -m nanoslg_b200.build [--force] [--verbose]
 """
@@ -21,6 +22,7 @@ INCLUDE = os.path.join(ROOT, "include")
 BUILD = os.path.join(ROOT, "_build")
 LIB_DIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIB_DIR, "libnslg_b200.so")
+KV8 = os.path.join(LIB_DIR, "_kv8.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O2",
@@ -75,7 +77,37 @@ def build(force=False, verbose=False, extra=()):
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    build_torch(force, verbose)
     return LIB
+
+
+def build_torch(force=False, verbose=False):
+    """Compiles csrc/kv8_torch.cpp against the installed torch (host code; it calls the
+    shared library beside it); returns its path."""
+    import sysconfig
+
+    import torch
+    src = os.path.join(CSRC, "kv8_torch.cpp")
+    stamp = os.path.join(BUILD, "kv8_torch." + torch.__version__)      # another torch: again
+    if not force and os.path.exists(stamp) and not _stale(KV8, [src, *_headers()]):
+        return KV8
+    t = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(nvcc()))
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", src, "-o", KV8]
+    for d in (INCLUDE, os.path.join(t, "include"),
+              os.path.join(t, "include", "torch", "csrc", "api", "include"),
+              os.path.join(cuda, "include"), sysconfig.get_paths()["include"]):
+        cmd += ["-I", d]
+    cmd += ["-L", os.path.join(t, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda",
+            "-ltorch_python", "-L", LIB_DIR, "-lnslg_b200", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on kv8_torch.cpp:\n{r.stdout}\n{r.stderr}")
+    open(stamp, "w").close()
+    return KV8
 
 
 def main():

@@ -4,7 +4,6 @@ Each op checks devices, dtypes and layouts, passes raw pointers and the current 
 stream to the native library, and raises on any non-zero status.  Nothing here
 computes on the CPU: the ops need CUDA tensors and the built library.
 """
-import ctypes
 import os
 import threading
 
@@ -72,7 +71,6 @@ class _DeviceState:
     def __init__(self):
         self.lock = threading.Lock()
         self.ws = {}
-        self.stream_ws = {}
         self.status = {}
 
     def workspace(self, device, nbytes):
@@ -87,25 +85,6 @@ class _DeviceState:
                 buf = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
                 self.ws[device] = buf
             return buf
-
-    def stream_workspace(self, device, stream, nbytes):
-        """Scratch that starts zeroed and that every kernel leaves with its counts at zero,
-        one per stream (calls on two streams may overlap) and one per graph capture (so may
-        the replays of two graphs; there the zeroing is captured, once a graph). Allocated on
-        the stream that uses it, so a regrown one is only reused behind its readers."""
-        cap = 0
-        if torch.cuda.is_current_stream_capturing():
-            cid = ctypes.c_uint64()
-            N.call("nslg_stream_capture_id", stream, ctypes.byref(cid))
-            cap = cid.value
-        key = (device, stream)
-        ent = self.stream_ws.get((key, cap > 0))
-        if ent is not None and ent[0] == cap and ent[1].numel() >= nbytes:
-            return ent[1]
-        with torch.cuda.device(device):
-            buf = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
-        self.stream_ws[(key, cap > 0)] = (cap, buf)
-        return buf
 
     def status_word(self, device):
         st = self.status.get(device)
@@ -486,7 +465,8 @@ def argmax_rows(x, index_offset=0, values=False):
 
 # ---------------------------------------------------------------- 8-bit KV cache
 # One layer of the cache: e4m3 codes [num_pages, Hkv, page_size, D] and a fp32 scale per
-# (page, kv head) for K and for V (kv8_pages allocates them); value = code * scale.
+# (page, kv head) for K and for V (kv8_pages allocates them); value = code * scale. The
+# checks, outputs, scratch and streams of these ops are csrc/kv8_torch.cpp.
 KV8_DTYPE = torch.float8_e4m3fn
 
 
@@ -497,56 +477,6 @@ def kv8_pages(num_pages, page_size, hkv, d, device):
             torch.zeros(shape, dtype=KV8_DTYPE, device=device),
             torch.zeros((num_pages, hkv), dtype=torch.float32, device=device),
             torch.zeros((num_pages, hkv), dtype=torch.float32, device=device))
-
-
-def _kv8_cache(dev, pool_k, pool_v, scale_k, scale_v, kv_indptr, kv_indices, kv_last_page_len):
-    """Checks one layer of the cache and a page list on device ``dev``; returns (num_pages,
-    Hkv, page_size, D, batch)."""
-    if pool_k.dim() != 4 or pool_k.shape != pool_v.shape:
-        raise ValueError("kv8 pools must be [num_pages, Hkv, page_size, D], K and V alike")
-    num_pages, hkv, ps, d = pool_k.shape
-    for t in (pool_k, pool_v):
-        if t.dtype != KV8_DTYPE:
-            raise TypeError(f"kv8 pools are float8_e4m3fn, got {t.dtype}")
-        if not t.is_contiguous():
-            raise ValueError("kv8 pool layers must be contiguous")
-    for t in (scale_k, scale_v):
-        if t.dtype != torch.float32 or t.shape != (num_pages, hkv) or not t.is_contiguous():
-            raise ValueError("kv8 scales must be contiguous float32 [num_pages, Hkv]")
-    for t in (kv_indptr, kv_indices, kv_last_page_len):
-        if t.dtype != torch.int32 or not t.is_contiguous():
-            raise ValueError("CSR arrays must be contiguous int32")
-    batch = kv_indptr.numel() - 1
-    if batch < 0 or kv_last_page_len.numel() < batch:
-        raise ValueError("kv_indptr needs batch + 1 entries and kv_last_page_len batch")
-    for t in (pool_k, pool_v, scale_k, scale_v, kv_indptr, kv_indices, kv_last_page_len):
-        if t.device != dev:
-            raise RuntimeError(f"nanoslg_b200 kernels need CUDA tensors of one device: {t.device} "
-                               f"beside {dev}")
-    return num_pages, hkv, ps, d, batch
-
-
-def _kv8_rows(x, name, hkv, d):
-    """(rows, row stride) of [..., H, D] rows whose head_dim is the cache's."""
-    if x.shape[-1] != d or x.dim() < 3 or x.shape[-2] % hkv:
-        raise ValueError(f"{name}: {tuple(x.shape)} does not go with {hkv} kv heads of {d}")
-    return _rows(x, name)
-
-
-def _index_rows(qo_indptr, q_row_start, batch, dev):
-    for t, n in ((qo_indptr, batch + 1), (q_row_start, batch)):
-        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous() or t.numel() != n
-                              or t.device != dev):
-            raise ValueError("qo_indptr (batch + 1) and q_row_start (batch) must be contiguous "
-                             "int32 on the rows' device")
-
-
-def _kv8_call(dev, name, *args):
-    """N.call with ``dev`` current (the launch goes to the current device)."""
-    if dev.index == torch.cuda.current_device():
-        return N.call(name, *args)
-    with torch.cuda.device(dev):
-        return N.call(name, *args)
 
 
 def rope_kv8_append(q, k, v, cos, sin, pool_k, pool_v, scale_k, scale_v, qo_indptr, max_qo_len,
@@ -564,45 +494,9 @@ def rope_kv8_append(q, k, v, cos, sin, pool_k, pool_v, scale_k, scale_v, qo_indp
     are), or None when q is None. With ``rotate=False`` q and k are taken as already
     rotated, cos and sin are ignored.
     """
-    _need_cuda(q, k, v)
-    dev = k.device
-    dt = _dtype_code(k)
-    num_pages, hkv, ps, d, batch = _kv8_cache(dev, pool_k, pool_v, scale_k, scale_v, kv_indptr,
-                                              kv_indices, kv_last_page_len)
-    _index_rows(qo_indptr, q_row_start, batch, dev)
-    nk, ks = _kv8_rows(k, "k", hkv, d)
-    nv, vs = _kv8_rows(v, "v", hkv, d)
-    if nk != nv or k.dtype != v.dtype or k.shape[-2] != hkv or v.shape[-2] != hkv or v.device != dev:
-        raise ValueError("k and v must have the same rows and type and the cache's kv heads")
-    hq, qs = hkv, 0
-    if q is not None:
-        nq, qs = _kv8_rows(q, "q", hkv, d)
-        hq = q.shape[-2]
-        if nq != nk or q.dtype != k.dtype or q.device != dev:
-            raise ValueError("q must match k in row count, dtype and device")
-        if q_out is None:
-            q_out = torch.empty((nq, hq, d), dtype=q.dtype, device=dev)
-        elif (q_out.dtype != q.dtype or q_out.device != dev or not q_out.is_contiguous()
-              or q_out.numel() != nq * hq * d):
-            raise ValueError("q_out must be contiguous [rows, Hq, D] of q's dtype")
-    elif q_out is not None:
-        raise ValueError("q_out given without q")
-    rows = 0
-    if rotate:
-        for t in (cos, sin):
-            if (t is None or t.dtype != torch.float32 or not t.is_contiguous() or t.dim() != 2
-                    or t.shape[1] != d or t.device != dev):
-                raise ValueError("cos/sin tables must be contiguous float32 [rows, D]")
-        rows = min(cos.shape[0], sin.shape[0])
-    else:
-        cos = sin = None
-    _kv8_call(dev, "nslg_rope_kv8_append", dt, batch, hq, hkv, d, ps, _ptr(q), qs, k.data_ptr(),
-              ks, v.data_ptr(), vs, nk, _ptr(q_out), _ptr(cos), _ptr(sin), rows,
-              pool_k.data_ptr(), pool_v.data_ptr(), scale_k.data_ptr(), scale_v.data_ptr(),
-              num_pages, qo_indptr.data_ptr(), _ptr(q_row_start), int(max_qo_len),
-              kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_last_page_len.data_ptr(),
-              status_word(dev).data_ptr(), _stream(k))
-    return q_out
+    return N.kv8().append(q, k, v, cos, sin, pool_k, pool_v, scale_k, scale_v, kv_indptr,
+                          kv_indices, kv_last_page_len, qo_indptr, max_qo_len, q_row_start,
+                          q_out, rotate)
 
 
 def kv8_gather(pool_k, pool_v, scale_k, scale_v, kv_indptr, kv_indices, kv_last_page_len, dtype,
@@ -610,61 +504,17 @@ def kv8_gather(pool_k, pool_v, scale_k, scale_v, kv_indptr, kv_indices, kv_last_
     """The listed pages read back as values: (k, v), each [kv_indices.numel(), page_size,
     Hkv, D] of ``dtype``, page j of the list at row j, zeros behind a sequence's last token.
     Rows behind the list (kv_indptr[-1]) are left as they are."""
-    _need_cuda(pool_k)
-    dev = pool_k.device
-    num_pages, hkv, ps, d, batch = _kv8_cache(dev, pool_k, pool_v, scale_k, scale_v, kv_indptr,
-                                              kv_indices, kv_last_page_len)
-    if dtype not in _DTYPES:
-        raise TypeError(f"nanoslg_b200 kernels support bfloat16, float16 and float32, got {dtype}")
-    n = kv_indices.numel()
-    shape = (n, ps, hkv, d)
-    if out is None:
-        out = (torch.empty(shape, dtype=dtype, device=dev),
-               torch.empty(shape, dtype=dtype, device=dev))
-    for t in out:
-        if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or t.device != dev:
-            raise ValueError(f"kv8_gather: the outputs must be contiguous {shape} of {dtype}")
-    _kv8_call(dev, "nslg_kv8_gather", _DTYPES[dtype], batch, hkv, d, ps, pool_k.data_ptr(),
-              pool_v.data_ptr(), scale_k.data_ptr(), scale_v.data_ptr(), num_pages,
-              kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_last_page_len.data_ptr(), n,
-              out[0].data_ptr(), out[1].data_ptr(), status_word(dev).data_ptr(),
-              _stream(pool_k))
-    return out
+    k, v = (None, None) if out is None else out
+    return N.kv8().gather(pool_k, pool_v, scale_k, scale_v, kv_indptr, kv_indices,
+                          kv_last_page_len, dtype, k, v)
 
 
 def paged_decode_kv8(q, pool_k, pool_v, scale_k, scale_v, kv_indptr, kv_indices,
                      kv_last_page_len, sm_scale, out=None):
     """``paged_decode`` over the 8-bit cache: one query per sequence, q [B, Hq, D] -> out
     [B, Hq, D], zeros for a sequence without pages."""
-    _need_cuda(q)
-    dev = q.device
-    dt = _dtype_code(q)
-    num_pages, hkv, ps, d, batch = _kv8_cache(dev, pool_k, pool_v, scale_k, scale_v, kv_indptr,
-                                              kv_indices, kv_last_page_len)
-    nb, qs = _kv8_rows(q, "q", hkv, d)
-    hq = q.shape[-2]
-    if nb != batch:
-        raise ValueError(f"paged_decode_kv8: {nb} queries for {batch} sequences")
-    if out is None:
-        out = torch.empty((nb, hq, d), dtype=q.dtype, device=dev)
-    os_ = _kv8_out(out, q, nb)
-    wsb = N.lib().nslg_decode_kv8_workspace_bytes(nb, hq, hkv, d)
-    stream = _stream(q)
-    ws = _STATE.stream_workspace(dev, stream, wsb)
-    _kv8_call(dev, "nslg_paged_decode_kv8", dt, nb, hq, hkv, d, ps, q.data_ptr(), qs,
-              out.data_ptr(), os_, pool_k.data_ptr(), pool_v.data_ptr(), scale_k.data_ptr(),
-              scale_v.data_ptr(), num_pages, kv_indptr.data_ptr(), kv_indices.data_ptr(),
-              kv_last_page_len.data_ptr(), float(sm_scale), ws.data_ptr(), ws.numel(),
-              status_word(dev).data_ptr(), stream)
-    return out
-
-
-def _kv8_out(out, q, rows):
-    """Row stride of an output that has q's rows and heads."""
-    n, stride = _rows(out, "out")
-    if n != rows or out.shape[-2:] != q.shape[-2:] or out.dtype != q.dtype or out.device != q.device:
-        raise ValueError("out must have q's rows, heads, head_dim, dtype and device")
-    return stride
+    return N.kv8().decode(q, pool_k, pool_v, scale_k, scale_v, kv_indptr, kv_indices,
+                          kv_last_page_len, sm_scale, out)
 
 
 def paged_prefill_kv8(q, qo_indptr, max_qo_len, pool_k, pool_v, scale_k, scale_v, kv_indptr,
@@ -674,30 +524,5 @@ def paged_prefill_kv8(q, qo_indptr, max_qo_len, pool_k, pool_v, scale_k, scale_v
     (q [rows, Hq, D] or [B, S, Hq, D]) over its pages. out has q's row layout; rows of no
     sequence are left as they are: in the out made here they are zeros with ``q_row_start``
     (padded rows) and undefined without (packed rows)."""
-    _need_cuda(q)
-    dev = q.device
-    dt = _dtype_code(q)
-    num_pages, hkv, ps, d, batch = _kv8_cache(dev, pool_k, pool_v, scale_k, scale_v, kv_indptr,
-                                              kv_indices, kv_last_page_len)
-    _index_rows(qo_indptr, q_row_start, batch, dev)
-    nrows, qs = _kv8_rows(q, "q", hkv, d)
-    hq = q.shape[-2]
-    if out is None:
-        out = (torch.empty if q_row_start is None else torch.zeros)(q.shape, dtype=q.dtype,
-                                                                     device=dev)
-    os_ = _kv8_out(out, q, nrows)
-    if nrows == 0 or batch == 0 or max_qo_len == 0:
-        return out
-    n = kv_indices.numel()
-    lib, stream, most = N.lib(), _stream(q), int(max_qo_len)
-    ws = _STATE.stream_workspace(dev, stream,
-                                 lib.nslg_prefill_kv8_workspace_bytes(hq, hkv, d, most))
-    stb = lib.nslg_prefill_kv8_staging_bytes(dt, hq, hkv, d, ps, most, n)
-    staging = torch.empty(stb, dtype=torch.uint8, device=dev) if stb else None
-    _kv8_call(dev, "nslg_paged_prefill_kv8", dt, batch, hq, hkv, d, ps, q.data_ptr(), qs, nrows,
-              out.data_ptr(), os_, qo_indptr.data_ptr(), _ptr(q_row_start), most,
-              pool_k.data_ptr(), pool_v.data_ptr(), scale_k.data_ptr(), scale_v.data_ptr(),
-              num_pages, kv_indptr.data_ptr(), kv_indices.data_ptr(),
-              kv_last_page_len.data_ptr(), n, float(sm_scale), 1 if causal else 0,
-              ws.data_ptr(), ws.numel(), _ptr(staging), stb, status_word(dev).data_ptr(), stream)
-    return out
+    return N.kv8().prefill(q, qo_indptr, max_qo_len, pool_k, pool_v, scale_k, scale_v, kv_indptr,
+                           kv_indices, kv_last_page_len, sm_scale, causal, q_row_start, out)

@@ -113,42 +113,77 @@ def test_gather_and_prefill_refusals(lib):
     assert rc == N.ERR_ARG and b"null" in lib.nslg_last_error()
 
 
-def test_ops_refuse_cpu_tensors_and_wrong_layouts():
-    pool = ops.kv8_pages(4, 16, 2, 64, "cpu")
-    assert pool[0].shape == (4, 2, 16, 64) and pool[2].shape == (4, 2)
-    i = torch.zeros(2, dtype=torch.int32)
-    q = torch.zeros(1, 4, 64, dtype=torch.bfloat16)
-    with pytest.raises(RuntimeError, match="CUDA"):
-        ops.paged_decode_kv8(q, *pool, i, i, i, 0.1)
-    with pytest.raises(RuntimeError, match="CUDA"):
-        ops.paged_prefill_kv8(q, i, 1, *pool, i, i, i, 0.1)
-    with pytest.raises(RuntimeError, match="CUDA"):
-        ops.kv8_gather(*pool, i, i, i, torch.bfloat16)
-    with pytest.raises(RuntimeError, match="CUDA"):
-        ops.rope_kv8_append(None, q, q, None, None, *pool, i, 1, i, i, i, rotate=False)
-    cpu = torch.device("cpu")
+def _calls(row, pool, i, bad):
+    """The four operators on one row, with arguments replaced by name."""
+    a = dict(q=row, k=row[:, :2], v=row[:, :2], cos=torch.zeros(8, 64), sin=torch.zeros(8, 64), pool_k=pool[0],
+             pool_v=pool[1], scale_k=pool[2], scale_v=pool[3], qo_indptr=i, max_qo_len=1, kv_indptr=i,
+             kv_indices=i, kv_last_page_len=i, sm_scale=0.1, dtype=torch.bfloat16, out=None, q_out=None) | bad
+    cache = [a[n] for n in ("pool_k", "pool_v", "scale_k", "scale_v")]
+    seqs = [a[n] for n in ("kv_indptr", "kv_indices", "kv_last_page_len")]
+    return {"append": lambda: ops.rope_kv8_append(a["q"], a["k"], a["v"], a["cos"], a["sin"], *cache,
+                                                  a["qo_indptr"], a["max_qo_len"], *seqs, q_out=a["q_out"],
+                                                  q_row_start=a.get("q_row_start")),
+            "gather": lambda: ops.kv8_gather(*cache, *seqs, a["dtype"], out=a["out"]),
+            "decode": lambda: ops.paged_decode_kv8(a["q"], *cache, *seqs, a["sm_scale"], out=a["out"]),
+            "prefill": lambda: ops.paged_prefill_kv8(a["q"], a["qo_indptr"], a["max_qo_len"], *cache, *seqs,
+                                                     a["sm_scale"], out=a["out"],
+                                                     q_row_start=a.get("q_row_start"))}
 
-    def check(a=pool[0], b=pool[1], c=pool[2], d=pool[3], ptr=i, idx=i, lpl=i):
-        return ops._kv8_cache(cpu, a, b, c, d, ptr, idx, lpl)
-    assert check() == (4, 2, 16, 64, 1)
-    with pytest.raises(TypeError, match="float8"):
-        check(a=pool[0].float())
-    with pytest.raises(ValueError, match="alike"):
-        check(b=pool[1][:3])
-    with pytest.raises(ValueError, match="contiguous"):
-        check(a=pool[0].transpose(2, 3), b=pool[1].transpose(2, 3))
-    with pytest.raises(ValueError, match="scales"):
-        check(c=pool[2].double())
-    with pytest.raises(ValueError, match="scales"):
-        check(d=pool[3][:, :1])
-    with pytest.raises(ValueError, match="int32"):
-        check(idx=i.long())
-    with pytest.raises(ValueError, match="entries"):
-        check(ptr=torch.zeros(4, dtype=torch.int32))
-    with pytest.raises(ValueError, match="kv heads"):
-        ops._kv8_rows(torch.zeros(1, 3, 64), "q", 2, 64)
-    with pytest.raises(ValueError, match="kv heads"):
-        ops._kv8_rows(torch.zeros(1, 4, 32), "q", 2, 64)
+
+EVERY = ("append", "gather", "decode", "prefill")
+POOL = ops.kv8_pages(4, 16, 2, 64, "cpu")
+Q = torch.zeros(1, 4, 64, dtype=torch.bfloat16)
+I = torch.zeros(2, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("names,bad,error,what", [
+    (EVERY, dict(), RuntimeError, "CUDA"),
+    (EVERY, dict(pool_k=POOL[0].float()), TypeError, "float8_e4m3fn"),
+    (EVERY, dict(pool_v=POOL[1].view(torch.uint8)), TypeError, "float8_e4m3fn"),
+    (EVERY, dict(pool_v=POOL[1][:3]), ValueError, "alike"),
+    (EVERY, dict(pool_k=POOL[0][0]), ValueError, "alike"),
+    (EVERY, dict(pool_k=POOL[0].transpose(2, 3), pool_v=POOL[1].transpose(2, 3)), ValueError, "contiguous"),
+    (EVERY, dict(scale_k=POOL[2].double()), ValueError, "scales"),
+    (EVERY, dict(scale_v=POOL[3][:, :1]), ValueError, "scales"),
+    (EVERY, dict(scale_v=POOL[3].t().contiguous().t()), ValueError, "scales"),
+    (EVERY, dict(kv_indices=I.long()), ValueError, "int32"),
+    (EVERY, dict(kv_indptr=torch.zeros(4, dtype=torch.int32)), ValueError, "entries"),
+    (EVERY, dict(kv_indptr=torch.zeros(0, dtype=torch.int32)), ValueError, "entries"),
+    (EVERY, dict(pool_k=None), TypeError, "pool_k"),
+    (("append", "decode", "prefill"), dict(q=torch.zeros(1, 3, 64, dtype=torch.bfloat16)), ValueError, "kv heads"),
+    (("append", "decode", "prefill"), dict(q=torch.zeros(1, 4, 32, dtype=torch.bfloat16)), ValueError, "kv heads"),
+    (("append", "decode", "prefill"), dict(q=torch.zeros(4, 64, dtype=torch.bfloat16)), ValueError, "kv heads"),
+    (("append", "decode", "prefill"), dict(q=torch.zeros(1, 64, 4, dtype=torch.bfloat16).transpose(1, 2)),
+     ValueError, "contiguous"),
+    (("append", "decode", "prefill"), dict(q=torch.zeros(1, 2, 4, 64, dtype=torch.bfloat16).expand(3, 2, 4, 64)),
+     ValueError, "."),
+    (("decode", "prefill"), dict(q=Q.double()), TypeError, "bfloat16, float16 and float32"),
+    (("gather",), dict(dtype=torch.float64), TypeError, "bfloat16, float16 and float32"),
+    (("gather",), dict(dtype="bf16"), TypeError, "dtype"),
+    (("gather",), dict(out=(Q, Q)), ValueError, "outputs"),
+    (("decode",), dict(q=torch.zeros(2, 4, 64, dtype=torch.bfloat16)), ValueError, "2 queries for 1"),
+    (("decode", "prefill"), dict(out=Q.float()), ValueError, "out must"),
+    (("decode", "prefill"), dict(out=torch.zeros(2, 4, 64, dtype=torch.bfloat16)), ValueError, "out must"),
+    (("decode", "prefill"), dict(sm_scale="x"), TypeError, "."),
+    (("append", "prefill"), dict(qo_indptr=torch.zeros(3, dtype=torch.int32)), ValueError, "qo_indptr"),
+    (("append", "prefill"), dict(q_row_start=I), ValueError, "q_row_start"),
+    (("append", "prefill"), dict(max_qo_len=1 << 40), ValueError, "range"),
+    (("append",), dict(k=Q), ValueError, "kv heads"),
+    (("append",), dict(v=Q[:, :2].float()), ValueError, "same rows"),
+    (("append",), dict(q=Q.float()), ValueError, "q must match"),
+    (("append",), dict(q=None, q_out=Q), ValueError, "without q"),
+    (("append",), dict(q_out=Q.float()), ValueError, "q_out must"),
+    (("append",), dict(cos=None), ValueError, "cos/sin"),
+    (("append",), dict(sin=torch.zeros(8, 32)), ValueError, "cos/sin"),
+    (("append",), dict(cos=torch.zeros(8, 64).double()), ValueError, "cos/sin"),
+])
+def test_ops_refuse(lib, names, bad, error, what):
+    """Layouts and types are refused before the device is looked at; sound CPU tensors then are
+    for being on the CPU."""
+    calls = _calls(Q, POOL, I, bad)
+    for n in names:
+        with pytest.raises(error, match=what):
+            calls[n]()
 
 
 def test_manager_bookkeeping_does_not_depend_on_the_cache_type():
