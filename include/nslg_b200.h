@@ -439,15 +439,10 @@ int nslg_paged_decode_kv8(int dtype, int batch, int num_qo_heads, int num_kv_hea
                           const int32_t* kv_last_page_len, float sm_scale, void* workspace,
                           int64_t workspace_bytes, uint32_t* dev_status, void* stream);
 
-/* Scratch of nslg_paged_prefill_kv8: the workspace has the decode's rules (zeroed before its
- * first use, its counts left at zero; the same buffer may serve both calls). The staging
- * area, for prompts, holds the listed pages as 16-bit values while the call runs and needs
- * no clearing; its size is 0 where the call does not use it. num_indices is the capacity of
- * the page list (kv_indptr[batch] <= num_indices). */
+/* Bytes of scratch nslg_paged_prefill_kv8 needs, under the decode's rules (zeroed before its
+ * first use, its counts left at zero; the same buffer may serve both calls). */
 int64_t nslg_prefill_kv8_workspace_bytes(int num_qo_heads, int num_kv_heads, int head_dim,
                                          int max_qo_len);
-int64_t nslg_prefill_kv8_staging_bytes(int dtype, int num_qo_heads, int num_kv_heads, int head_dim,
-                                       int page_size, int max_qo_len, int64_t num_indices);
 
 /* nslg_paged_prefill over the 8-bit cache: the same rows, mask and head conventions. Rows of
  * no sequence are left as they are; a row that sees no position (qo_len(b) > kv_len(b)) is
@@ -458,9 +453,9 @@ int nslg_paged_prefill_kv8(int dtype, int batch, int num_qo_heads, int num_kv_he
                            const int32_t* q_row_start, int max_qo_len, const void* codes_k,
                            const void* codes_v, const float* scale_k, const float* scale_v,
                            int64_t num_pages, const int32_t* kv_indptr, const int32_t* kv_indices,
-                           const int32_t* kv_last_page_len, int64_t num_indices, float sm_scale,
-                           int causal, void* workspace, int64_t workspace_bytes, void* staging,
-                           int64_t staging_bytes, uint32_t* dev_status, void* stream);
+                           const int32_t* kv_last_page_len, float sm_scale, int causal,
+                           void* workspace, int64_t workspace_bytes, uint32_t* dev_status,
+                           void* stream);
 
 /* The number of the graph capture that `stream` is part of, 0 when it is not capturing: a
  * caller that keeps a workspace per stream gives each captured graph one of its own. */

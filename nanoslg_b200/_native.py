@@ -89,10 +89,9 @@ SIGNATURES = {
     "nslg_paged_decode_kv8": (_i32, [_i32] * 6 + [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64,
                                      _vp, _vp, _vp, _f32, _vp, _i64, _vp, _vp]),
     "nslg_prefill_kv8_workspace_bytes": (_i64, [_i32] * 4),
-    "nslg_prefill_kv8_staging_bytes": (_i64, [_i32] * 6 + [_i64]),
     "nslg_paged_prefill_kv8": (_i32, [_i32] * 6 + [_vp, _i64, _i64, _vp, _i64, _vp, _vp, _i32,
-                                      _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _f32,
-                                      _i32, _vp, _i64, _vp, _i64, _vp, _vp]),
+                                      _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _f32, _i32, _vp,
+                                      _i64, _vp, _vp]),
     "nslg_stream_capture_id": (_i32, [_vp, _vp]),
 }
 

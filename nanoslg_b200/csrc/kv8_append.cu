@@ -398,11 +398,6 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8App
 // listed one are left as they are. A thread takes 16 codes of one head row: 16-byte loads,
 // 16-byte stores, consecutive threads along the output. Bound by its bytes (one read and two
 // or four written per element).
-//
-// kStage: the pages staged for the 16-bit prefill kernel, which reads them through an
-// identity page list (`ids`). There the value of a masked position still meets a probability
-// of 0 in a product, so the NaN of a V block is moved to its K block, whose scores are masked
-// by selection; and rows that see no position, which that kernel does not visit, are zeroed.
 constexpr int kGatherThreads = 256;
 
 template <typename T>
@@ -421,28 +416,13 @@ __device__ __forceinline__ void store16(T* dst, const uint4& c, float sc) {
     *reinterpret_cast<uint4*>(dst + i) = *reinterpret_cast<const uint4*>(v + i);
 }
 
-template <typename T, bool kStage>
+template <typename T>
 __global__ void __launch_bounds__(kGatherThreads) kv8_gather_kernel(const Kv8GatherParams p) {
   pdl_wait();
   pdl_trigger();
   __shared__ int s_fill;
   const int64_t j = blockIdx.x;
   const int tid = threadIdx.x;
-  if constexpr (kStage) {
-    for (int64_t b = j; b < p.batch; b += gridDim.x) {
-      const int q0 = p.qo_indptr[b], len = p.qo_indptr[b + 1] - q0;
-      const int np = p.kv_indptr[b + 1] - p.kv_indptr[b];
-      const int kv_len = np > 0 ? (np - 1) * p.page_size + p.kv_lpl[b] : 0;
-      const int none = kv_len == 0 ? len : p.causal ? len - kv_len : 0;
-      const int64_t row0 = p.q_row_start != nullptr ? p.q_row_start[b] : q0;
-      if (none <= 0 || len > p.max_qo_len || row0 < 0 || row0 + len > p.num_rows) continue;
-      const int words = p.hq * p.d * static_cast<int>(sizeof(T)) / 16;
-      for (int64_t i = tid; i < static_cast<int64_t>(none) * words; i += kGatherThreads)
-        reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (row0 + i / words) * p.out_stride)[i % words] =
-            make_uint4(0u, 0u, 0u, 0u);
-    }
-    if (tid == 0) p.ids[j] = static_cast<int32_t>(j);
-  }
   if (j >= p.kv_indptr[p.batch]) return;
   const int64_t page = p.kv_indices[j];
   for (int b = tid; b < p.batch; b += kGatherThreads) {
@@ -465,10 +445,6 @@ __global__ void __launch_bounds__(kGatherThreads) kv8_gather_kernel(const Kv8Gat
       cv = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.codes_v) + off);
       sk = p.scale_k[blk0 + h];
       sv = p.scale_v[blk0 + h];
-      if (kStage && sv != sv) {
-        sk = sv;
-        sv = 0.f;
-      }
     }
     const int64_t dst = (j * n + i) * 16;
     store16(static_cast<T*>(p.out_k) + dst, ck, sk);
@@ -518,17 +494,10 @@ int launch_kv8_append(int dtype, const Kv8AppendParams& p, cudaStream_t stream) 
 int launch_kv8_gather(int dtype, const Kv8GatherParams& p, cudaStream_t stream) {
   const dim3 grid(static_cast<unsigned>(p.num_indices)), block(kGatherThreads);
   if (dtype == NSLG_DTYPE_BF16)
-    return launch_pdl("kv8_gather", kv8_gather_kernel<__nv_bfloat16, false>, grid, block, 0, stream, p);
+    return launch_pdl("kv8_gather", kv8_gather_kernel<__nv_bfloat16>, grid, block, 0, stream, p);
   if (dtype == NSLG_DTYPE_F16)
-    return launch_pdl("kv8_gather", kv8_gather_kernel<__half, false>, grid, block, 0, stream, p);
-  return launch_pdl("kv8_gather", kv8_gather_kernel<float, false>, grid, block, 0, stream, p);
-}
-
-int launch_kv8_stage(int dtype, const Kv8GatherParams& p, cudaStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(p.num_indices)), block(kGatherThreads);
-  if (dtype == NSLG_DTYPE_BF16)
-    return launch_pdl("kv8_stage", kv8_gather_kernel<__nv_bfloat16, true>, grid, block, 0, stream, p);
-  return launch_pdl("kv8_stage", kv8_gather_kernel<__half, true>, grid, block, 0, stream, p);
+    return launch_pdl("kv8_gather", kv8_gather_kernel<__half>, grid, block, 0, stream, p);
+  return launch_pdl("kv8_gather", kv8_gather_kernel<float>, grid, block, 0, stream, p);
 }
 
 }  // namespace nslg

@@ -23,17 +23,22 @@
 // Mathematics of a unit, transposed so that a short group wastes little of an mma: the 16
 // tokens (of K) and 16-dim chunks (of V) are the rows of m16n8k16 products, the query rows
 // their 8 columns (one or two column tiles, NT):
-//   x^T = code_k . q^T  (16 tokens x 8 NT rows), times scale_k * sm_scale * log2 e
-//   p = 2^(x - m)        m: running reference, raised only when x passes it by 8 (p <= 2^8)
-//   o^T = o^T + scale_v * (code_v^T . p^T);  l = l + sum p
+//   s^T = code_k . q^T  (16 tokens x 8 NT rows)
+//   t = s F + E          F = scale_k sm_scale log2(e) / (the row's q factor), E = log2 scale_v
+//   p = 2^(t - M)        M: running reference, raised only when t passes it by 8 (p <= 2^8)
+//   o^T = o^T + code_v^T . p^T;  l = l + 2^-E sum p;  out = o / l
+// The scales cost nothing per element: K's is a factor the score needs anyway, V's joins the
+// exponent, so p is what multiplies the code and M follows the largest of these weights.
+// p is rounded to f16 (2^-11, whatever the activation type) relative to that, so the scales
+// of neighbouring pages may differ by any factor. A block of zeros in V has no E, only a part
+// in l: it takes one kZeroE below the last page's, so that it raises M only where it outweighs
+// the row's other pages by 2^60, and the first page that has an E sets M anew.
 // Against rows-first products (16 query rows, 4 of them in use at a group of 4) this halves
 // the products, the accumulators (32 registers instead of 64 at head_dim 128, so 16 warps
 // fit an SM instead of 8) and the exponentials.
 // Codes become f16 exactly (one cvt per two). q of bf16 becomes f16 exactly too: each row is
 // first multiplied by the power of two that brings its largest magnitude to [2^14, 2^15)
-// (elements 2^-38 below it vanish). p is rounded to f16, 2^-11 relative, whatever the
-// activation type. The products of a page are scaled as fp32 sums, so the scales of
-// neighbouring pages may differ by any factor.
+// (elements 2^-38 below it vanish).
 // Operand layouts: the order of head_dim inside a k step of K.q is free as long as q and K
 // agree, so K fragments are plain ldmatrix words (4 codes = dims 4t .. 4t + 3 of a 16-dim
 // chunk) and q is loaded to match. V^T comes from ldmatrix.trans of 16-bit units (two dims
@@ -66,6 +71,7 @@ constexpr int kMaxStages = 8;
 constexpr int kStaticSmem = 2048;     // at least the kernel's __shared__ arrays
 constexpr int kMaxSmem = 232448;      // 227 KiB
 constexpr int kSmemBatch = 2048;      // batches up to this size keep the page list's bounds in smem
+constexpr float kZeroE = 60.f;
 constexpr float kHeadroom = 8.f;      // log2 of the largest probability before m is raised
 
 struct TcParams : Kv8AttnParams {
@@ -280,7 +286,7 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
   // ---- metadata of 32 units at a time, one per lane
   struct Meta {
     int blk, vid, j;       // block (page * kv heads + head; -1: a bad page), sequence, page of it
-    float sk, sv;
+    float sk, sv;          // scale_k; scale_v, 0 where V is zeros or not finite
   };
   auto locate = [&](int u, int& vid, int& first) {   // unit u: its sequence and page list entry
     const int b = seq_of(indptr, p.batch, u / hm);
@@ -336,6 +342,8 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
   float m[NT][2], nb[NT][2], l[NT][2], f[NT][2];   // of rows 2tq, 2tq + 1
   int pos[NT][2];                        // last position they see
   int low = 0;                           // ... the least of all the tile's rows
+  float ev = 0.f, iv = 1.f;              // E of the last page that had one, 2^-E
+  bool seen = false;                     // ... whether there was one
   int vid = -1;
   Tile t{};
   bool ok = true;
@@ -349,6 +357,9 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
     t.qo_len = new_rows(p, t.b, &t.row0);
     t.kv_len = (indptr[t.b + 1] - indptr[t.b] - 1) * kPS + lpl[t.b];
     low = 0x7fffffff;
+    ev = 0.f;
+    iv = 1.f;
+    seen = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int pair = t.r0 + nt * 8 + g;
@@ -501,11 +512,17 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
         begin(v);
       }
       float sk = __shfl_sync(0xffffffffu, cur.sk, i);
-      float sv = __shfl_sync(0xffffffffu, cur.sv, i);
-      if (sv != sv) {        // NaN rides on the scores
-        sk = sv;
-        sv = 0.f;
+      const float sv = __shfl_sync(0xffffffffu, cur.sv, i);
+      const bool plain = sv > 0.f && sv < INFINITY;
+      if (sv != sv) sk = sv;       // NaN rides on the scores
+      const bool anew = plain && !seen;
+      if (plain) {
+        ev = __log2f(sv);          // any value near log2 sv will do: iv is its inverse
+        iv = fast_exp2(-ev);
+        seen = true;
       }
+      const float eu = plain ? ev : fmaxf(ev - kZeroE, -120.f);
+      const float iu = plain ? iv : fast_exp2(-eu);
       const int tok0 = __shfl_sync(0xffffffffu, cur.j, i) * kPS;
       ok = __all_sync(0xffffffffu, mbar_wait(&full[slot], phase));
       if (!ok) {
@@ -540,12 +557,12 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
       // a page some row does not see whole, or that ends the sequence
       const int held = t.kv_len - tok0;
       const bool edge = low < tok0 + kPS - 1 || held < kPS;
-      bool raise = false;
+      bool raise = anew;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          s[nt][e] *= f[nt][e & 1] * sk;
+          s[nt][e] = fmaf(s[nt][e], f[nt][e & 1] * sk, eu);
           if (edge && tok0 + (e >> 1) * 8 + g > pos[nt][e & 1]) s[nt][e] = -INFINITY;
           raise |= s[nt][e] > m[nt][e & 1] + kHeadroom;
         }
@@ -560,36 +577,39 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-            const float mn = fmaxf(m[nt][e], x);
-            const float cf = mn == -INFINITY ? 1.f : fast_exp2(m[nt][e] - mn);
+            // anew: o is all zeros, M may go down (where the row sees the page)
+            const float mn = anew && x > -INFINITY ? x : fmaxf(m[nt][e], x);
+            const float cf = mn == -INFINITY || m[nt][e] == -INFINITY ? 1.f : fast_exp2(m[nt][e] - mn);
             m[nt][e] = mn;
             nb[nt][e] = mn == -INFINITY ? 0.f : -mn;
             l[nt][e] *= cf;
+            if (!anew)
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
-              o[nt][k][e] *= cf;
-              o[nt][k][2 + e] *= cf;
-            }
+              for (int k = 0; k < KS; ++k) {
+                o[nt][k][e] *= cf;
+                o[nt][k][2 + e] *= cf;
+              }
           }
       }
       uint32_t pb[NT][2];      // p^T: tokens 0-7, 8-15
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        float pr[4];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float p0 = fast_exp2(s[nt][2 * e] + nb[nt][0]);
-          const float p1 = fast_exp2(s[nt][2 * e + 1] + nb[nt][1]);
-          l[nt][0] += p0;
-          l[nt][1] += p1;
-          pb[nt][e] = movmatrix_trans(pack_f16x2(p0, p1));
-        }
-      // ---- o^T += scale_v * (V^T . p^T)
+        for (int e = 0; e < 4; ++e) pr[e] = fast_exp2(s[nt][e] + nb[nt][e & 1]);
+        l[nt][0] = fmaf(pr[0] + pr[2], iu, l[nt][0]);
+        l[nt][1] = fmaf(pr[1] + pr[3], iu, l[nt][1]);
+        pb[nt][0] = movmatrix_trans(pack_f16x2(pr[0], pr[1]));
+        pb[nt][1] = movmatrix_trans(pack_f16x2(pr[2], pr[3]));
+      }
+      // ---- o^T += V^T . p^T
       uint32_t clear[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
-      if (held < kPS) {     // codes behind the last token count as 0
+      if (held < kPS || !plain) {   // codes behind the last token, and of a scale of 0 or NaN, count as 0
+        const int live = plain ? held : 0;
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          clear[e] = (tq * 2 + 8 * e < held ? 0x00FF00FFu : 0u) |
-                     (tq * 2 + 8 * e + 1 < held ? 0xFF00FF00u : 0u);
+          clear[e] = (tq * 2 + 8 * e < live ? 0x00FF00FFu : 0u) |
+                     (tq * 2 + 8 * e + 1 < live ? 0xFF00FF00u : 0u);
       }
 #pragma unroll
       for (int k = 0; k < KS; k += 2) {
@@ -604,12 +624,8 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
                                  f16x2_from_e4m3x2(static_cast<uint16_t>(w[2 * e + 1])),
                                  f16x2_from_e4m3x2(static_cast<uint16_t>(w[2 * e + 1] >> 16))};
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float pv[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_f16_16816(pv, a, pb[nt][0], pb[nt][1]);
-#pragma unroll
-            for (int x = 0; x < 4; ++x) o[nt][k + e][x] = fmaf(pv[x], sv, o[nt][k + e][x]);
-          }
+          for (int nt = 0; nt < NT; ++nt)
+            mma_f16_16816(o[nt][k + e], a, pb[nt][0], pb[nt][1]);
         }
       }
       __syncwarp();        // the slot has been read by every lane

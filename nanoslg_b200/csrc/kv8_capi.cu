@@ -8,7 +8,7 @@ using namespace nslg;
 
 namespace {
 
-constexpr int kStageRows = 64;
+constexpr int kSplitRows = 64;
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
@@ -53,18 +53,6 @@ int check_attention(const std::string& what, int dtype, const Kv8AttnParams& p) 
   if ((rc = check_rows(what, "q", p.q, p.q_stride, width, dtype))) return rc;
   if ((rc = check_rows(what, "out", p.out, p.out_stride, width, dtype))) return rc;
   return NSLG_OK;
-}
-
-// Whether a prefill call reads the pages through a 16-bit copy made for it (launch_kv8_stage)
-// with the kernel of the 16-bit cache.
-bool stages(int dtype, int hq, int hkv, int d, int page_size, int max_qo_len) {
-  return prefill_tc_supported(dtype, hq, hkv, d, page_size) &&
-         static_cast<int64_t>(hq / hkv) * max_qo_len > kStageRows;
-}
-
-// Bytes of the staged K (or V) pages, a multiple of 256.
-int64_t staged_bytes(int hkv, int d, int page_size, int64_t num_indices) {
-  return (num_indices * page_size * hkv * d * 2 + 255) / 256 * 256;
 }
 
 template <typename F>
@@ -241,32 +229,21 @@ int64_t nslg_prefill_kv8_workspace_bytes(int num_qo_heads, int num_kv_heads, int
   return kv8_attn_tc_workspace_bytes(num_qo_heads / num_kv_heads, max_qo_len, head_dim);
 }
 
-int64_t nslg_prefill_kv8_staging_bytes(int dtype, int num_qo_heads, int num_kv_heads, int head_dim,
-                                       int page_size, int max_qo_len, int64_t num_indices) {
-  if (num_qo_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || page_size <= 0 ||
-      max_qo_len < 0 || num_indices < 0 ||
-      !stages(dtype, num_qo_heads, num_kv_heads, head_dim, page_size, max_qo_len))
-    return 0;
-  return staged_bytes(num_kv_heads, head_dim, page_size, num_indices) * 2 + num_indices * 4 + 256;
-}
-
 int nslg_paged_prefill_kv8(int dtype, int batch, int num_qo_heads, int num_kv_heads, int head_dim,
                            int page_size, const void* q, int64_t q_stride, int64_t q_rows,
                            void* out, int64_t out_stride, const int32_t* qo_indptr,
                            const int32_t* q_row_start, int max_qo_len, const void* codes_k,
                            const void* codes_v, const float* scale_k, const float* scale_v,
                            int64_t num_pages, const int32_t* kv_indptr, const int32_t* kv_indices,
-                           const int32_t* kv_last_page_len, int64_t num_indices, float sm_scale,
-                           int causal, void* workspace, int64_t workspace_bytes, void* staging,
-                           int64_t staging_bytes, uint32_t* dev_status, void* stream) {
+                           const int32_t* kv_last_page_len, float sm_scale, int causal,
+                           void* workspace, int64_t workspace_bytes, uint32_t* dev_status,
+                           void* stream) {
   return guarded([&]() -> int {
     const std::string what = "paged_prefill_kv8";
     if (batch == 0 || max_qo_len == 0) return NSLG_OK;
     if (max_qo_len < 0 || q_rows <= 0)
       return set_error(NSLG_ERR_ARG, what + ": bad max_qo_len or q_rows");
     if (!qo_indptr) return set_error(NSLG_ERR_ARG, what + ": null pointer");
-    if (num_indices < 0 || num_indices > 0x7fffffff)
-      return set_error(NSLG_ERR_ARG, what + ": num_indices out of range");
     Kv8AttnParams p{};
     p.codes_k = const_cast<void*>(codes_k);
     p.codes_v = const_cast<void*>(codes_v);
@@ -295,40 +272,9 @@ int nslg_paged_prefill_kv8(int dtype, int batch, int num_qo_heads, int num_kv_he
     const int rc = check_attention(what, dtype, p);
     if (rc) return rc;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (num_indices > 0 && stages(dtype, p.hq, p.hkv, p.d, p.page_size, max_qo_len)) {
-      const int64_t need = nslg_prefill_kv8_staging_bytes(dtype, p.hq, p.hkv, p.d, p.page_size,
-                                                          max_qo_len, num_indices);
-      if (staging == nullptr || staging_bytes < need)
-        return set_error(NSLG_ERR_WORKSPACE, what + ": the staging area needs " +
-                                                 std::to_string(need) + " bytes");
-      const int64_t each = staged_bytes(p.hkv, p.d, p.page_size, num_indices);
-      const uintptr_t at = (reinterpret_cast<uintptr_t>(staging) + 255) & ~static_cast<uintptr_t>(255);
-      Kv8GatherParams g{};
-      static_cast<Kv8Cache&>(g) = p;
-      g.out_k = reinterpret_cast<void*>(at);
-      g.out_v = reinterpret_cast<void*>(at + each);
-      g.ids = reinterpret_cast<int32_t*>(at + 2 * each);
-      g.num_indices = num_indices;
-      g.batch = batch;
-      g.hkv = p.hkv;
-      g.d = p.d;
-      g.page_size = page_size;
-      g.status = dev_status;
-      g.out = out;
-      g.qo_indptr = qo_indptr;
-      g.q_row_start = q_row_start;
-      g.out_stride = out_stride;
-      g.num_rows = q_rows;
-      g.hq = p.hq;
-      g.max_qo_len = max_qo_len;
-      g.causal = p.causal;
-      const int rs = launch_kv8_stage(dtype, g, st);
-      if (rs != NSLG_OK) return rs;
-      return launch_paged_prefill_tc(dtype, batch, p.hq, p.hkv, q, q_stride, q_rows, out, out_stride,
-                                     qo_indptr, q_row_start, max_qo_len, g.out_k, g.out_v,
-                                     num_indices, kv_indptr, g.ids, kv_last_page_len, sm_scale,
-                                     p.causal, dev_status, st);
-    }
+    if (kv8_prefill_tc_supported(dtype, p) &&
+        static_cast<int64_t>(p.hq / p.hkv) * max_qo_len > kSplitRows)
+      return launch_kv8_prefill_tc(dtype, p, st);
     if (kv8_attn_tc_supported(dtype, p))
       return launch_kv8_attention_tc(dtype, p, workspace, workspace_bytes, st);
     return launch_kv8_attention_simt(dtype, p, st);

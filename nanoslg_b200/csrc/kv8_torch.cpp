@@ -364,23 +364,16 @@ PyObject* prefill(PyObject* const* a) {
   if (given == nullptr && start != nullptr) out.zero_();
   if (rq.n > 0) {
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(dev));
-    const int64_t n = c.indices->numel();
     at::Tensor& ws = workspace(
         dev, stream, nslg_prefill_kv8_workspace_bytes(rq.heads, c.hkv, c.d, std::max(most, 0)));
-    const int64_t bytes =
-        nslg_prefill_kv8_staging_bytes(dt, rq.heads, c.hkv, c.d, c.ps, std::max(most, 0), n);
-    at::Tensor staging;
-    if (bytes > 0) staging = empty({bytes}, at::kByte, dev);
     check("nslg_paged_prefill_kv8",
           nslg_paged_prefill_kv8(dt, c.batch, rq.heads, c.hkv, c.d, c.ps, data(&q), rq.stride, rq.n,
                                  out.mutable_data_ptr(), ro.stride, data<int32_t>(&qo),
                                  data<int32_t>(start), most, data(c.k), data(c.v),
                                  data<float>(c.sk), data<float>(c.sv), c.pages,
                                  data<int32_t>(c.indptr), data<int32_t>(c.indices),
-                                 data<int32_t>(c.lpl), n, static_cast<float>(sm), causal ? 1 : 0,
-                                 ws.mutable_data_ptr(), ws.numel(),
-                                 bytes > 0 ? staging.mutable_data_ptr() : nullptr, bytes,
-                                 status_word(dev), stream));
+                                 data<int32_t>(c.lpl), static_cast<float>(sm), causal ? 1 : 0,
+                                 ws.mutable_data_ptr(), ws.numel(), status_word(dev), stream));
   }
   return THPVariable_Wrap(out);
 }

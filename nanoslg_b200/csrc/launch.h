@@ -203,17 +203,8 @@ struct Kv8GatherParams : Kv8Cache {
   int64_t num_indices;
   int batch, hkv, d, page_size;
   uint32_t* status;
-  // staging for the prefill kernel only: the identity page list, and the rows of `out` that
-  // see no position
-  int32_t* ids;
-  void* out;
-  const int32_t* qo_indptr;
-  const int32_t* q_row_start;
-  int64_t out_stride, num_rows;
-  int hq, max_qo_len, causal;
 };
 int launch_kv8_gather(int dtype, const Kv8GatherParams& p, cudaStream_t stream);
-int launch_kv8_stage(int dtype, const Kv8GatherParams& p, cudaStream_t stream);
 
 struct Kv8AttnParams : Kv8Cache {
   const void* q;
@@ -233,5 +224,9 @@ bool kv8_attn_tc_supported(int dtype, const Kv8AttnParams& p);
 int64_t kv8_attn_tc_workspace_bytes(int group, int max_qo_len, int d);
 int launch_kv8_attention_tc(int dtype, const Kv8AttnParams& p, void* workspace,
                             int64_t workspace_bytes, cudaStream_t stream);
+
+// tcgen05 (kv8_prefill_tc.cu): head_dim 128, groups that divide 128.
+bool kv8_prefill_tc_supported(int dtype, const Kv8AttnParams& p);
+int launch_kv8_prefill_tc(int dtype, const Kv8AttnParams& p, cudaStream_t stream);
 
 }  // namespace nslg

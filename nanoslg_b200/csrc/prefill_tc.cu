@@ -85,8 +85,7 @@ struct PrefillParams {
   const int32_t* indices;
   const int32_t* lpl;
   int64_t out_stride, num_pages;
-  int64_t q_rows;
-  int batch, hq, hkv, group, tokens_per_tile, max_qo_len, causal, n_items;
+  int batch, hq, hkv, group, tokens_per_tile, causal, n_items;
   float scale_log2;
   uint32_t* status;
 };
@@ -137,11 +136,6 @@ __device__ __forceinline__ bool finish_item(const PrefillParams& p, const ItemLo
   it.h = L.h;
   const int tpt = p.tokens_per_tile;
   it.qo_len = L.qo1 - L.qo0;
-  if (it.qo_len > 0 &&
-      (it.qo_len > p.max_qo_len || L.rs < 0 || static_cast<int64_t>(L.rs) + it.qo_len > p.q_rows)) {
-    report(p.status, NSLG_DEV_BAD_PLAN);   // rows outside q and out: the sequence is skipped
-    return false;
-  }
   const int ntile_q = (it.qo_len + tpt - 1) / tpt;
   const int npairs = (ntile_q + 1) / 2;
   const int pk = npairs - 1 - L.pk_rev;
@@ -661,8 +655,6 @@ int launch_paged_prefill_tc(int dtype, int batch, int hq, int hkv, const void* q
   p.hkv = hkv;
   p.group = G;
   p.tokens_per_tile = tpt;
-  p.q_rows = q_rows;
-  p.max_qo_len = max_qo_len;
   p.causal = causal;
   p.scale_log2 = sm_scale * 1.4426950408889634f;
   p.status = status;

@@ -77,16 +77,17 @@ def attention(q, k, v, sm_scale, causal=True):
     q, k, v = (np.asarray(t, dtype=np.float64) for t in (q, k, v))
     n, hq, _ = q.shape
     length, hkv = k.shape[0], k.shape[1]
-    out = np.zeros_like(q)
+    out = np.zeros((n, hq, v.shape[2]))
+    if not length:
+        return out
+    seen = np.arange(length)[None] <= np.arange(length - n, length)[:, None] if causal else \
+        np.ones((n, length), bool)
     for h in range(hq):
-        w = q[:, h] @ k[:, h * hkv // hq].T * sm_scale
-        if causal:
-            w[np.arange(length)[None] > np.arange(length - n, length)[:, None]] = -np.inf
-        for i in range(n):
-            m = w[i].max() if length else -np.inf
-            if m == -np.inf:
-                continue
-            p = np.exp(w[i] - m)
-            seen = w[i] > -np.inf
-            out[i, h] = (p[seen] / p[seen].sum()) @ v[seen, h * hkv // hq] if not np.isnan(m) else np.nan
+        kh, vh = k[:, h * hkv // hq], v[:, h * hkv // hq]
+        w = np.where(seen, q[:, h] @ kh.T * sm_scale, -np.inf)
+        m = w.max(1, keepdims=True)
+        p = np.exp(w - np.where(m == -np.inf, 0.0, m))
+        out[:, h] = p / np.where(m == -np.inf, 1.0, p.sum(1, keepdims=True)) @ np.where(np.isnan(vh), 0.0, vh)
+        # a value that is not a number reaches the rows that see it
+        out[:, h][(seen @ np.isnan(vh).any(1)) > 0] = np.nan
     return out

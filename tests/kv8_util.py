@@ -57,18 +57,34 @@ def values(pool, scale, table, length):
     return x.permute(0, 2, 1, 3).reshape(-1, pool.shape[1], pool.shape[3])[:length].numpy()
 
 
-def attention_bound(q, k, v, sm_scale, out, dtype, p_half, causal=True):
+def attention_bound(q, k, v, vs, sm_scale, out, dtype, p_half, causal=True):
     """How far an output may be from the 64-bit ``out``, per element: the output rounded once
-    (half a step of its type), plus, relative to A = sum p |v|: the probabilities rounded to
-    the type the products take (p_half), the fp32 score (D products of at most S in all, each
-    sum rounded), the exponential's argument (2^-24 of up to log2(e) S + its own 2^-22) and the
-    fp32 sums over the keys (at most one rounding a key, numerator and denominator)."""
+    (half a step of its type; 2^-25 where fp16 is subnormal), plus, relative to A = sum p |v|:
+    the weights rounded to the type the products take (p_half), the fp32 score (D products of
+    at most S in all, each sum rounded), the exponential's argument (2^-24 of up to log2(e) S
+    and of the scales' exponents, its own 2^-22) and the fp32 sums over the keys (at most one
+    rounding a key, numerator and denominator); plus, for weights p scale_v that are fp16
+    subnormals beside the row's largest W, at most 2^-25 W times the key's code.
+    ``vs`` [tokens, hkv]: the scales of the V blocks."""
     n, hq, d = q.shape
     length, hkv = k.shape[0], k.shape[1]
     a = kv8.attention(q, k, np.abs(v), sm_scale, causal)
+    w = np.zeros_like(a)
     s = 0.0
     for h in range(hq):
-        if length:
-            s = max(s, float((np.abs(q[:, h]) @ np.abs(k[:, h * hkv // hq]).T).max()) * sm_scale)
-    rel = p_half + (d + 8) * s * 2.0 ** -24 + 2.0 ** -20 + 2 * length * 2.0 ** -24
-    return HALF[dtype] * np.abs(out) + rel * a + 1e-30
+        if not length:
+            break
+        kh = h * hkv // hq
+        s = max(s, float((np.abs(q[:, h]) @ np.abs(k[:, kh]).T).max()) * sm_scale)
+        # p scale_v: attention over the diagonal matrix of the scales
+        one = kv8.attention(q[:, h:h + 1], k[:, kh:kh + 1], np.diag(vs[:, kh])[:, None], sm_scale, causal)
+        codes = np.abs(v[:, kh]) / np.where(vs[:, kh] > 0, vs[:, kh], 1.0)[:, None]
+        w[:, h] = one[:, 0].max(1, keepdims=True) * codes.sum(0)[None]
+    rel = p_half + (d + 40) * s * 2.0 ** -24 + 2.0 ** -19 + 2 * length * 2.0 ** -24
+    half = HALF[dtype] * np.abs(out) + (2.0 ** -25 if dtype == torch.float16 else 0.0)
+    return half + rel * a + (2.0 ** -25 * w if p_half else 0.0) + 1e-30
+
+
+def token_scales(scale, table, length, page_size):
+    """[length, hkv] scales of a sequence's tokens in 64 bits."""
+    return np.repeat(scale.cpu().double().numpy()[np.asarray(table, dtype=int)], page_size, 0)[:length]

@@ -221,8 +221,14 @@ def _check_attention(out, q, cache, tables, lens, counts, row_start, sm_scale, p
         k, v = (U.values(cache[i], cache[2 + i], t, n) for i in range(2))
         qd = q[r].cpu().double().numpy()
         want = kv8.attention(qd, k, v, sm_scale, causal)
-        bound = U.attention_bound(qd, k, v, sm_scale, want, out.dtype, p_half, causal)
-        err = np.abs(out[r].double().numpy() - want)
+        vs = U.token_scales(cache[3], t, n, cache[0].shape[2])
+        bound = U.attention_bound(qd, k, v, vs, sm_scale, want, out.dtype, p_half, causal)
+        got = out[r].double().numpy()
+        # an exact value that the bound takes past the type's largest one (fp16: 65504; from
+        # 65520 on the nearest value is an infinity) may be the infinity of its sign
+        most = torch.finfo(out.dtype).max
+        past = (np.abs(want) + bound > most) & np.isinf(got) & (np.sign(got) == np.sign(want))
+        err = np.where(past, 0.0, np.abs(got - want))
         assert not np.isnan(err).any(), (b, n)
         assert (err <= bound).all(), (b, n, float((err / bound).max()))
 
@@ -284,6 +290,13 @@ PREFILL = [
     (torch.float16, 16, 2, 64, 16, [129], [100], True, 2),
     (torch.float16, 12, 2, 128, 16, [40], [12], True, 0),
     (torch.bfloat16, 34, 2, 128, 16, [20], [6], True, 0),
+    (torch.bfloat16, 64, 4, 128, 16, [300, 77], [300, 40], True, 0),
+    (torch.float16, 4, 4, 128, 16, [700], [260], True, 0),
+    (torch.bfloat16, 8, 2, 128, 16, [513, 128, 129, 1], [70, 128, 129, 1], False, 0),
+    (torch.bfloat16, 16, 8, 128, 16, [256, 127, 384], [256, 127, 300], True, 5),
+    # more work items than SMs
+    (torch.bfloat16, 16, 4, 128, 16, [170 + 9 * i for i in range(24)], [150 + 5 * i for i in range(24)], True, 0),
+    (torch.float16, 8, 8, 128, 16, [400 - 9 * i for i in range(20)], [300 - 9 * i for i in range(20)], True, 0),
     (torch.float32, 4, 2, 64, 16, [32, 20], [32, 1], True, 0),
     (torch.bfloat16, 6, 3, 96, 5, [12, 6], [5, 6], True, 1),
 ]
@@ -331,6 +344,57 @@ def test_prefill_rows_that_see_nothing_are_zeros(dt, d):
     ops.paged_prefill_kv8(q, qo, 5, *cache, *U.csr(tables, lens, ps, DEV), sm, out=out)
     _check_attention(out, q, cache, tables, lens, counts, [0, 5, 9], sm, _p_half(dt))
     assert bool((out[:2] == 0).all()) and bool((out[5:9] == 0).all())
+
+
+@pytest.mark.parametrize("dt,d,rows", [(torch.bfloat16, 128, 1), (torch.float16, 64, 7),
+                                       (torch.bfloat16, 128, 90), (torch.float16, 128, 150),
+                                       (torch.float32, 64, 5)])
+def test_scales_of_neighbouring_pages_may_differ_by_any_factor(dt, d, rows):
+    """V scales over 40 powers of two, K scales over 8 (zeros and non-powers among them): the
+    pages with the large values get next to no weight where K is large."""
+    hq, hkv, n = 8, 2, 333
+    cache = U.random_cache(30, hkv, 16, d, DEV, 31)
+    table = U.page_lists([n], 16, 30, 32)
+    g = torch.Generator().manual_seed(33)
+    for t, lo, hi in ((cache[2], -11, -3), (cache[3], -20, 20)):
+        s = torch.exp2(torch.randint(lo, hi, t.shape, generator=g).float())
+        s[torch.rand(t.shape, generator=g) < 0.15] = 0.0
+        s[int(table[0][3])] = 0.0
+        s[:, 1] *= 1.0 + torch.rand(t.shape[0], generator=g)
+        t.copy_(s)
+    q = (U.rows((rows, hq, d), dt, 34) * 2).to(DEV)
+    sm = 1 / math.sqrt(d)
+    plan = U.csr(table, [n], 16, DEV)
+    qo = torch.tensor([0, rows], dtype=torch.int32, device=DEV)
+    out = ops.paged_prefill_kv8(q, qo, rows, *cache, *plan, sm)
+    _check_attention(out, q, cache, table, [n], [rows], [0], sm, _p_half(dt))
+    if rows == 1:
+        out = ops.paged_decode_kv8(q, *cache, *plan, sm)
+        _check_attention(out, q, cache, table, [n], [1], [0], sm, _p_half(dt))
+
+
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("dt,rows", [(torch.bfloat16, 12), (torch.float16, 150), (torch.bfloat16, 260),
+                                     (torch.float32, 40)])
+def test_a_block_that_is_not_finite_in_a_masked_place(dt, rows, which):
+    """Rows that come before the block see nothing of it; the others are NaN."""
+    hq, hkv, d, n = 8, 2, 128, 300
+    cache = U.random_cache(22, hkv, 16, d, DEV, 41)
+    table = U.page_lists([n], 16, 22, 42)
+    bad = n // 16 - 0                                # the last, partly filled page
+    page = int(table[0][bad])
+    i = "kv".index(which)
+    cache[2 + i][page, 1] = math.nan
+    cache[i].view(torch.uint8)[page, 1] = 0          # as the append leaves such a block
+    q = U.rows((rows, hq, d), dt, 43).to(DEV)
+    sm = 1 / math.sqrt(d)
+    qo = torch.tensor([0, rows], dtype=torch.int32, device=DEV)
+    out = ops.paged_prefill_kv8(q, qo, rows, *cache, *U.csr(table, [n], 16, DEV), sm).cpu()
+    first = bad * 16 - (n - rows)                    # first row that sees the block
+    assert 0 <= first < rows or rows == 12
+    first = max(first, 0)
+    assert bool(torch.isnan(out[first:, 4:]).all())
+    assert bool(torch.isfinite(out[:first]).all()) and bool(torch.isfinite(out[:, :4]).all())
 
 
 def test_attention_bad_pages_are_reported():

@@ -79,7 +79,8 @@ def test_context_steps_are_the_definition(hq, hkv, d, dt, ps, rope):
                 for i, x in enumerate((kk, vv)):
                     np.testing.assert_array_equal(U.values(cache[i], cache[2 + i], st.block_table, start + n), x)
                 want = kv8.attention(qr, kk, vv, 1 / math.sqrt(d))
-                bound = U.attention_bound(qr, kk, vv, 1 / math.sqrt(d), want, dt,
+                vs = U.token_scales(cache[3], st.block_table, start + n, ps)
+                bound = U.attention_bound(qr, kk, vv, vs, 1 / math.sqrt(d), want, dt,
                                           U.HALF[dt] if dt != torch.float32 else 0.0)
                 assert (np.abs(out[b, o:o + n].double().numpy() - want) <= bound).all(), (s, layer)
         mgr.end_forward(ctx)

@@ -106,10 +106,10 @@ def test_gather_and_prefill_refusals(lib):
     rc = lib.nslg_kv8_gather(N.DTYPE_BF16, 1, 2, 128, 16, p, p, p, p, 4, p, p, p, -1, p, p, None, None)
     assert rc == N.ERR_ARG and b"num_indices" in lib.nslg_last_error()
     rc = lib.nslg_paged_prefill_kv8(N.DTYPE_BF16, 1, 8, 2, 128, 16, p, 1024, 0, p, 1024, p, None, 4, p,
-                                    p, p, p, 4, p, p, p, 8, 0.1, 1, None, 0, None, 0, None, None)
+                                    p, p, p, 4, p, p, p, 0.1, 1, None, 0, None, None)
     assert rc == N.ERR_ARG and b"q_rows" in lib.nslg_last_error()
     rc = lib.nslg_paged_prefill_kv8(N.DTYPE_BF16, 1, 8, 2, 128, 16, p, 1024, 4, p, 1024, None, None, 4,
-                                    p, p, p, p, 4, p, p, p, 8, 0.1, 1, None, 0, None, 0, None, None)
+                                    p, p, p, p, 4, p, p, p, 0.1, 1, None, 0, None, None)
     assert rc == N.ERR_ARG and b"null" in lib.nslg_last_error()
 
 
