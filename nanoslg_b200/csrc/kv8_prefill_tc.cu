@@ -20,22 +20,23 @@
 //
 // Work item: two query tiles of 128 rows ("halves" A and B) of one sequence and kv head, each
 // 128 / G new tokens times the G query heads that share the kv head; both read the same K and
-// V tiles of 128 positions (N = 128: at N = 64 an m128 product reads its operands from shared
-// memory for longer than it computes). A persistent grid, one CTA an SM, takes the items,
+// V tiles of 64 positions. A persistent grid, one CTA an SM, takes the items,
 // longest causal spans first.
 //
 // Roles (16 warps; registers moved to the softmax warps by setmaxnreg):
 //   producer warp   bulk copies of the tile's page blocks (2 KiB each, contiguous) into raw
-//                   buffers, TMA boxes of Q; the pages' F and E factors into a ring of 4.
-//   converters (4)  raw codes -> 16-bit tiles in the 128-byte swizzled layout (rings of 2 for
+//                   buffers, TMA boxes of Q; the pages' factors F and E and the items into rings.
+//   converters (4)  raw codes -> 16-bit tiles in the 128-byte swizzled layout (rings of 4 for
 //                   K and for V), zeros behind the sequence's end and for bad pages.
-//   MMA warp        per tile: P_A.V, S_A(t+1), P_B.V, S_B(t+1), across items: while the softmax of one half
-//                   runs, the pipe does the other half's products. P is written over S
-//                   (tcgen05.mma of one thread execute in the order of issue, so S(t+1) may
-//                   follow P(t).V into the same columns).
+//   MMA A, B        one warp a half, per tile: P(t).V, S(t+2), across items. P is written
+//                   over S (tcgen05.mma of one thread execute in the order of issue, so S(t+2)
+//                   may follow P(t).V into the same columns), and each half has two such
+//                   buffers, so its softmax goes from tile to tile without waiting for the pipe.
+//                   With one buffer of 128 positions the scores of a half waited for its
+//                   softmax and the other way round: 2.9 us per 128 positions.
 //   softmax A, B    one thread a row: S from TMEM, p to TMEM as f16, o rescaled there when M is
 //                   raised; at the end of an item o / l straight to `out`.
-// TMEM per half: S (and P over it) 128 + O 128 columns; 512 in all.
+// TMEM per half: two S (and P over it) of 64 + O 128 columns; 512 in all.
 //
 // A block whose scale is NaN (K's or V's) gives NaN to the rows that see it: its F is NaN, and
 // masked positions are left out by selection. Every mbarrier wait is bounded; on a timeout
@@ -55,22 +56,26 @@ namespace {
 
 constexpr int kD = 128;
 constexpr int kBM = 128;              // rows per half
-constexpr int kBN = 128;              // positions per tile
+constexpr int kBN = 64;               // positions per tile
 constexpr int kPS = 16;
 constexpr int kPages = kBN / kPS;
-constexpr int kThreads = 512;         // warps 0-3 converters, 4 producer, 5 MMA, 8-11 / 12-15 softmax
+constexpr int kThreads = 512;         // warps 0-3 converters, 4 producer, 5 / 6 MMA, 8-11 / 12-15 softmax
 constexpr int kTmemCols = 512;
-constexpr int kHalfCols = 256;        // S / P at +0, O at +128
+constexpr int kHalfCols = 256;        // S / P of even tiles at +0, of odd ones at +64, O at +128
 constexpr int kColO = 128;
-constexpr int kDimHalf = 128 * 128;   // [128 rows][128 bytes]: 64 dims of a Q half or a K / V tile
-constexpr int kTileBytes = 2 * kDimHalf;
-constexpr int kRaw = kBN * kD;        // codes of a tile
+constexpr int kQBytes = kBM * kD * 2;         // a Q half: [64-dim half][128 rows][128 bytes]
+constexpr int kQDimHalf = kBM * 128;
+constexpr int kTileBytes = kBN * kD * 2;      // a K or V tile: [64-dim half][64 positions][128 bytes]
+constexpr int kDimHalf = kBN * 128;
+constexpr int kRing = 4;                      // K tiles, V tiles
+constexpr int kRaw = kBN * kD;                // codes of a tile
+constexpr int kRawRing = 2;
 constexpr int kBlockBytes = kPS * kD;
 constexpr float kZeroE = 60.f;
-constexpr int kFactors = 4;           // ring of the pages' factors
+constexpr int kFactors = 8;           // ring of the pages' factors
 constexpr int kItems = 4;             // ring of published items
-constexpr int kSmemBytes = 1024 + 2 * kTileBytes /* Q */ + 4 * kTileBytes /* K, V rings */ +
-                           2 * kRaw + 1024;   // and the factors and barriers
+constexpr int kSmemBytes = 1024 + 2 * kQBytes + 2 * kRing * kTileBytes + 2 * kRawRing * kRaw +
+                           1536;   // and the factors, barriers and items
 
 struct PrefillParams : Kv8AttnParams {
   int group, tokens_per_tile, n_items;
@@ -155,6 +160,26 @@ __device__ __forceinline__ bool elect_one() {
   return e != 0u;
 }
 
+// Pairs of fp32 values: one instruction for two of the softmax's products or sums.
+__device__ __forceinline__ uint64_t f32x2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void from_f32x2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 template <int kRegs>
 __device__ __forceinline__ void regs_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
@@ -171,55 +196,59 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* sq = smem;                                 // [half][64-dim half][128 rows][128 B]
-  uint8_t* sk = sq + 2 * kTileBytes;                  // [2][64-dim half][128 positions][128 B]
-  uint8_t* sv = sk + 2 * kTileBytes;
-  uint8_t* raw = sv + 2 * kTileBytes;                 // [K, V][128 positions][128 codes]
-  Factors* fac = reinterpret_cast<Factors*>(raw + 2 * kRaw);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(fac) + 512);
+  uint8_t* sq = smem;                                 // [half]
+  uint8_t* sk = sq + 2 * kQBytes;                     // [kRing]
+  uint8_t* sv = sk + kRing * kTileBytes;              // [kRing]
+  uint8_t* raw = sv + kRing * kTileBytes;             // [K, V][kRawRing][64 positions][128 codes]
+  Factors* fac = reinterpret_cast<Factors*>(raw + 2 * kRawRing * kRaw);
+  Item* items = reinterpret_cast<Item*>(fac + kFactors);   // [kItems]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(items + kItems);
   uint64_t* q_full = bars + 0;       // [half] Q arrived
   uint64_t* q_empty = bars + 2;      // [half] last S of the item done
-  uint64_t* raw_full = bars + 6;     // [K, V]
-  uint64_t* raw_empty = bars + 8;    // [K, V]
-  uint64_t* k_full = bars + 10;      // [2]
-  uint64_t* k_empty = bars + 12;
-  uint64_t* v_full = bars + 14;
-  uint64_t* v_empty = bars + 16;
-  uint64_t* s_full = bars + 18;      // [half]
-  uint64_t* p_full = bars + 20;      // [half]
-  uint64_t* pv_done = bars + 22;     // [half]
-  uint64_t* o_free = bars + 24;      // [half]
-  uint64_t* f_full = bars + 26;      // [kFactors]
-  uint64_t* drain = bars + 30;
-  uint64_t* item_full = bars + 32;   // [kItems]
-  uint64_t* item_empty = bars + 36;  // [kItems] read by the converter, MMA and softmax warps
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 40);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 41);
-  Item* items = reinterpret_cast<Item*>(bars + 42);   // [kItems]
+  uint64_t* raw_full = bars + 4;     // [K, V][kRawRing]
+  uint64_t* raw_empty = bars + 8;
+  uint64_t* k_full = bars + 12;      // [kRing]
+  uint64_t* k_empty = bars + 16;
+  uint64_t* v_full = bars + 20;
+  uint64_t* v_empty = bars + 24;
+  uint64_t* s_full = bars + 28;      // [half][2]
+  uint64_t* p_full = bars + 32;      // [half][2]
+  uint64_t* pv_done = bars + 36;     // [half][2]
+  uint64_t* o_free = bars + 40;      // [half]
+  uint64_t* f_full = bars + 42;      // [kFactors]
+  uint64_t* item_full = bars + 50;   // [kItems]
+  uint64_t* item_empty = bars + 54;  // [kItems] read by the converter, MMA and softmax warps
+  uint64_t* drain = bars + 58;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 59);
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
+      mbar_init(&o_free[i], 128);
+    }
+    for (int i = 0; i < 2 * kRawRing; ++i) {
       mbar_init(&raw_full[i], 1);
       mbar_init(&raw_empty[i], 4);
+    }
+    for (int i = 0; i < kRing; ++i) {
       mbar_init(&k_full[i], 4);
-      mbar_init(&k_empty[i], 1);
+      mbar_init(&k_empty[i], 2);
       mbar_init(&v_full[i], 4);
-      mbar_init(&v_empty[i], 1);
+      mbar_init(&v_empty[i], 2);
+    }
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 128);
       mbar_init(&pv_done[i], 1);
-      mbar_init(&o_free[i], 128);
     }
     for (int i = 0; i < kFactors; ++i) mbar_init(&f_full[i], 1);
     for (int i = 0; i < kItems; ++i) {
       mbar_init(&item_full[i], 1);
-      mbar_init(&item_empty[i], 4 + 1 + 8);
+      mbar_init(&item_empty[i], 4 + 2 + 8);
     }
-    mbar_init(drain, 1);
-    *abort_flag = 0;
+    mbar_init(drain, 2);
     fence_barrier_init();
   }
   if (warp == 5) {
@@ -233,9 +262,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  auto gone = [&]() { return *abort_flag != 0; };
   auto all_wait = [&](uint64_t* bar, uint32_t par) {   // by a converged warp
-    return static_cast<bool>(__all_sync(0xffffffffu, !gone() && mbar_wait(bar, par)));
+    return static_cast<bool>(__all_sync(0xffffffffu, mbar_wait(bar, par)));
   };
   // item number n as published, copied out of its slot; false: a wait gave up
   auto take_item = [&](int n, Item& it) -> bool {
@@ -246,37 +274,33 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) mbar_arrive(&item_empty[s]);
     return true;
   };
-  auto give_up = [&]() {
-    report(p.status, NSLG_DEV_WAIT_TIMEOUT);
-    *abort_flag = 1;
-  };
+  // after a wait that gave up a role leaves, and the waits of the others for it give up too
+  auto give_up = [&]() { report(p.status, NSLG_DEV_WAIT_TIMEOUT); };
 
   // 128 registers a thread at launch: 2 x 128 x 184 + 128 x 80 + 128 x 64 = 512 x 128
   if (warp < 4) {
     // -------------------------------------------------------------- converters
     regs_dec<80>();
     const int tid = threadIdx.x;
-    const int c = tid & 7, t0 = tid >> 3;              // 16-code chunk; positions t0 + 16 i
+    // 16-code chunk c of positions t0 + 16 i. The lanes of the upper 64 dims take the
+    // neighbouring position: the swizzle then puts the eight lanes that store together into
+    // eight banks
+    const int c = tid & 7, t0 = (tid >> 3) ^ (c >> 2);
     int nk = 0, nv = 0;                                // K tiles, V tiles
     bool ok = true;
-    const int swz = t0 & 7, odd = c >> 2, c0 = 2 * (c & 3);
-    // 16-byte chunks c0 and c0 + 1 of the row's 128 bytes; the lanes of the upper 64 dims write
-    // theirs in the other order, so that eight lanes meet eight banks
-    const uint32_t at0 = odd * kDimHalf + t0 * 128 + (((c0 + odd) ^ swz) << 4);
-    const uint32_t at1 = odd * kDimHalf + t0 * 128 + (((c0 + 1 - odd) ^ swz) << 4);
+    const uint32_t row0 = (c >> 2) * kDimHalf + t0 * 128;
+    const uint32_t at0 = row0 + (((2 * (c & 3)) ^ (t0 & 7)) << 4);
+    const uint32_t at1 = row0 + (((2 * (c & 3) + 1) ^ (t0 & 7)) << 4);
     // one tile of codes to 16 bits: K (number n of its kind) to q's type, V to f16; positions
     // `held` of it exist
     auto convert = [&](auto kind, int n, int held) -> bool {
       constexpr int kv = decltype(kind)::value;
-      uint64_t* full = kv ? v_full : k_full;
-      uint64_t* empty = kv ? v_empty : k_empty;
-      const int s = n & 1;
-      if (!all_wait(&raw_full[kv], n & 1)) return false;
+      const int s = n % kRing, rs = kv * kRawRing + n % kRawRing;
+      if (!all_wait(&raw_full[rs], (n / kRawRing) & 1)) return false;
+      if (!all_wait(&(kv ? v_empty : k_empty)[s], ((n / kRing) & 1) ^ 1)) return false;
       // pages whose codes count (V: not those of a scale of 0 or NaN)
       const uint32_t valid = kv ? fac[n % kFactors].plain : fac[n % kFactors].valid;
-      const uint8_t* src = raw + kv * kRaw + t0 * 128 + c * 16;
-      if (!all_wait(&empty[s], ((n >> 1) & 1) ^ 1)) return false;
-      const bool full_tile = held >= kBN && valid == (1u << kPages) - 1u;
+      const uint8_t* src = raw + rs * kRaw + t0 * 128 + c * 16;
       uint8_t* dst = (kv ? sv : sk) + s * kTileBytes;
       auto two = [&](uint32_t codes) -> uint32_t {     // the low two codes
         const uint32_t h = f16x2_from_e4m3x2(static_cast<uint16_t>(codes));
@@ -287,29 +311,26 @@ __global__ void __launch_bounds__(kThreads, 1)
           return pack_bf16x2(f.x, f.y);
         }
       };
-#pragma unroll 1
-      for (int i0 = 0; i0 < 8; i0 += 4) {
-        uint4 w[4];
+      uint4 w[kPages];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint4*>(src + (i0 + i) * 2048);
-        if (!full_tile) {
+      for (int i = 0; i < kPages; ++i) w[i] = *reinterpret_cast<const uint4*>(src + i * kBlockBytes);
+      if (held < kBN || valid != (1u << kPages) - 1u) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)                  // position t0 + 16 i: page i of the tile
-            if (t0 + 16 * (i0 + i) >= held || !((valid >> (i0 + i)) & 1u)) w[i] = make_uint4(0u, 0u, 0u, 0u);
-        }
+        for (int i = 0; i < kPages; ++i)               // position t0 + 16 i: page i of the tile
+          if (t0 + kPS * i >= held || !((valid >> i) & 1u)) w[i] = make_uint4(0u, 0u, 0u, 0u);
+      }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint4 lo = make_uint4(two(w[i].x), two(w[i].x >> 16), two(w[i].y), two(w[i].y >> 16));
-          const uint4 hi = make_uint4(two(w[i].z), two(w[i].z >> 16), two(w[i].w), two(w[i].w >> 16));
-          *reinterpret_cast<uint4*>(dst + at0 + (i0 + i) * 2048) = odd ? hi : lo;
-          *reinterpret_cast<uint4*>(dst + at1 + (i0 + i) * 2048) = odd ? lo : hi;
-        }
+      for (int i = 0; i < kPages; ++i) {
+        const uint4 lo = make_uint4(two(w[i].x), two(w[i].x >> 16), two(w[i].y), two(w[i].y >> 16));
+        const uint4 hi = make_uint4(two(w[i].z), two(w[i].z >> 16), two(w[i].w), two(w[i].w >> 16));
+        *reinterpret_cast<uint4*>(dst + at0 + i * kPS * 128) = lo;
+        *reinterpret_cast<uint4*>(dst + at1 + i * kPS * 128) = hi;
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&raw_empty[kv]);
-        mbar_arrive(&full[s]);
+        mbar_arrive(&raw_empty[rs]);
+        mbar_arrive(&(kv ? v_full : k_full)[s]);
       }
       return true;
     };
@@ -340,17 +361,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         return lane < kPages && j < it.ntiles && pi < it.npages ? p.kv_indices[it.kv_beg + pi] : -2;
       };
       auto copy = [&](int kv, int n, const Item& it, int page) -> bool {
-        if (!all_wait(&raw_empty[kv], (n & 1) ^ 1)) return false;
+        const int rs = kv * kRawRing + n % kRawRing;
+        if (!all_wait(&raw_empty[rs], ((n / kRawRing) & 1) ^ 1)) return false;
         const bool has = page >= 0 && page < p.num_pages;
         if (page != -2 && !has) report(p.status, NSLG_DEV_BAD_PAGE);
         const uint32_t valid = __ballot_sync(0xffffffffu, has);
-        if (lane == 0) mbar_arrive_expect_tx(&raw_full[kv], __popc(valid) * kBlockBytes);
+        if (lane == 0) mbar_arrive_expect_tx(&raw_full[rs], __popc(valid) * kBlockBytes);
         __syncwarp();
         if (has)
-          bulk_load(raw + kv * kRaw + lane * kBlockBytes,
+          bulk_load(raw + rs * kRaw + lane * kBlockBytes,
                     static_cast<const uint8_t*>(kv ? p.codes_v : p.codes_k) +
                         (static_cast<int64_t>(page) * p.hkv + it.h) * kBlockBytes,
-                    kBlockBytes, &raw_full[kv]);
+                    kBlockBytes, &raw_full[rs]);
         return true;
       };
       auto scales = [&](const Item& it, int page, float& sk_, float& sv_) {
@@ -413,8 +435,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int page2 = page_of(it, j + 2);
             float f1 = 0.f, v1 = 0.f;
             scales(it, page1, f1, v1);
-            // tile nk - 4 has left its ring slot: the last V copy waited until V(nk - 2) was
-            // converted, which waited for P(nk - 4).V
+            // tile nk - 8 has left its ring slot: the last V copy waited until V(nk - 3) was
+            // converted, which waited for P(nk - 7).V
             factors(nk, page, f, v);
             if (!(ok = copy(0, nk, it, page))) break;
             ++nk;
@@ -423,11 +445,11 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int x = 0; ok && x < 2; ++x) {
                 if (!(ok = all_wait(&q_empty[x], (n_it & 1) ^ 1))) break;
                 if (lane == 0) {
-                  mbar_arrive_expect_tx(&q_full[x], kTileBytes);
-                  uint8_t* dst = sq + x * kTileBytes;
+                  mbar_arrive_expect_tx(&q_full[x], kQBytes);
+                  uint8_t* dst = sq + x * kQBytes;
                   const int row = it.row0 + x * p.tokens_per_tile;
                   tma_load_3d(dst, &tmap_q, &q_full[x], 0, it.h * G, row, keep);
-                  tma_load_3d(dst + kDimHalf, &tmap_q, &q_full[x], 64, it.h * G, row, keep);
+                  tma_load_3d(dst + kQDimHalf, &tmap_q, &q_full[x], 64, it.h * G, row, keep);
                 }
                 ++nq;
                 __syncwarp();
@@ -452,101 +474,108 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) {
         if (lane == 0) give_up();
         // no copy may still be writing shared memory when the CTA leaves (bounded waits)
-        if (nk > 0) (void)mbar_wait(&raw_full[0], (nk - 1) & 1);
-        if (nv > 0) (void)mbar_wait(&raw_full[1], (nv - 1) & 1);
+        for (int k = 0; k < 2; ++k)
+          for (int u = max((k ? nv : nk) - kRawRing, 0); u < (k ? nv : nk); ++u)
+            (void)mbar_wait(&raw_full[k * kRawRing + u % kRawRing], (u / kRawRing) & 1);
         for (int x = 0; x < 2; ++x) {
           const int loads = (nq + 1 - x) / 2;
           if (loads > 0) (void)mbar_wait(&q_full[x], (loads - 1) & 1);
         }
       }
-    } else if (warp == 5) {
-      // -------------------------------------------------------------- MMA issuer
+    } else if (warp < 7) {
+      // -------------------------------------------------------------- MMA issuers, one per half
       // The whole warp runs the loop and one elected lane issues: the descriptors then stay
       // warp-uniform. With the loop in one lane an MMA costs enough instructions that the
       // softmax warps on the same scheduler held it to 118 clocks an m128n128k16 instead of 64
-      // (71 this way, FMA-bound warps beside it).
+      // (71 this way, FMA-bound warps beside it); and one warp for both halves spent 2.1 us of
+      // issuing and waiting on a tile whose products take 0.7.
+      const int x = warp - 5;
       constexpr uint32_t kIdescS = idesc_f16(Mma16<T>::kFormat, kBN, false);
       constexpr uint32_t kIdescO = idesc_f16(0, kD, true);
       constexpr uint32_t kDescHi = smem_desc_hi(1024);
-      const uint32_t q_lo0 = smem_desc_lo(smem_u32(sq), 16);
+      const uint32_t q_lo = smem_desc_lo(smem_u32(sq + x * kQBytes), 16);
       const uint32_t k_lo0 = smem_desc_lo(smem_u32(sk), 16);
       const uint32_t v_lo0 = smem_desc_lo(smem_u32(sv), kDimHalf);
+      const uint32_t hb = tmem + x * kHalfCols;
       bool ok = true;
-      // The tiles of all items form one stream: S of an item's first tile is issued behind P.V
-      // of the last tile of the item before, so the pipe and the softmax go on while that
-      // item's rows are written.
-      struct Tile {
-        bool first, last;      // of its item
-      };
-      int n = 0, left = 0;     // items taken, tiles left of the last one
-      auto next_tile = [&](Tile& w) -> bool {          // false: no more, or a wait gave up (ok)
-        w.first = left == 0;
-        Item it;
-        while (left == 0) {
-          if (!(ok = take_item(n, it)) || it.ntiles < 0) return false;
-          ++n;
-          left = it.ntiles;
-        }
-        w.last = --left == 0;
-        return true;
-      };
-      int t = 0, n_q = 0, n_o = 0;                     // tiles; items whose Q / O were begun
-      Tile cur, nxt;
-      bool have = next_tile(cur);
-      bool start = true;                               // the first tile has no P.V before its S
-      nxt = cur;
-      while (ok && have) {
-        // tile t (none at the start) and, behind its products, S of the tile after it
-        const bool more = start ? true : next_tile(nxt);
-        if (!ok) break;
-        const int slot = t & 1, u = start ? 0 : t + 1, kslot = u & 1;
-        if (!start && !(ok = all_wait(&v_full[slot], (t >> 1) & 1))) break;
-        const uint32_t v_lo = v_lo0 + slot * (kTileBytes >> 4);
-        const uint32_t k_lo = k_lo0 + kslot * (kTileBytes >> 4);
-#pragma unroll 1
-        for (int x = 0; x < 2; ++x) {
-          const uint32_t hb = tmem + x * kHalfCols;
-          if (!start) {
-            if (!(ok = all_wait(&p_full[x], t & 1))) break;
-            if (cur.first && n_o > 0 && !(ok = all_wait(&o_free[x], (n_o - 1) & 1))) break;
-            tc_fence_after();
-            if (elect_one()) {
-#pragma unroll
-              for (int kt = 0; kt < kBN / 16; ++kt)
-                mma_ts_w(hb + kColO, hb + kt * 8, v_lo + (kt * 2048 >> 4), kDescHi, kIdescO,
-                         (!cur.first || kt > 0) ? 1u : 0u);
-              mma_commit(&pv_done[x]);
-              if (x == 1) mma_commit(&v_empty[slot]);
-            }
-            __syncwarp();
+      // The tiles of all items form one stream. S(u) goes into the buffer of P(u - 2), right
+      // behind P(u - 2).V in the pipe, so it is there when the softmax has done tile u - 1, and
+      // an item's first scores are computed while the rows before are written.
+      int u = 0, sj = 0, snt = 0, n = 0, n_q = 0;   // tiles scored; tile of the item being scored;
+                                             // items taken, items with tiles
+      bool end = false;
+      int nts[3] = {0, 0, 0};                // tiles of the items between P.V and S, oldest first
+      int held = 0;                          // ... how many
+      // S of the tiles up to t + 2 (t + 1 where Q is not there yet)
+      auto score = [&](int t) {
+        while (!end && u <= t + 2) {
+          if (sj == snt) {                   // the next item with tiles
+            Item it;
+            do {
+              if (!(ok = take_item(n, it)) || it.ntiles < 0) {
+                end = true;
+                return;
+              }
+              ++n;
+            } while (it.ntiles == 0);
+            snt = it.ntiles;
+            sj = 0;
+            if (held == 0) nts[0] = snt;
+            else if (held == 1) nts[1] = snt;
+            else nts[2] = snt;
+            ++held;
+            ++n_q;
           }
-          if (!more) continue;
-          // S_x(u) = Q_x . K(u)^T; P_x(t).V, issued before, reads the same columns
-          if (x == 0 && !(ok = all_wait(&k_full[kslot], (u >> 1) & 1))) break;
-          if (nxt.first && !(ok = all_wait(&q_full[x], n_q & 1))) break;
+          const uint32_t q_par = (n_q - 1) & 1;
+          if (sj == 0) {
+            if (u > t + 1 && !__all_sync(0xffffffffu, mbar_try_wait(&q_full[x], q_par))) return;
+            if (!(ok = all_wait(&q_full[x], q_par))) return;
+          }
+          const int slot = u % kRing;
+          if (!(ok = all_wait(&k_full[slot], (u / kRing) & 1))) return;
           tc_fence_after();
-          const uint32_t q_lo = q_lo0 + x * (kTileBytes >> 4);
           if (elect_one()) {
+            const uint32_t k_lo = k_lo0 + slot * (kTileBytes >> 4), dcol = hb + 64 * (u & 1);
 #pragma unroll
-            for (int ks = 0; ks < kD / 16; ++ks) {
-              const uint32_t off = ((ks >> 2) * kDimHalf + (ks & 3) * 32) >> 4;
-              mma_ss_w(hb, q_lo + off, k_lo + off, kDescHi, kIdescS, ks > 0 ? 1u : 0u);
-            }
-            mma_commit(&s_full[x]);
-            if (x == 1) mma_commit(&k_empty[kslot]);
-            if (nxt.last) mma_commit(&q_empty[x]);
+            for (int ks = 0; ks < kD / 16; ++ks)
+              mma_ss_w(dcol, q_lo + (((ks >> 2) * kQDimHalf + (ks & 3) * 32) >> 4),
+                       k_lo + (((ks >> 2) * kDimHalf + (ks & 3) * 32) >> 4), kDescHi, kIdescS,
+                       ks > 0 ? 1u : 0u);
+            mma_commit(&s_full[x * 2 + (u & 1)]);
+            mma_commit(&k_empty[slot]);
+            if (sj + 1 == snt) mma_commit(&q_empty[x]);
           }
           __syncwarp();
+          ++sj;
+          ++u;
         }
-        if (!ok) break;
-        if (!start) {
-          if (cur.first) ++n_o;
-          ++t;
+      };
+      int t = -2, pj = 0, n_o = 0;           // tile, its place in its item, items whose O was begun
+#pragma unroll 1
+      for (; ok && t < 0; ++t) score(t);
+      for (t = 0; ok && t < u; ++t) {
+        const int slot = t % kRing, b = t & 1;
+        if (!(ok = all_wait(&v_full[slot], (t / kRing) & 1))) break;
+        if (!(ok = all_wait(&p_full[x * 2 + b], (t >> 1) & 1))) break;
+        if (pj == 0 && n_o++ > 0 && !(ok = all_wait(&o_free[x], n_o & 1))) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t v_lo = v_lo0 + slot * (kTileBytes >> 4);
+#pragma unroll
+          for (int kt = 0; kt < kBN / 16; ++kt)
+            mma_ts_w(hb + kColO, hb + 64 * b + kt * 8, v_lo + (kt * 2048 >> 4), kDescHi, kIdescO,
+                     (pj > 0 || kt > 0) ? 1u : 0u);
+          mma_commit(&pv_done[x * 2 + b]);
+          mma_commit(&v_empty[slot]);
         }
-        if (more && nxt.first) ++n_q;
-        start = false;
-        cur = nxt;
-        have = more;
+        __syncwarp();
+        if (++pj == nts[0]) {
+          pj = 0;
+          nts[0] = nts[1];
+          nts[1] = nts[2];
+          --held;
+        }
+        score(t);
       }
       if (!ok && lane == 0) give_up();
       if (elect_one()) mma_commit(drain);              // everything issued has completed (bounded)
@@ -586,37 +615,30 @@ __global__ void __launch_bounds__(kThreads, 1)
                                  : it.kv_len - 1;
       float m = -INFINITY, l = 0.f;
       bool seen = false;                               // a tile with an E of its own
-      // One tile, in two halves of 64 columns read twice from TMEM (for the maximum, for the
-      // weights): the loops keep the code of all roles together inside the instruction cache
-      // (unrolled over the tile, with a second copy for edges, 16 % of the fetches missed it).
-      // edge: some row of the warp does not see all of the tile
+      // one tile; edge: some row of the warp does not see all of it
       auto softmax = [&](bool edge, int j) -> bool {
         const Factors& fc = fac[t % kFactors];
-        const int past = lim - j * kBN;                // last column the row sees
+        const int gap = lim - j * kBN;                 // last column the row sees
+        const int b = t & 1;
+        float s[kBN];
+        tmem_ld64(base + 64 * b, s);
+        tmem_wait_ld();
+        if (edge) {
+#pragma unroll
+          for (int c = 0; c < kBN; ++c)
+            if (c > gap) s[c] = -INFINITY;
+        }
         float mt = -INFINITY;
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          float s[64];
-          tmem_ld64(base + 64 * h, s);
-          tmem_wait_ld();
-          if (edge) {
-            const int gap = past - 64 * h;
 #pragma unroll
-            for (int c = 0; c < 64; ++c)
-              if (c > gap) s[c] = -INFINITY;
-          }
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const float* sg = s + g * 16;
-            float a = fmaxf(fmaxf(sg[0], sg[1]), sg[2]), b = fmaxf(fmaxf(sg[3], sg[4]), sg[5]);
-            a = fmaxf(fmaxf(a, sg[6]), sg[7]);
-            b = fmaxf(fmaxf(b, sg[8]), sg[9]);
-            a = fmaxf(fmaxf(a, sg[10]), sg[11]);
-            b = fmaxf(fmaxf(b, sg[12]), sg[13]);
-            a = fmaxf(fmaxf(a, sg[14]), sg[15]);
-            // NaN is ignored
-            mt = fmaxf(mt, fmaf(fmaxf(a, b), fc.f[4 * h + g], fc.e[4 * h + g]));
-          }
+        for (int g = 0; g < kPages; ++g) {
+          const float* sg = s + g * 16;
+          float a = fmaxf(fmaxf(sg[0], sg[1]), sg[2]), b2 = fmaxf(fmaxf(sg[3], sg[4]), sg[5]);
+          a = fmaxf(fmaxf(a, sg[6]), sg[7]);
+          b2 = fmaxf(fmaxf(b2, sg[8]), sg[9]);
+          a = fmaxf(fmaxf(a, sg[10]), sg[11]);
+          b2 = fmaxf(fmaxf(b2, sg[12]), sg[13]);
+          a = fmaxf(fmaxf(a, sg[14]), sg[15]);
+          mt = fmaxf(mt, fmaf(fmaxf(a, b2), fc.f[g], fc.e[g]));   // NaN is ignored
         }
         const bool own = fc.plain != 0u, anew = !seen && own;   // anew: O is all zeros so far,
         seen = seen || own;                            // M may go down too
@@ -625,42 +647,40 @@ __global__ void __launch_bounds__(kThreads, 1)
             raise && m != -INFINITY && mt != -INFINITY ? fast_exp2(m - mt) : 1.f;
         if (raise) m = mt;
         const float nb = m == -INFINITY ? 0.f : -m;
+#pragma unroll
+        for (int g = 0; g < kPages; ++g) {
+          const float add = fc.e[g] + nb;
+          const uint64_t F2 = f32x2(fc.f[g], fc.f[g]), add2_ = f32x2(add, add);
+#pragma unroll
+          for (int c = g * 16; c < g * 16 + 16; c += 2) {
+            from_f32x2(fma2(f32x2(s[c], s[c + 1]), F2, add2_), s[c], s[c + 1]);
+            s[c] = fast_exp2(s[c]);
+            s[c + 1] = fast_exp2(s[c + 1]);
+          }
+        }
+        if (edge) {                                    // F = 0 or NaN times -inf is NaN
+#pragma unroll
+          for (int c = 0; c < kBN; ++c)
+            if (c > gap) s[c] = 0.f;
+        }
         float sum = 0.f;
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          float s[64];
-          tmem_ld64(base + 64 * h, s);
-          tmem_wait_ld();
+        uint32_t pk[32];
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const float F = fc.f[4 * h + g], add = fc.e[4 * h + g] + nb;
+        for (int g = 0; g < kPages; ++g) {
+          uint64_t gs = f32x2(s[g * 16], s[g * 16 + 1]);
 #pragma unroll
-            for (int c = 0; c < 16; ++c) s[g * 16 + c] = fast_exp2(fmaf(s[g * 16 + c], F, add));
+          for (int c = 0; c < 16; c += 2) {
+            if (c > 0) gs = add2(gs, f32x2(s[g * 16 + c], s[g * 16 + c + 1]));
+            pk[g * 8 + c / 2] = pack_f16x2(s[g * 16 + c], s[g * 16 + c + 1]);
           }
-          if (edge) {
-            const int gap = past - 64 * h;
-#pragma unroll
-            for (int c = 0; c < 64; ++c)
-              if (c > gap) s[c] = 0.f;
-          }
-          uint32_t pk[32];
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            float gs[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int c = 0; c < 16; c += 2) {
-              gs[c / 2 % 2] += s[g * 16 + c];
-              gs[2 + c / 2 % 2] += s[g * 16 + c + 1];
-              pk[g * 8 + c / 2] = pack_f16x2(s[g * 16 + c], s[g * 16 + c + 1]);
-            }
-            sum = fmaf((gs[0] + gs[1]) + (gs[2] + gs[3]), fc.inv[4 * h + g], sum);
-          }
-          tmem_st32(base + 32 * h, pk);                // P over the columns of S already read
+          float a, b2;
+          from_f32x2(gs, a, b2);
+          sum = fmaf(a + b2, fc.inv[g], sum);
         }
         // O may only be rescaled once P(t-1).V(t-1) is done (tcgen05.ld / st are
         // warp-collective; rows with alpha == 1 multiply by 1)
         if (j > 0 && !anew && __any_sync(0xffffffffu, alpha != 1.f)) {
-          if (!all_wait(&pv_done[x], (t - 1) & 1)) return false;
+          if (!all_wait(&pv_done[x * 2 + (b ^ 1)], ((t - 1) >> 1) & 1)) return false;
           tc_fence_after();
 #pragma unroll 1
           for (int cb = 0; cb < kD; cb += 32) {
@@ -674,21 +694,22 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         l = fmaf(l, alpha, sum);
+        tmem_st32(base + 64 * b, pk);                  // P over S
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(&p_full[x]);
+        mbar_arrive(&p_full[x * 2 + b]);
         return true;
       };
       for (int j = 0; j < it.ntiles; ++j, ++t) {
         if (j + 1 == it.ntiles && !(ok = take_item(n, nx))) break;
         if (!(ok = all_wait(&f_full[t % kFactors], (t / kFactors) & 1))) break;
-        if (!(ok = all_wait(&s_full[x], t & 1))) break;
+        if (!(ok = all_wait(&s_full[x * 2 + (t & 1)], (t >> 1) & 1))) break;
         tc_fence_after();
         if (!(ok = softmax(!__all_sync(0xffffffffu, (j + 1) * kBN - 1 <= lim), j))) break;
       }
       if (!ok) break;
       const int tl = t - 1;
-      if (!(ok = all_wait(&pv_done[x], tl & 1))) break;
+      if (!(ok = all_wait(&pv_done[x * 2 + (tl & 1)], (tl >> 1) & 1))) break;
       tc_fence_after();
       const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
