@@ -101,7 +101,7 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
 // Rows of one virtual sequence's tile in q and out, and what they see.
 struct Tile {
   int b, h, r0;           // sequence, kv head, first (token, head) pair of the tile
-  int qo_len, kv_len;
+  int qo_len, kv_len, pages;
   int64_t row0;           // row of the sequence's first new token
 };
 
@@ -286,7 +286,8 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
   // ---- metadata of 32 units at a time, one per lane
   struct Meta {
     int blk, vid, j;       // block (page * kv heads + head; -1: a bad page), sequence, page of it
-    float sk, sv;          // scale_k; scale_v, 0 where V is zeros or not finite
+    float sk, sv;          // scale_k and scale_v as loaded; then what weigh() makes of them
+    float iv;
   };
   auto locate = [&](int u, int& vid, int& first) {   // unit u: its sequence and page list entry
     const int b = seq_of(indptr, p.batch, u / hm);
@@ -315,6 +316,14 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
     m.sk = m.blk >= 0 ? p.scale_k[m.blk] : 0.f;
     m.sv = m.blk >= 0 ? p.scale_v[m.blk] : 0.f;
   };
+  // sv becomes E = log2 scale_v, NaN where V is zeros or not finite, and iv 2^-E; sk becomes NaN
+  // where scale_v is (the NaN rides on the scores). Once for 32 units, when they are begun.
+  auto weigh = [&](Meta& m) {
+    const bool plain = m.sv > 0.f && m.sv < INFINITY;
+    if (m.sv != m.sv) m.sk = m.sv;
+    m.sv = plain ? __log2f(m.sv) : NAN;   // any value near the logarithm will do: iv is its inverse
+    m.iv = fast_exp2(-m.sv);
+  };
   const uint64_t policy = p.tiles > 1 ? l2_policy_evict_last() : l2_policy_evict_first();
   auto issue = [&](const Meta& m, int i) {   // by the lane that holds unit i
     const int s = i % stages;
@@ -342,7 +351,7 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
   float m[NT][2], nb[NT][2], l[NT][2], f[NT][2];   // of rows 2tq, 2tq + 1
   int pos[NT][2];                        // last position they see
   int low = 0;                           // ... the least of all the tile's rows
-  float ev = 0.f, iv = 1.f;              // E of the last page that had one, 2^-E
+  float ev = 0.f;                        // E of the last page that had one
   bool seen = false;                     // ... whether there was one
   int vid = -1;
   Tile t{};
@@ -355,10 +364,10 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
     t.h = vs / p.tiles;
     t.r0 = vs % p.tiles * Shape<NT>::kRows;
     t.qo_len = new_rows(p, t.b, &t.row0);
-    t.kv_len = (indptr[t.b + 1] - indptr[t.b] - 1) * kPS + lpl[t.b];
+    t.pages = indptr[t.b + 1] - indptr[t.b];
+    t.kv_len = (t.pages - 1) * kPS + lpl[t.b];
     low = 0x7fffffff;
     ev = 0.f;
-    iv = 1.f;
     seen = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -498,32 +507,34 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
       }
   };
 
+  int left = 0, tok0 = 0;                // units of `vid` to come, the first token of this one
   int slot = 0;
   uint32_t phase = 0;
   for (int base = 0; base < units && ok; base += 32) {
     cur = nxt;
+    weigh(cur);
     look_up(base + 32 + lane, nxt);
     load_scales(nxt);
     const int stop = min(32, units - base);
     for (int i = 0; i < stop; ++i) {
-      const int v = __shfl_sync(0xffffffffu, cur.vid, i);
-      if (v != vid) {
+      if (left == 0) {             // the next virtual sequence
         if (vid >= 0) finish();
-        begin(v);
+        begin(__shfl_sync(0xffffffffu, cur.vid, i));
+        const int j = __shfl_sync(0xffffffffu, cur.j, i);
+        tok0 = j * kPS;
+        left = t.pages - j;
       }
-      float sk = __shfl_sync(0xffffffffu, cur.sk, i);
-      const float sv = __shfl_sync(0xffffffffu, cur.sv, i);
-      const bool plain = sv > 0.f && sv < INFINITY;
-      if (sv != sv) sk = sv;       // NaN rides on the scores
+      const float sk = __shfl_sync(0xffffffffu, cur.sk, i);
+      float eu = __shfl_sync(0xffffffffu, cur.sv, i), iu = __shfl_sync(0xffffffffu, cur.iv, i);
+      const bool plain = eu == eu;
       const bool anew = plain && !seen;
       if (plain) {
-        ev = __log2f(sv);          // any value near log2 sv will do: iv is its inverse
-        iv = fast_exp2(-ev);
+        ev = eu;
         seen = true;
+      } else {
+        eu = fmaxf(ev - kZeroE, -120.f);
+        iu = fast_exp2(-eu);
       }
-      const float eu = plain ? ev : fmaxf(ev - kZeroE, -120.f);
-      const float iu = plain ? iv : fast_exp2(-eu);
-      const int tok0 = __shfl_sync(0xffffffffu, cur.j, i) * kPS;
       ok = __all_sync(0xffffffffu, mbar_wait(&full[slot], phase));
       if (!ok) {
         if (lane == 0) report(p.status, NSLG_DEV_WAIT_TIMEOUT);
@@ -631,6 +642,8 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
       __syncwarp();        // the slot has been read by every lane
       const int ahead = i + stages;
       if (base + ahead < units && lane == (ahead & 31)) issue(ahead < 32 ? cur : nxt, base + ahead);
+      tok0 += kPS;
+      --left;
       if (++slot == stages) {
         slot = 0;
         phase ^= 1;
