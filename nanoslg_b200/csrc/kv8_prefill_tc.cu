@@ -24,10 +24,12 @@
 // longest causal spans first.
 //
 // Roles (16 warps; registers moved to the softmax warps by setmaxnreg):
-//   producer warp   bulk copies of the tile's page blocks (2 KiB each, contiguous) into raw
-//                   buffers, TMA boxes of Q; the pages' factors F and E and the items into rings.
-//   converters (4)  raw codes -> 16-bit tiles in the 128-byte swizzled layout (rings of 4 for
-//                   K and for V), zeros behind the sequence's end and for bad pages.
+//   producer warp   the items and, per tile, the pages' blocks and factors F and E into rings.
+//   Q warp          TMA boxes of Q.
+//   converters (4)  a thread fetches its 16-byte pieces of the raw codes two tiles ahead
+//                   (cp.async into places of its own, so nothing but its own wait is needed),
+//                   widens them into 16-bit tiles in the 128-byte swizzled layout (rings of 4
+//                   for K and for V); zeros behind the sequence's end and for bad pages.
 //   MMA A, B        one warp a half, per tile: P(t).V, S(t+2), across items. P is written
 //                   over S (tcgen05.mma of one thread execute in the order of issue, so S(t+2)
 //                   may follow P(t).V into the same columns), and each half has two such
@@ -59,7 +61,7 @@ constexpr int kBM = 128;              // rows per half
 constexpr int kBN = 64;               // positions per tile
 constexpr int kPS = 16;
 constexpr int kPages = kBN / kPS;
-constexpr int kThreads = 512;         // warps 0-3 converters, 4 producer, 5 / 6 MMA, 8-11 / 12-15 softmax
+constexpr int kThreads = 512;         // warps 0-3 converters, 4 producer, 5 / 6 MMA, 7 Q, 8-11 / 12-15 softmax
 constexpr int kTmemCols = 512;
 constexpr int kHalfCols = 256;        // S / P of even tiles at +0, of odd ones at +64, O at +128
 constexpr int kColO = 128;
@@ -82,16 +84,17 @@ struct PrefillParams : Kv8AttnParams {
   float scale_log2;
 };
 
-// The factors of a tile's pages.
+// What a tile's pages are.
 struct alignas(16) Factors {
   float f[kPages];      // scale_k (NaN where the block of K or V is not finite)
   float e[kPages];      // log2 scale_v
   float inv[kPages];    // 2^-e
-  uint32_t valid;       // pages with codes
+  int blk[kPages];      // block (page * kv heads + head), -1: none
   uint32_t plain;       // pages with an e of their own
+  int held;             // positions that exist, maybe more than the tile's; -1: no more tiles
 };
 
-// A work item as the producer publishes it. ntiles 0: rows that see no position; -1: no more.
+// A work item as the producer publishes it. ntiles -1: no more.
 struct Item {
   int h, qo_len, kv_len, ntiles;
   int i0, row0;         // half A's first new token and its row; half B's: tokens_per_tile on
@@ -145,12 +148,16 @@ __device__ __forceinline__ bool finish_item(const PrefillParams& p, const ItemLo
   return true;
 }
 
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-          smem_u32(dst)),
-      "l"(src), "r"(bytes), "r"(smem_u32(bar))
-      : "memory");
+// 16 bytes, or zeros.
+__device__ __forceinline__ void copy16(void* dst, const void* src, bool full) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src),
+               "r"(full ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {   // all but the last N groups
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // True in one lane of the (converged) warp, the same one every time.
@@ -205,19 +212,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(items + kItems);
   uint64_t* q_full = bars + 0;       // [half] Q arrived
   uint64_t* q_empty = bars + 2;      // [half] last S of the item done
-  uint64_t* raw_full = bars + 4;     // [K, V][kRawRing]
-  uint64_t* raw_empty = bars + 8;
-  uint64_t* k_full = bars + 12;      // [kRing]
-  uint64_t* k_empty = bars + 16;
-  uint64_t* v_full = bars + 20;
-  uint64_t* v_empty = bars + 24;
-  uint64_t* s_full = bars + 28;      // [half][2]
-  uint64_t* p_full = bars + 32;      // [half][2]
-  uint64_t* pv_done = bars + 36;     // [half][2]
-  uint64_t* o_free = bars + 40;      // [half]
-  uint64_t* f_full = bars + 42;      // [kFactors]
+  uint64_t* k_full = bars + 4;       // [kRing]
+  uint64_t* k_empty = bars + 8;
+  uint64_t* v_full = bars + 12;
+  uint64_t* v_empty = bars + 16;
+  uint64_t* s_full = bars + 20;      // [half][2]
+  uint64_t* p_full = bars + 24;      // [half][2]
+  uint64_t* pv_done = bars + 28;     // [half][2]
+  uint64_t* o_free = bars + 32;      // [half]
+  uint64_t* f_full = bars + 34;      // [kFactors]
+  uint64_t* f_empty = bars + 42;     // [kFactors] P.V of the tile done: all have read them
   uint64_t* item_full = bars + 50;   // [kItems]
-  uint64_t* item_empty = bars + 54;  // [kItems] read by the converter, MMA and softmax warps
+  uint64_t* item_empty = bars + 54;  // [kItems] read by the Q, MMA and softmax warps
   uint64_t* drain = bars + 58;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 59);
 
@@ -227,10 +233,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
       mbar_init(&o_free[i], 128);
-    }
-    for (int i = 0; i < 2 * kRawRing; ++i) {
-      mbar_init(&raw_full[i], 1);
-      mbar_init(&raw_empty[i], 4);
     }
     for (int i = 0; i < kRing; ++i) {
       mbar_init(&k_full[i], 4);
@@ -243,10 +245,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&p_full[i], 128);
       mbar_init(&pv_done[i], 1);
     }
-    for (int i = 0; i < kFactors; ++i) mbar_init(&f_full[i], 1);
+    for (int i = 0; i < kFactors; ++i) {
+      mbar_init(&f_full[i], 1);
+      mbar_init(&f_empty[i], 2);
+    }
     for (int i = 0; i < kItems; ++i) {
       mbar_init(&item_full[i], 1);
-      mbar_init(&item_empty[i], 4 + 2 + 8);
+      mbar_init(&item_empty[i], 1 + 2 + 8);
     }
     mbar_init(drain, 2);
     fence_barrier_init();
@@ -277,30 +282,62 @@ __global__ void __launch_bounds__(kThreads, 1)
   // after a wait that gave up a role leaves, and the waits of the others for it give up too
   auto give_up = [&]() { report(p.status, NSLG_DEV_WAIT_TIMEOUT); };
 
-  // 128 registers a thread at launch: 2 x 128 x 184 + 128 x 80 + 128 x 64 = 512 x 128
+  // 128 registers a thread at launch: 2 x 128 x 184 + 2 x 128 x 72 = 512 x 128
   if (warp < 4) {
     // -------------------------------------------------------------- converters
-    regs_dec<80>();
+    regs_dec<72>();
     const int tid = threadIdx.x;
     // 16-code chunk c of positions t0 + 16 i. The lanes of the upper 64 dims take the
     // neighbouring position: the swizzle then puts the eight lanes that store together into
     // eight banks
     const int c = tid & 7, t0 = (tid >> 3) ^ (c >> 2);
-    int nk = 0, nv = 0;                                // K tiles, V tiles
     bool ok = true;
     const uint32_t row0 = (c >> 2) * kDimHalf + t0 * 128;
     const uint32_t at0 = row0 + (((2 * (c & 3)) ^ (t0 & 7)) << 4);
     const uint32_t at1 = row0 + (((2 * (c & 3) + 1) ^ (t0 & 7)) << 4);
-    // one tile of codes to 16 bits: K (number n of its kind) to q's type, V to f16; positions
-    // `held` of it exist
-    auto convert = [&](auto kind, int n, int held) -> bool {
+    const uint32_t from = t0 * 128 + c * 16;           // in a page's block
+    bool more = true;                                  // tiles to come behind those fetched
+    // starts the copies of tile n's codes: a group of K, a group of V (empty behind the last tile)
+    auto fetch = [&](int n) -> bool {
+      if (more) {
+        const int fs = n % kFactors;
+        if (!all_wait(&f_full[fs], (n / kFactors) & 1)) return false;
+        const int held = fac[fs].held;
+        more = held >= 0;
+        if (more) {
+          const int4 bk = *reinterpret_cast<const int4*>(fac[fs].blk);
+          const int blk[kPages] = {bk.x, bk.y, bk.z, bk.w};
+          const uint32_t plain = fac[fs].plain;
+          const uint8_t* ck = static_cast<const uint8_t*>(p.codes_k);
+          const uint8_t* cv = static_cast<const uint8_t*>(p.codes_v);
+          uint8_t* dst = raw + (n % kRawRing) * kRaw + from;
+          bool has[kPages];
+#pragma unroll
+          for (int i = 0; i < kPages; ++i) {           // position t0 + 16 i: page i of the tile
+            has[i] = blk[i] >= 0 && t0 + kPS * i < held;
+            const int64_t at = has[i] ? static_cast<int64_t>(blk[i]) * kBlockBytes + from : 0;
+            copy16(dst + i * kBlockBytes, ck + at, has[i]);
+          }
+          copy_commit();
+#pragma unroll
+          for (int i = 0; i < kPages; ++i) {           // no codes of a scale of 0 or NaN in V
+            const int64_t at = has[i] ? static_cast<int64_t>(blk[i]) * kBlockBytes + from : 0;
+            copy16(dst + kRawRing * kRaw + i * kBlockBytes, cv + at, has[i] && ((plain >> i) & 1u));
+          }
+          copy_commit();
+          return true;
+        }
+      }
+      copy_commit();
+      copy_commit();
+      return true;
+    };
+    // one tile of codes to 16 bits: K to q's type, V to f16
+    auto convert = [&](auto kind, int n) -> bool {
       constexpr int kv = decltype(kind)::value;
-      const int s = n % kRing, rs = kv * kRawRing + n % kRawRing;
-      if (!all_wait(&raw_full[rs], (n / kRawRing) & 1)) return false;
+      const int s = n % kRing;
       if (!all_wait(&(kv ? v_empty : k_empty)[s], ((n / kRing) & 1) ^ 1)) return false;
-      // pages whose codes count (V: not those of a scale of 0 or NaN)
-      const uint32_t valid = kv ? fac[n % kFactors].plain : fac[n % kFactors].valid;
-      const uint8_t* src = raw + rs * kRaw + t0 * 128 + c * 16;
+      const uint8_t* src = raw + (kv * kRawRing + n % kRawRing) * kRaw + from;
       uint8_t* dst = (kv ? sv : sk) + s * kTileBytes;
       auto two = [&](uint32_t codes) -> uint32_t {     // the low two codes
         const uint32_t h = f16x2_from_e4m3x2(static_cast<uint16_t>(codes));
@@ -314,11 +351,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint4 w[kPages];
 #pragma unroll
       for (int i = 0; i < kPages; ++i) w[i] = *reinterpret_cast<const uint4*>(src + i * kBlockBytes);
-      if (held < kBN || valid != (1u << kPages) - 1u) {
-#pragma unroll
-        for (int i = 0; i < kPages; ++i)               // position t0 + 16 i: page i of the tile
-          if (t0 + kPS * i >= held || !((valid >> i) & 1u)) w[i] = make_uint4(0u, 0u, 0u, 0u);
-      }
 #pragma unroll
       for (int i = 0; i < kPages; ++i) {
         const uint4 lo = make_uint4(two(w[i].x), two(w[i].x >> 16), two(w[i].y), two(w[i].y >> 16));
@@ -328,161 +360,200 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&raw_empty[rs]);
-        mbar_arrive(&(kv ? v_full : k_full)[s]);
-      }
+      if (lane == 0) mbar_arrive(&(kv ? v_full : k_full)[s]);
       return true;
     };
     constexpr std::integral_constant<int, 0> kK{};
     constexpr std::integral_constant<int, 1> kV{};
-    Item it;
-    for (int n = 0; (ok = take_item(n, it)) && it.ntiles >= 0; ++n) {
-      if (it.ntiles == 0) continue;
-      ok = convert(kK, nk++, it.kv_len);
-      for (int j = 0; ok && j < it.ntiles; ++j) {
-        ok = convert(kV, nv++, it.kv_len - j * kBN);
-        if (ok && j + 1 < it.ntiles) ok = convert(kK, nk++, it.kv_len - (j + 1) * kBN);
-      }
-      if (!ok) break;
+    int tiles = 0;                                     // fetched
+    for (int i = 0; ok && i < kRawRing; ++i) {
+      ok = fetch(i);
+      tiles += more ? 1 : 0;                           // false once a fetch has found the end
     }
+    for (int n = 0; ok && n < tiles; ++n) {
+      copy_wait<2 * kRawRing - 1>();
+      if (!(ok = convert(kK, n))) break;
+      copy_wait<2 * kRawRing - 2>();
+      if (!(ok = convert(kV, n))) break;
+      ok = fetch(tiles);
+      tiles += more ? 1 : 0;
+    }
+    copy_wait<0>();                                    // none may still be writing shared memory
     if (!ok && lane == 0) give_up();
   } else if (warp < 8) {
-    regs_dec<64>();
+    regs_dec<72>();
     if (warp == 4) {
       // -------------------------------------------------------------- producer
-      int nk = 0, nv = 0, n_it = 0, nq = 0;
+      // Pages are looked up 32 at a time (a group: 8 tiles of an item), one a lane, two groups
+      // ahead: their numbers, then their scales, then the factors. Tile by tile
+      // the loads' latency was 1.5 us a tile, more than all the rest of it.
+      struct Group {
+        int n, j0, page;                               // item (-1: none), first tile, the lane's page (-1: none)
+        float sk, sv;
+      };
+      int n = 0;                                       // tiles published
       float carry = 0.f;                               // least e of this item's last tile that had one
-      const uint64_t keep = l2_policy_evict_last();
-      bool ok = true;
-      // lane i < kPages: page i of tile j, -2: none, -1: outside the pool
-      auto page_of = [&](const Item& it, int j) {
-        const int pi = j * kPages + lane;
-        return lane < kPages && j < it.ntiles && pi < it.npages ? p.kv_indices[it.kv_beg + pi] : -2;
-      };
-      auto copy = [&](int kv, int n, const Item& it, int page) -> bool {
-        const int rs = kv * kRawRing + n % kRawRing;
-        if (!all_wait(&raw_empty[rs], ((n / kRawRing) & 1) ^ 1)) return false;
-        const bool has = page >= 0 && page < p.num_pages;
-        if (page != -2 && !has) report(p.status, NSLG_DEV_BAD_PAGE);
-        const uint32_t valid = __ballot_sync(0xffffffffu, has);
-        if (lane == 0) mbar_arrive_expect_tx(&raw_full[rs], __popc(valid) * kBlockBytes);
-        __syncwarp();
-        if (has)
-          bulk_load(raw + rs * kRaw + lane * kBlockBytes,
-                    static_cast<const uint8_t*>(kv ? p.codes_v : p.codes_k) +
-                        (static_cast<int64_t>(page) * p.hkv + it.h) * kBlockBytes,
-                    kBlockBytes, &raw_full[rs]);
-        return true;
-      };
-      auto scales = [&](const Item& it, int page, float& sk_, float& sv_) {
-        const bool has = page >= 0 && page < p.num_pages;
-        const int64_t blk = static_cast<int64_t>(page) * p.hkv + it.h;
-        sk_ = has ? p.scale_k[blk] : 0.f;
-        sv_ = has ? p.scale_v[blk] : 0.f;
-      };
-      auto factors = [&](int n, int page, float f, float v) {   // of tile n, before its K codes are copied
-        const bool has = page >= 0 && page < p.num_pages;
-        if (v != v) f = v;                             // NaN rides on the scores
-        float e = log2f(v);
-        const bool plain = v > 0.f && v < INFINITY;
-        float least = plain ? e : INFINITY;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
-        if (least != INFINITY) carry = least;
-        if (!plain) e = fmaxf(carry - kZeroE, -120.f);
-        const uint32_t own = __ballot_sync(0xffffffffu, plain), valid = __ballot_sync(0xffffffffu, has);
-        if (lane < kPages) {
-          Factors& fc = fac[n % kFactors];
-          fc.f[lane] = f * p.scale_log2;
-          fc.e[lane] = e;
-          fc.inv[lane] = exp2f(-e);
-          if (lane == 0) {
-            fc.valid = valid;
-            fc.plain = own;
+      int item = blockIdx.x, n_items = 0;              // items with tiles
+      int j_next = 0, nt = 0, kv_beg = 0, npages = 0;  // of the item being looked up
+      ItemLoads ahead;
+      issue_item(p, item, ahead);
+      auto fetch = [&](Group& gr) -> bool {
+        while (j_next >= nt) {                         // the next item with tiles
+          if (item >= p.n_items) {
+            gr.n = -1;
+            return true;
           }
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&f_full[n % kFactors]);
-      };
-      int n_pub = 0;
-      auto publish = [&](const Item& it) -> bool {
-        const int s = n_pub % kItems;
-        if (!all_wait(&item_empty[s], ((n_pub / kItems) & 1) ^ 1)) return false;
-        if (lane == 0) {
-          items[s] = it;
-          mbar_arrive(&item_full[s]);
-        }
-        __syncwarp();
-        ++n_pub;
-        return true;
-      };
-      ItemLoads nxt;
-      issue_item(p, blockIdx.x, nxt);
-      for (int item = blockIdx.x; ok && item < p.n_items; item += gridDim.x) {
-        const ItemLoads L = nxt;
-        issue_item(p, item + gridDim.x, nxt);
-        Item it;
-        if (!finish_item(p, L, it)) continue;
-        if (!(ok = publish(it))) break;
-        if (it.ntiles == 0) continue;
-        carry = 0.f;
-        int page = page_of(it, 0), page1 = page_of(it, 1);
-        float f, v;
-        scales(it, page, f, v);
-        for (int j = 0; ok && j < it.ntiles; ++j) {    // K(j), Q behind the first, V(j)
-          {
-            const int page2 = page_of(it, j + 2);
-            float f1 = 0.f, v1 = 0.f;
-            scales(it, page1, f1, v1);
-            // tile nk - 8 has left its ring slot: the last V copy waited until V(nk - 3) was
-            // converted, which waited for P(nk - 7).V
-            factors(nk, page, f, v);
-            if (!(ok = copy(0, nk, it, page))) break;
-            ++nk;
-            if (j == 0) {
-#pragma unroll 1
-              for (int x = 0; ok && x < 2; ++x) {
-                if (!(ok = all_wait(&q_empty[x], (n_it & 1) ^ 1))) break;
-                if (lane == 0) {
-                  mbar_arrive_expect_tx(&q_full[x], kQBytes);
-                  uint8_t* dst = sq + x * kQBytes;
-                  const int row = it.row0 + x * p.tokens_per_tile;
-                  tma_load_3d(dst, &tmap_q, &q_full[x], 0, it.h * G, row, keep);
-                  tma_load_3d(dst + kQDimHalf, &tmap_q, &q_full[x], 64, it.h * G, row, keep);
-                }
-                ++nq;
-                __syncwarp();
-              }
-              if (!ok) break;
+          const ItemLoads L = ahead;
+          item += gridDim.x;
+          issue_item(p, item, ahead);
+          Item it;
+          if (!finish_item(p, L, it)) continue;
+          if (it.ntiles == 0) {                        // rows that see no position
+            const int rows = min(2 * p.tokens_per_tile, it.qo_len - it.i0);
+            for (int i = 0; i < rows; ++i) {
+              uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) +
+                                                    (static_cast<int64_t>(it.row0) + i) * p.out_stride +
+                                                    static_cast<int64_t>(it.h) * G * kD);
+              for (int e = lane; e < G * (kD / 8); e += 32) dst[e] = make_uint4(0u, 0u, 0u, 0u);
             }
-            if (!(ok = copy(1, nv, it, page))) break;
-            ++nv;
-            page = page1;
-            page1 = page2;
-            f = f1;
-            v = v1;
+            continue;
+          }
+          // what has been published is at most two items behind: the roles get on to the item
+          // that held this slot
+          const int s = n_items % kItems;
+          if (!all_wait(&item_empty[s], ((n_items / kItems) & 1) ^ 1)) return false;
+          if (lane == 0) items[s] = it;
+          __syncwarp();
+          ++n_items;
+          j_next = 0;
+          nt = it.ntiles;
+          kv_beg = it.kv_beg;
+          npages = it.npages;
+        }
+        gr.n = n_items - 1;
+        gr.j0 = j_next;
+        const int pi = j_next * kPages + lane;
+        gr.page = -1;
+        if (pi < min(npages, nt * kPages)) {
+          gr.page = p.kv_indices[kv_beg + pi];
+          if (gr.page < 0) gr.page = -2;
+        }
+        j_next += 32 / kPages;
+        return true;
+      };
+      auto load_scales = [&](Group& gr) {
+        gr.sk = gr.sv = 0.f;
+        if (gr.n < 0) return;
+        if (gr.page < -1 || gr.page >= p.num_pages) {
+          report(p.status, NSLG_DEV_BAD_PAGE);
+          gr.page = -1;
+        }
+        if (gr.page >= 0) {
+          const int64_t blk = static_cast<int64_t>(gr.page) * p.hkv + items[gr.n % kItems].h;
+          gr.sk = p.scale_k[blk];
+          gr.sv = p.scale_v[blk];
+        }
+      };
+      auto publish = [&](const Group& gr) -> bool {
+        const int s = gr.n % kItems;
+        const int h = items[s].h, tiles = min(32 / kPages, items[s].ntiles - gr.j0);
+        if (gr.j0 == 0) carry = 0.f;
+        // ---- the factors of the lane's page
+        const float f = gr.sv != gr.sv ? gr.sv : gr.sk;   // NaN rides on the scores
+        const bool plain = gr.sv > 0.f && gr.sv < INFINITY;
+        float e = log2f(gr.sv);
+        const uint32_t own = __ballot_sync(0xffffffffu, plain);
+        float least = plain ? e : INFINITY;            // of the tile's pages
+        least = fminf(least, __shfl_xor_sync(0xffffffffu, least, 1));
+        least = fminf(least, __shfl_xor_sync(0xffffffffu, least, 2));
+        if (own != 0xffffffffu) {                      // the last tile, this one included, that has one
+          const uint32_t upto = own & ((2u << (lane | (kPages - 1))) - 1u);
+          const float last = __shfl_sync(0xffffffffu, least, upto != 0u ? 31 - __clz(upto) : 0);
+          if (!plain) e = fmaxf((upto != 0u ? last : carry) - kZeroE, -120.f);
+        }
+        if (own != 0u) carry = __shfl_sync(0xffffffffu, least, 31 - __clz(own));
+        const float inv = exp2f(-e), f_log2 = f * p.scale_log2;
+        const int blk = gr.page >= 0 ? gr.page * p.hkv + h : -1;
+        for (int j = 0; j < tiles; ++j, ++n) {
+          const int fs = n % kFactors;
+          if (!all_wait(&f_empty[fs], ((n / kFactors) & 1) ^ 1)) return false;
+          Factors& fc = fac[fs];
+          if (lane / kPages == j) {
+            fc.f[lane % kPages] = f_log2;
+            fc.e[lane % kPages] = e;
+            fc.inv[lane % kPages] = inv;
+            fc.blk[lane % kPages] = blk;
+            if (lane % kPages == 0) {
+              fc.plain = (own >> lane) & ((1u << kPages) - 1u);
+              fc.held = items[s].kv_len - (gr.j0 + j) * kBN;
+            }
+          }
+          const bool first = gr.j0 == 0 && j == 0;
+          __syncwarp();
+          if (lane == 0) {
+            if (first) mbar_arrive(&item_full[s]);
+            mbar_arrive(&f_full[fs]);
           }
         }
-        ++n_it;
+        return true;
+      };
+      Group g0, g1, g2;
+      bool ok = fetch(g0);
+      if (ok) {
+        load_scales(g0);
+        ok = fetch(g1);
+      }
+      while (ok && g0.n >= 0) {
+        load_scales(g1);
+        if (!(ok = fetch(g2)) || !(ok = publish(g0))) break;
+        g0 = g1;
+        g1 = g2;
       }
       if (ok) {
-        Item end{};
-        end.ntiles = -1;
-        ok = publish(end);
+        const int s = n_items % kItems, fs = n % kFactors;
+        ok = all_wait(&item_empty[s], ((n_items / kItems) & 1) ^ 1) &&
+             all_wait(&f_empty[fs], ((n / kFactors) & 1) ^ 1);
+        if (ok && lane == 0) {
+          items[s].ntiles = -1;
+          mbar_arrive(&item_full[s]);
+          fac[fs].held = -1;
+          mbar_arrive(&f_full[fs]);
+        }
+      }
+      if (!ok && lane == 0) give_up();
+    } else if (warp == 7) {
+      // -------------------------------------------------------------- Q
+      // a warp of its own: the rows of an item may be copied only when the last scores of the
+      // one before are done, and the producer is tiles ahead of that
+      const uint64_t keep = l2_policy_evict_last();
+      bool ok = true;
+      int nq = 0;                                      // halves copied
+      Item it;
+      for (int n = 0; (ok = take_item(n, it)) && it.ntiles >= 0; ++n) {
+#pragma unroll 1
+        for (int x = 0; ok && x < 2; ++x) {
+          if (!(ok = all_wait(&q_empty[x], (n & 1) ^ 1))) break;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&q_full[x], kQBytes);
+            uint8_t* dst = sq + x * kQBytes;
+            const int row = it.row0 + x * p.tokens_per_tile;
+            tma_load_3d(dst, &tmap_q, &q_full[x], 0, it.h * G, row, keep);
+            tma_load_3d(dst + kQDimHalf, &tmap_q, &q_full[x], 64, it.h * G, row, keep);
+          }
+          ++nq;
+          __syncwarp();
+        }
+        if (!ok) break;
       }
       if (!ok) {
         if (lane == 0) give_up();
         // no copy may still be writing shared memory when the CTA leaves (bounded waits)
-        for (int k = 0; k < 2; ++k)
-          for (int u = max((k ? nv : nk) - kRawRing, 0); u < (k ? nv : nk); ++u)
-            (void)mbar_wait(&raw_full[k * kRawRing + u % kRawRing], (u / kRawRing) & 1);
         for (int x = 0; x < 2; ++x) {
           const int loads = (nq + 1 - x) / 2;
           if (loads > 0) (void)mbar_wait(&q_full[x], (loads - 1) & 1);
         }
       }
-    } else if (warp < 7) {
+    } else {
       // -------------------------------------------------------------- MMA issuers, one per half
       // The whole warp runs the loop and one elected lane issues: the descriptors then stay
       // warp-uniform. With the loop in one lane an MMA costs enough instructions that the
@@ -501,8 +572,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // The tiles of all items form one stream. S(u) goes into the buffer of P(u - 2), right
       // behind P(u - 2).V in the pipe, so it is there when the softmax has done tile u - 1, and
       // an item's first scores are computed while the rows before are written.
-      int u = 0, sj = 0, snt = 0, n = 0, n_q = 0;   // tiles scored; tile of the item being scored;
-                                             // items taken, items with tiles
+      int u = 0, sj = 0, snt = 0, n = 0;     // tiles scored; tile of the item being scored; items
       bool end = false;
       int nts[3] = {0, 0, 0};                // tiles of the items between P.V and S, oldest first
       int held = 0;                          // ... how many
@@ -511,22 +581,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         while (!end && u <= t + 2) {
           if (sj == snt) {                   // the next item with tiles
             Item it;
-            do {
-              if (!(ok = take_item(n, it)) || it.ntiles < 0) {
-                end = true;
-                return;
-              }
-              ++n;
-            } while (it.ntiles == 0);
+            if (!(ok = take_item(n, it)) || it.ntiles < 0) {
+              end = true;
+              return;
+            }
+            ++n;
             snt = it.ntiles;
             sj = 0;
             if (held == 0) nts[0] = snt;
             else if (held == 1) nts[1] = snt;
             else nts[2] = snt;
             ++held;
-            ++n_q;
           }
-          const uint32_t q_par = (n_q - 1) & 1;
+          const uint32_t q_par = (n - 1) & 1;
           if (sj == 0) {
             if (u > t + 1 && !__all_sync(0xffffffffu, mbar_try_wait(&q_full[x], q_par))) return;
             if (!(ok = all_wait(&q_full[x], q_par))) return;
@@ -567,6 +634,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                      (pj > 0 || kt > 0) ? 1u : 0u);
           mma_commit(&pv_done[x * 2 + b]);
           mma_commit(&v_empty[slot]);
+          mma_commit(&f_empty[t % kFactors]);
         }
         __syncwarp();
         if (++pj == nts[0]) {
@@ -602,13 +670,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       T* dst = static_cast<T*>(p.out) +
                (static_cast<int64_t>(it.row0) + x * p.tokens_per_tile + tok) * p.out_stride +
                static_cast<int64_t>(it.h * G + hd) * kD;
-      if (it.ntiles == 0) {                            // rows that see no position
-        if (live)
-#pragma unroll
-          for (int i = 0; i < kD / 8; ++i) reinterpret_cast<uint4*>(dst)[i] = make_uint4(0u, 0u, 0u, 0u);
-        ok = take_item(n, nx);
-        continue;
-      }
       // last position the row sees; a row of no sequence sees everything and is not written
       const int lim = !live      ? 0x7fffffff
                       : p.causal ? min(it.kv_len - it.qo_len + i0, it.kv_len - 1)
