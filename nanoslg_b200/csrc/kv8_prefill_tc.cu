@@ -661,19 +661,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool wide = ((reinterpret_cast<uintptr_t>(p.out) | static_cast<uintptr_t>(p.out_stride) * sizeof(T)) & 31) == 0;
     int t = 0;
     bool ok = true;
+    // The rows of the item before, whose o is written behind this item's first tile of
+    // softmax: its last P.V has been done by then.
+    bool due = false;
+    T* due_dst = nullptr;                              // null: a row of no sequence
+    float due_l = 0.f;
     Item it, nx;
     ok = take_item(0, nx);
-    for (int n = 1; ok && nx.ntiles >= 0; ++n) {
+    for (int n = 1; ok && (nx.ntiles >= 0 || due); ++n) {
       it = nx;
+      const bool end = it.ntiles < 0;                  // no more: only o is due
       const int i0 = it.i0 + x * p.tokens_per_tile + tok;   // the row's new token
       const bool live = i0 < it.qo_len;
-      T* dst = static_cast<T*>(p.out) +
-               (static_cast<int64_t>(it.row0) + x * p.tokens_per_tile + tok) * p.out_stride +
-               static_cast<int64_t>(it.h * G + hd) * kD;
       // last position the row sees; a row of no sequence sees everything and is not written
       const int lim = !live      ? 0x7fffffff
                       : p.causal ? min(it.kv_len - it.qo_len + i0, it.kv_len - 1)
                                  : it.kv_len - 1;
+      const int low = __reduce_min_sync(0xffffffffu, lim);
       float m = -INFINITY, l = 0.f;
       bool seen = false;                               // a tile with an E of its own
       // one tile; edge: some row of the warp does not see all of it
@@ -761,48 +765,59 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(&p_full[x * 2 + b]);
         return true;
       };
-      for (int j = 0; j < it.ntiles; ++j, ++t) {
-        if (j + 1 == it.ntiles && !(ok = take_item(n, nx))) break;
-        if (!(ok = all_wait(&f_full[t % kFactors], (t / kFactors) & 1))) break;
-        if (!(ok = all_wait(&s_full[x * 2 + (t & 1)], (t >> 1) & 1))) break;
-        tc_fence_after();
-        if (!(ok = softmax(!__all_sync(0xffffffffu, (j + 1) * kBN - 1 <= lim), j))) break;
-      }
-      if (!ok) break;
-      const int tl = t - 1;
-      if (!(ok = all_wait(&pv_done[x * 2 + (tl & 1)], (tl >> 1) & 1))) break;
-      tc_fence_after();
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll 1
-      for (int cb = 0; cb < kD; cb += 64) {
-        float o[64];
-        tmem_ld64(base + kColO + cb, o);
-        tmem_wait_ld();
-        if (cb + 64 == kD) {
-          tc_fence_before();
-          mbar_arrive(&o_free[x]);                     // O may be overwritten now
+      for (int j = 0; j == 0 || j < it.ntiles; ++j) {
+        if (!end) {
+          if (j + 1 == it.ntiles && !(ok = take_item(n, nx))) break;
+          // S(t) is made of K(t), which was fetched with the factors: they are there
+          if (!(ok = all_wait(&s_full[x * 2 + (t & 1)], (t >> 1) & 1))) break;
+          tc_fence_after();
+          if (!(ok = softmax(!__all_sync(0xffffffffu, (j + 1) * kBN - 1 <= lim), j))) break;
         }
-        if (live) {
+        if (j == 0 && due) {
+          const int tl = t - 1;                        // the last tile of the item before
+          if (!(ok = all_wait(&pv_done[x * 2 + (tl & 1)], (tl >> 1) & 1))) break;
+          tc_fence_after();
+          const float inv = due_l == 0.f ? 0.f : 1.f / due_l;
+#pragma unroll 1
+          for (int cb = 0; cb < kD; cb += 64) {
+            float o[64];
+            tmem_ld64(base + kColO + cb, o);
+            tmem_wait_ld();
+            if (cb + 64 == kD) {
+              tc_fence_before();
+              mbar_arrive(&o_free[x]);                 // O may be overwritten now
+            }
+            if (due_dst != nullptr) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t w[8];
+              for (int c = 0; c < 4; ++c) {
+                uint32_t w[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              w[e] = Mma16<T>::pack(o[16 * c + 2 * e] * inv, o[16 * c + 2 * e + 1] * inv);
-            T* at = dst + cb + 16 * c;
-            if (wide) {
-              // a thread's row against the others' is a line each: fewer, wider stores
-              asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at),
-                           "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
-                           "r"(w[6]), "r"(w[7])
-                           : "memory");
-            } else {
-              reinterpret_cast<uint4*>(at)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-              reinterpret_cast<uint4*>(at)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+                for (int e = 0; e < 8; ++e)
+                  w[e] = Mma16<T>::pack(o[16 * c + 2 * e] * inv, o[16 * c + 2 * e + 1] * inv);
+                T* at = due_dst + cb + 16 * c;
+                if (wide) {
+                  // a thread's row against the others' is a line each: fewer, wider stores
+                  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at),
+                               "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
+                               "r"(w[6]), "r"(w[7])
+                               : "memory");
+                } else {
+                  reinterpret_cast<uint4*>(at)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                  reinterpret_cast<uint4*>(at)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+                }
+              }
             }
           }
         }
+        if (!end) ++t;
       }
+      if (end) break;
+      due = true;
+      due_l = l;
+      due_dst = live ? static_cast<T*>(p.out) +
+                           (static_cast<int64_t>(it.row0) + x * p.tokens_per_tile + tok) * p.out_stride +
+                           static_cast<int64_t>(it.h * G + hd) * kD
+                     : nullptr;
     }
     if (!ok && lane == 0) give_up();
   }
