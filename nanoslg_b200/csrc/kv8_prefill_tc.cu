@@ -69,7 +69,7 @@ constexpr int kQBytes = kBM * kD * 2;         // a Q half: [64-dim half][128 row
 constexpr int kQDimHalf = kBM * 128;
 constexpr int kTileBytes = kBN * kD * 2;      // a K or V tile: [64-dim half][64 positions][128 bytes]
 constexpr int kDimHalf = kBN * 128;
-constexpr int kRing = 4;                      // K tiles, V tiles
+constexpr int kRing = 3;                      // K tiles, V tiles
 constexpr int kRaw = kBN * kD;                // codes of a tile
 constexpr int kRawRing = 2;
 constexpr int kBlockBytes = kPS * kD;
@@ -225,6 +225,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* item_full = bars + 50;   // [kItems]
   uint64_t* item_empty = bars + 54;  // [kItems] read by the Q, MMA and softmax warps
   uint64_t* drain = bars + 58;
+  uint64_t* turn = bars + 60;        // [half][quarter] the exponentials' turn
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 59);
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -253,6 +254,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&item_full[i], 1);
       mbar_init(&item_empty[i], 1 + 2 + 8);
     }
+    for (int i = 0; i < 8; ++i) mbar_init(&turn[i], 1);
     mbar_init(drain, 2);
     fence_barrier_init();
   }
@@ -712,6 +714,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             raise && m != -INFINITY && mt != -INFINITY ? fast_exp2(m - mt) : 1.f;
         if (raise) m = mt;
         const float nb = m == -INFINITY ? 0.f : -m;
+        if (!all_wait(&turn[x * 4 + quarter], (t & 1) ^ 1 ^ x)) return false;
 #pragma unroll
         for (int g = 0; g < kPages; ++g) {
           const float add = fc.e[g] + nb;
@@ -742,6 +745,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           from_f32x2(gs, a, b2);
           sum = fmaf(a + b2, fc.inv[g], sum);
         }
+        tmem_st32(base + 64 * b, pk);                  // P over S
+        if (lane == 0) mbar_arrive(&turn[(x ^ 1) * 4 + quarter]);
+        __syncwarp();
         // O may only be rescaled once P(t-1).V(t-1) is done (tcgen05.ld / st are
         // warp-collective; rows with alpha == 1 multiply by 1)
         if (j > 0 && !anew && __any_sync(0xffffffffu, alpha != 1.f)) {
@@ -759,7 +765,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         l = fmaf(l, alpha, sum);
-        tmem_st32(base + 64 * b, pk);                  // P over S
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&p_full[x * 2 + b]);
