@@ -133,10 +133,7 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio, bool nan) 
 // heads, so cos and sin are read once. A head costs one barrier: the largest magnitudes of
 // the 16 tokens meet in one of two rows of shared memory, used in turn.
 template <typename T, int D>
-#ifndef NSLG_MB
-#define NSLG_MB 4
-#endif
-__global__ void __launch_bounds__(D, NSLG_MB * 128 / D)
+__global__ void __launch_bounds__(D, 512 / D)
     kv8_append_pages_kernel(const Kv8AppendParams p) {
   constexpr int kRow = D / 16;           // threads a row
   constexpr int kWarps = D / 32;         // 16 slots x kRow threads
@@ -152,7 +149,6 @@ __global__ void __launch_bounds__(D, NSLG_MB * 128 / D)
   if (base >= r.kv_len) return;
   const int page = p.kv_indices[r.first + pi];
   const bool paged = page >= 0 && page < p.num_pages;
-  if (!paged && tid == 0) report(p.status, NSLG_DEV_BAD_PAGE);
   const int pos = base + slot;
   const bool fresh = pos >= r.start && pos < r.kv_len;   // this thread's slot takes a new token
   const int older = max(r.start - base, 0);              // slots filled before this call
@@ -220,6 +216,8 @@ __global__ void __launch_bounds__(D, NSLG_MB * 128 / D)
       if (tid == 0) (kv ? p.scale_v : p.scale_k)[blk] = now;
     }
   }
+  // here, so that no row waits for the page's number
+  if (!paged && tid == 0) report(p.status, NSLG_DEV_BAD_PAGE);
 }
 
 // One new token a sequence (decode): a block owns a sequence and all its heads; D / 16 lanes
@@ -399,6 +397,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8App
 // 16-byte stores, consecutive threads along the output. Bound by its bytes (one read and two
 // or four written per element).
 constexpr int kGatherThreads = 256;
+constexpr int kBatch = 2;            // chunks a thread holds at a time
 
 template <typename T>
 __device__ __forceinline__ void store16(T* dst, const uint4& c, float sc) {
@@ -429,26 +428,43 @@ __global__ void __launch_bounds__(kGatherThreads) kv8_gather_kernel(const Kv8Gat
     const int lo = p.kv_indptr[b], hi = p.kv_indptr[b + 1];
     if (lo <= j && j < hi) s_fill = j == hi - 1 ? p.kv_lpl[b] : p.page_size;
   }
-  __syncthreads();
-  const int fill = s_fill;
   const bool bad = page < 0 || page >= p.num_pages;
   if (bad && tid == 0) report(p.status, NSLG_DEV_BAD_PAGE);
   const int chunks = p.d / 16, per_slot = p.hkv * chunks, n = p.page_size * per_slot;
   const int64_t blk0 = page * p.hkv;
-  for (int i = tid; i < n; i += kGatherThreads) {
-    const int s = i / per_slot, r = i - s * per_slot, h = r / chunks, c = r - h * chunks;
-    uint4 ck = make_uint4(0u, 0u, 0u, 0u), cv = ck;
-    float sk = 0.f, sv = 0.f;
-    if (!bad && s < fill) {
-      const int64_t off = ((blk0 + h) * p.page_size + s) * p.d + c * 16;
-      ck = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.codes_k) + off);
-      cv = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.codes_v) + off);
-      sk = p.scale_k[blk0 + h];
-      sv = p.scale_v[blk0 + h];
+  bool synced = false;
+  for (int i0 = tid; i0 - tid < n; i0 += kBatch * kGatherThreads) {
+    uint4 ck[kBatch], cv[kBatch];
+    float sk[kBatch], sv[kBatch];
+    int slot[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {             // every load before the first store
+      const int i = i0 + u * kGatherThreads;
+      slot[u] = i / per_slot;
+      ck[u] = cv[u] = make_uint4(0u, 0u, 0u, 0u);
+      sk[u] = sv[u] = 0.f;
+      if (!bad && i < n) {
+        const int r = i - slot[u] * per_slot, h = r / chunks, c = r - h * chunks;
+        const int64_t off = ((blk0 + h) * p.page_size + slot[u]) * p.d + c * 16;
+        ck[u] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.codes_k) + off);
+        cv[u] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.codes_v) + off);
+        sk[u] = p.scale_k[blk0 + h];
+        sv[u] = p.scale_v[blk0 + h];
+      }
     }
-    const int64_t dst = (j * n + i) * 16;
-    store16(static_cast<T*>(p.out_k) + dst, ck, sk);
-    store16(static_cast<T*>(p.out_v) + dst, cv, sv);
+    if (!synced) __syncthreads();                  // s_fill
+    synced = true;
+    const int fill = s_fill;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int i = i0 + u * kGatherThreads;
+      if (i >= n) break;
+      const bool held = slot[u] < fill;
+      const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+      const int64_t dst = (j * n + i) * 16;
+      store16(static_cast<T*>(p.out_k) + dst, held ? ck[u] : none, held ? sk[u] : 0.f);
+      store16(static_cast<T*>(p.out_v) + dst, held ? cv[u] : none, held ? sv[u] : 0.f);
+    }
   }
 }
 
