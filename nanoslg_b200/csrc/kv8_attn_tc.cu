@@ -63,9 +63,6 @@
 namespace nslg {
 namespace {
 
-#ifndef NSLG_W1
-#define NSLG_W1 12
-#endif
 constexpr int kPS = 16;
 constexpr int kMaxStages = 8;
 constexpr int kStaticSmem = 2048;     // at least the kernel's __shared__ arrays
@@ -82,11 +79,13 @@ struct TcParams : Kv8AttnParams {
   float scale_log2;
 };
 
-// W warps a CTA: 16 where the state of 8 query rows a warp fits 128 registers a thread, 8 for
-// the 16 rows of two column tiles.
+// W warps a CTA, one CTA an SM. With 12 the rings of a full SM are 192 KiB in 4 stages; at 8 query
+// rows a warp 8 / 12 / 16 warps took 119 / 98.7 / 100 us for 64 sequences of up to 8192 tokens
+// (8 kv heads of 128), 16.9 / 16.2 / 17.2 for 32 of up to 4096 (2 kv heads). The 16 rows of two
+// column tiles need more than the 168 registers of 12 warps.
 template <int NT>
 struct Shape {
-  static constexpr int kWarps = NT == 1 ? NSLG_W1 : 8;
+  static constexpr int kWarps = NT == 1 ? 12 : 8;
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kRows = 8 * NT;
 };
@@ -152,7 +151,6 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const void* tmap, uint64_
       : "memory");
 }
 
-// Sequences without pages: their rows are zeros. CTA c takes sequences c, c + grid, ...
 // Joined pieces of one row: sums relative to the running maximum m of their references.
 struct Sum {
   float m = -INFINITY, l = 0.f;
@@ -198,6 +196,7 @@ struct Join {
   Group to;
 };
 
+// Sequences without pages: their rows are zeros. CTA c takes sequences c, c + grid, ...
 template <typename T, int kThreads>
 __device__ void zero_empty(const TcParams& p, const int32_t* indptr) {
   const int words = p.hq * p.d / 8;

@@ -8,8 +8,6 @@ using namespace nslg;
 
 namespace {
 
-constexpr int kSplitRows = 64;
-
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 // Sizes and pointers every entry point of the cache shares.
@@ -273,7 +271,7 @@ int nslg_paged_prefill_kv8(int dtype, int batch, int num_qo_heads, int num_kv_he
     if (rc) return rc;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (kv8_prefill_tc_supported(dtype, p) &&
-        static_cast<int64_t>(p.hq / p.hkv) * max_qo_len > kSplitRows)
+        (kv8_prefill_tc_faster(p) || !kv8_attn_tc_supported(dtype, p)))
       return launch_kv8_prefill_tc(dtype, p, st);
     if (kv8_attn_tc_supported(dtype, p))
       return launch_kv8_attention_tc(dtype, p, workspace, workspace_bytes, st);

@@ -1,7 +1,7 @@
 // Causal prefill / extend attention over the 8-bit paged cache on the 5th-generation tensor
-// cores (tcgen05.mma, accumulators in TMEM): page_size 16, head_dim 128, bf16 or fp16 q.
+// cores (tcgen05.mma, accumulators in TMEM): page_size 16, head_dim 64 or 128, bf16 or fp16 q.
 //
-// What bounds it: 4 * 128 flop and one exponential per (query row, head, position). At 16
+// What bounds it: 4 * head_dim flop and one exponential per (query row, head, position). At 16
 // exponentials a clock and SM they take as long as the products at full rate, so everything
 // else has to stay off the softmax warps. The codes are therefore not dequantised: they are
 // only widened, which is exact (K to q's type, V to f16), and the blocks' scales join the
@@ -56,7 +56,6 @@
 namespace nslg {
 namespace {
 
-constexpr int kD = 128;
 constexpr int kBM = 128;              // rows per half
 constexpr int kBN = 64;               // positions per tile
 constexpr int kPS = 16;
@@ -65,19 +64,23 @@ constexpr int kThreads = 512;         // warps 0-3 converters, 4 producer, 5 / 6
 constexpr int kTmemCols = 512;
 constexpr int kHalfCols = 256;        // S / P of even tiles at +0, of odd ones at +64, O at +128
 constexpr int kColO = 128;
-constexpr int kQBytes = kBM * kD * 2;         // a Q half: [64-dim half][128 rows][128 bytes]
-constexpr int kQDimHalf = kBM * 128;
-constexpr int kTileBytes = kBN * kD * 2;      // a K or V tile: [64-dim half][64 positions][128 bytes]
+constexpr int kQDimHalf = kBM * 128;  // 16-bit tiles are [64 dims][rows][128 bytes]
 constexpr int kDimHalf = kBN * 128;
-constexpr int kRing = 3;                      // K tiles, V tiles
-constexpr int kRaw = kBN * kD;                // codes of a tile
+constexpr int kRing = 3;              // K tiles, V tiles
 constexpr int kRawRing = 2;
-constexpr int kBlockBytes = kPS * kD;
 constexpr float kZeroE = 60.f;
 constexpr int kFactors = 8;           // ring of the pages' factors
 constexpr int kItems = 4;             // ring of published items
-constexpr int kSmemBytes = 1024 + 2 * kQBytes + 2 * kRing * kTileBytes + 2 * kRawRing * kRaw +
-                           1536;   // and the factors, barriers and items
+template <int D>
+struct Shape {
+  static constexpr int kQBytes = kBM * D * 2;       // a Q half
+  static constexpr int kTileBytes = kBN * D * 2;    // a K or V tile
+  static constexpr int kRaw = kBN * D;              // codes of a tile
+  static constexpr int kBlockBytes = kPS * D;
+  static constexpr int kRows = 128 * 16 / D;        // positions the converters take at once
+  static constexpr int kSmemBytes = 1024 + 2 * kQBytes + 2 * kRing * kTileBytes + 2 * kRawRing * kRaw +
+                                    1536;   // and the factors, barriers and items
+};
 
 struct PrefillParams : Kv8AttnParams {
   int group, tokens_per_tile, n_items;
@@ -196,9 +199,11 @@ __device__ __forceinline__ void regs_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
 }
 
-template <typename T>
+template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
     kv8_prefill_tc_kernel(const __grid_constant__ CUtensorMap tmap_q, const PrefillParams p) {
+  constexpr int kQBytes = Shape<D>::kQBytes, kTileBytes = Shape<D>::kTileBytes;
+  constexpr int kRaw = Shape<D>::kRaw, kBlockBytes = Shape<D>::kBlockBytes;
   const int G = p.group;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -289,15 +294,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     // -------------------------------------------------------------- converters
     regs_dec<72>();
     const int tid = threadIdx.x;
-    // 16-code chunk c of positions t0 + 16 i. The lanes of the upper 64 dims take the
-    // neighbouring position: the swizzle then puts the eight lanes that store together into
-    // eight banks
-    const int c = tid & 7, t0 = (tid >> 3) ^ (c >> 2);
+    // 16-code chunk c of positions t0 + kRows i. At head_dim 128 the lanes of the upper 64 dims
+    // take the neighbouring position: the swizzle then puts the eight lanes that store
+    // together into eight banks (at 64 two positions share them anyway)
+    constexpr int kChunks = D / 16, kRows = Shape<D>::kRows, kSteps = kBN / kRows;
+    const int c = tid % kChunks, t0 = (tid / kChunks) ^ (c >> 2);
     bool ok = true;
     const uint32_t row0 = (c >> 2) * kDimHalf + t0 * 128;
     const uint32_t at0 = row0 + (((2 * (c & 3)) ^ (t0 & 7)) << 4);
     const uint32_t at1 = row0 + (((2 * (c & 3) + 1) ^ (t0 & 7)) << 4);
-    const uint32_t from = t0 * 128 + c * 16;           // in a page's block
+    const uint32_t from = t0 % kPS * D + c * 16;       // in a page's block
+    const uint32_t put = t0 * D + c * 16;              // in a raw tile
     bool more = true;                                  // tiles to come behind those fetched
     // starts the copies of tile n's codes: a group of K, a group of V (empty behind the last tile)
     auto fetch = [&](int n) -> bool {
@@ -307,25 +314,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int held = fac[fs].held;
         more = held >= 0;
         if (more) {
-          const int4 bk = *reinterpret_cast<const int4*>(fac[fs].blk);
-          const int blk[kPages] = {bk.x, bk.y, bk.z, bk.w};
           const uint32_t plain = fac[fs].plain;
           const uint8_t* ck = static_cast<const uint8_t*>(p.codes_k);
           const uint8_t* cv = static_cast<const uint8_t*>(p.codes_v);
-          uint8_t* dst = raw + (n % kRawRing) * kRaw + from;
-          bool has[kPages];
+          uint8_t* dst = raw + (n % kRawRing) * kRaw + put;
+          bool has[kSteps];
+          int64_t at[kSteps];
 #pragma unroll
-          for (int i = 0; i < kPages; ++i) {           // position t0 + 16 i: page i of the tile
-            has[i] = blk[i] >= 0 && t0 + kPS * i < held;
-            const int64_t at = has[i] ? static_cast<int64_t>(blk[i]) * kBlockBytes + from : 0;
-            copy16(dst + i * kBlockBytes, ck + at, has[i]);
+          for (int i = 0; i < kSteps; ++i) {
+            const int page = (t0 + kRows * i) / kPS;   // of the tile
+            const int blk = fac[fs].blk[page];
+            has[i] = blk >= 0 && t0 + kRows * i < held;
+            at[i] = has[i] ? static_cast<int64_t>(blk) * kBlockBytes + from : 0;
+            copy16(dst + i * kRows * D, ck + at[i], has[i]);
+            has[i] = has[i] && ((plain >> page) & 1u); // no codes of a scale of 0 or NaN in V
           }
           copy_commit();
 #pragma unroll
-          for (int i = 0; i < kPages; ++i) {           // no codes of a scale of 0 or NaN in V
-            const int64_t at = has[i] ? static_cast<int64_t>(blk[i]) * kBlockBytes + from : 0;
-            copy16(dst + kRawRing * kRaw + i * kBlockBytes, cv + at, has[i] && ((plain >> i) & 1u));
-          }
+          for (int i = 0; i < kSteps; ++i)
+            copy16(dst + kRawRing * kRaw + i * kRows * D, cv + at[i], has[i]);
           copy_commit();
           return true;
         }
@@ -339,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr int kv = decltype(kind)::value;
       const int s = n % kRing;
       if (!all_wait(&(kv ? v_empty : k_empty)[s], ((n / kRing) & 1) ^ 1)) return false;
-      const uint8_t* src = raw + (kv * kRawRing + n % kRawRing) * kRaw + from;
+      const uint8_t* src = raw + (kv * kRawRing + n % kRawRing) * kRaw + put;
       uint8_t* dst = (kv ? sv : sk) + s * kTileBytes;
       auto two = [&](uint32_t codes) -> uint32_t {     // the low two codes
         const uint32_t h = f16x2_from_e4m3x2(static_cast<uint16_t>(codes));
@@ -350,15 +357,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           return pack_bf16x2(f.x, f.y);
         }
       };
-      uint4 w[kPages];
+      uint4 w[kSteps];
 #pragma unroll
-      for (int i = 0; i < kPages; ++i) w[i] = *reinterpret_cast<const uint4*>(src + i * kBlockBytes);
+      for (int i = 0; i < kSteps; ++i) w[i] = *reinterpret_cast<const uint4*>(src + i * kRows * D);
 #pragma unroll
-      for (int i = 0; i < kPages; ++i) {
+      for (int i = 0; i < kSteps; ++i) {
         const uint4 lo = make_uint4(two(w[i].x), two(w[i].x >> 16), two(w[i].y), two(w[i].y >> 16));
         const uint4 hi = make_uint4(two(w[i].z), two(w[i].z >> 16), two(w[i].w), two(w[i].w >> 16));
-        *reinterpret_cast<uint4*>(dst + at0 + i * kPS * 128) = lo;
-        *reinterpret_cast<uint4*>(dst + at1 + i * kPS * 128) = hi;
+        *reinterpret_cast<uint4*>(dst + at0 + i * kRows * 128) = lo;
+        *reinterpret_cast<uint4*>(dst + at1 + i * kRows * 128) = hi;
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -415,8 +422,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < rows; ++i) {
               uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) +
                                                     (static_cast<int64_t>(it.row0) + i) * p.out_stride +
-                                                    static_cast<int64_t>(it.h) * G * kD);
-              for (int e = lane; e < G * (kD / 8); e += 32) dst[e] = make_uint4(0u, 0u, 0u, 0u);
+                                                    static_cast<int64_t>(it.h) * G * D);
+              for (int e = lane; e < G * (D / 8); e += 32) dst[e] = make_uint4(0u, 0u, 0u, 0u);
             }
             continue;
           }
@@ -540,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint8_t* dst = sq + x * kQBytes;
             const int row = it.row0 + x * p.tokens_per_tile;
             tma_load_3d(dst, &tmap_q, &q_full[x], 0, it.h * G, row, keep);
-            tma_load_3d(dst + kQDimHalf, &tmap_q, &q_full[x], 64, it.h * G, row, keep);
+            if constexpr (D == 128) tma_load_3d(dst + kQDimHalf, &tmap_q, &q_full[x], 64, it.h * G, row, keep);
           }
           ++nq;
           __syncwarp();
@@ -564,7 +571,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // issuing and waiting on a tile whose products take 0.7.
       const int x = warp - 5;
       constexpr uint32_t kIdescS = idesc_f16(Mma16<T>::kFormat, kBN, false);
-      constexpr uint32_t kIdescO = idesc_f16(0, kD, true);
+      constexpr uint32_t kIdescO = idesc_f16(0, D, true);
       constexpr uint32_t kDescHi = smem_desc_hi(1024);
       const uint32_t q_lo = smem_desc_lo(smem_u32(sq + x * kQBytes), 16);
       const uint32_t k_lo0 = smem_desc_lo(smem_u32(sk), 16);
@@ -606,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (elect_one()) {
             const uint32_t k_lo = k_lo0 + slot * (kTileBytes >> 4), dcol = hb + 64 * (u & 1);
 #pragma unroll
-            for (int ks = 0; ks < kD / 16; ++ks)
+            for (int ks = 0; ks < D / 16; ++ks)
               mma_ss_w(dcol, q_lo + (((ks >> 2) * kQDimHalf + (ks & 3) * 32) >> 4),
                        k_lo + (((ks >> 2) * kDimHalf + (ks & 3) * 32) >> 4), kDescHi, kIdescS,
                        ks > 0 ? 1u : 0u);
@@ -754,7 +761,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!all_wait(&pv_done[x * 2 + (b ^ 1)], ((t - 1) >> 1) & 1)) return false;
           tc_fence_after();
 #pragma unroll 1
-          for (int cb = 0; cb < kD; cb += 32) {
+          for (int cb = 0; cb < D; cb += 32) {
             float o[32];
             tmem_ld32(base + kColO + cb, o);
             tmem_wait_ld();
@@ -784,11 +791,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_after();
           const float inv = due_l == 0.f ? 0.f : 1.f / due_l;
 #pragma unroll 1
-          for (int cb = 0; cb < kD; cb += 64) {
+          for (int cb = 0; cb < D; cb += 64) {
             float o[64];
             tmem_ld64(base + kColO + cb, o);
             tmem_wait_ld();
-            if (cb + 64 == kD) {
+            if (cb + 64 == D) {
               tc_fence_before();
               mbar_arrive(&o_free[x]);                 // O may be overwritten now
             }
@@ -821,7 +828,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       due_l = l;
       due_dst = live ? static_cast<T*>(p.out) +
                            (static_cast<int64_t>(it.row0) + x * p.tokens_per_tile + tok) * p.out_stride +
-                           static_cast<int64_t>(it.h * G + hd) * kD
+                           static_cast<int64_t>(it.h * G + hd) * D
                      : nullptr;
     }
     if (!ok && lane == 0) give_up();
@@ -839,13 +846,55 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 }  // namespace
 
+namespace {
+
+template <typename T, int D>
+int launch_typed(const PrefillParams& p, cudaStream_t stream) {
+  CUtensorMap tq;
+  const int rc = encode_tiled_3d_bf16(&tq, p.q, D, p.hq, p.num_rows, static_cast<uint64_t>(D) * 2,
+                                      static_cast<uint64_t>(p.q_stride) * 2, 64, p.group,
+                                      p.tokens_per_tile);
+  if (rc != NSLG_OK) return rc;
+  constexpr int kSmemBytes = Shape<D>::kSmemBytes;
+  const int sms = sm_count();
+  const unsigned grid = static_cast<unsigned>(p.n_items < sms ? p.n_items : sms);
+  auto kern = kv8_prefill_tc_kernel<T, D>;
+  const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+  if (err != cudaSuccess) return set_error(NSLG_ERR_CUDA, cudaGetErrorString(err));
+  kern<<<grid, kThreads, kSmemBytes, stream>>>(tq, p);
+  return check_launch("kv8_prefill_tc");
+}
+
+// Pairs of query tiles of the longest sequence.
+int64_t pairs_of(int group, int max_qo_len) {
+  return (static_cast<int64_t>(max_qo_len) * group + 2 * kBM - 1) / (2 * kBM);
+}
+
+}  // namespace
+
 bool kv8_prefill_tc_supported(int dtype, const Kv8AttnParams& p) {
-  if ((dtype != NSLG_DTYPE_BF16 && dtype != NSLG_DTYPE_F16) || p.d != kD || p.page_size != kPS)
+  if ((dtype != NSLG_DTYPE_BF16 && dtype != NSLG_DTYPE_F16) || (p.d != 64 && p.d != 128) ||
+      p.page_size != kPS)
     return false;
   const int g = p.hq / p.hkv;
   if (g > 16 || kBM % g != 0 || p.num_rows >= (int64_t{1} << 31)) return false;
-  const int64_t pairs = (static_cast<int64_t>(p.max_qo_len) * g + 2 * kBM - 1) / (2 * kBM) + 1;
-  return pairs * p.batch * p.hkv < (int64_t{1} << 30);
+  if (p.num_pages * p.hkv >= (int64_t{1} << 31)) return false;   // blocks are 32-bit numbers
+  return pairs_of(g, p.max_qo_len) * p.batch * p.hkv < (int64_t{1} << 30);
+}
+
+// Against the split-KV kernel (kv8_attn_tc): that one streams the cache once per 16 query rows,
+// spread over all SMs; this one streams it once per 256, an SM to each item. A round of items
+// takes what the split kernel takes for about two tiles of 16 rows an SM, whatever the
+// lengths. Measured (us, this kernel against split; bf16, 32 / 8 heads of 128; sequences x
+// context, query rows a kv head):
+//   1 x 4096, 256 rows    80 : 43      16 x 1024, 48 rows    26 : 39
+//   4 x 4096, 128 rows    81 : 74      64 x 4096, 32 rows   305 : 257
+//   4 x 4096, 192 rows    81 : 103     64 x 4096, 48 rows   315 : 378
+bool kv8_prefill_tc_faster(const Kv8AttnParams& p) {
+  const int g = p.hq / p.hkv, sms = sm_count();
+  const int64_t vs = static_cast<int64_t>(p.batch) * p.hkv;
+  const int64_t rounds = (pairs_of(g, p.max_qo_len) * vs + sms - 1) / sms;
+  return vs * ((static_cast<int64_t>(p.max_qo_len) * g + 15) / 16) > 2 * rounds * sms;
 }
 
 int launch_kv8_prefill_tc(int dtype, const Kv8AttnParams& a, cudaStream_t stream) {
@@ -854,21 +903,11 @@ int launch_kv8_prefill_tc(int dtype, const Kv8AttnParams& a, cudaStream_t stream
   p.group = a.hq / a.hkv;
   p.tokens_per_tile = kBM / p.group;
   p.scale_log2 = a.sm_scale * 1.4426950408889634f;
-  CUtensorMap tq;
-  const int rc = encode_tiled_3d_bf16(&tq, a.q, kD, a.hq, a.num_rows, static_cast<uint64_t>(kD) * 2,
-                                      static_cast<uint64_t>(a.q_stride) * 2, 64, p.group,
-                                      p.tokens_per_tile);
-  if (rc != NSLG_OK) return rc;
-  const int64_t tiles = (static_cast<int64_t>(a.max_qo_len) + p.tokens_per_tile - 1) / p.tokens_per_tile;
-  const int64_t items = (tiles + 1) / 2 * a.batch * a.hkv;
-  p.n_items = static_cast<int>(items);
-  const int sms = sm_count();
-  const unsigned grid = static_cast<unsigned>(items < sms ? items : sms);
-  auto kern = dtype == NSLG_DTYPE_F16 ? kv8_prefill_tc_kernel<__half> : kv8_prefill_tc_kernel<__nv_bfloat16>;
-  const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-  if (err != cudaSuccess) return set_error(NSLG_ERR_CUDA, cudaGetErrorString(err));
-  kern<<<grid, kThreads, kSmemBytes, stream>>>(tq, p);
-  return check_launch("kv8_prefill_tc");
+  p.n_items = static_cast<int>(pairs_of(p.group, a.max_qo_len) * a.batch * a.hkv);
+  if (dtype == NSLG_DTYPE_F16)
+    return a.d == 128 ? launch_typed<__half, 128>(p, stream) : launch_typed<__half, 64>(p, stream);
+  return a.d == 128 ? launch_typed<__nv_bfloat16, 128>(p, stream)
+                    : launch_typed<__nv_bfloat16, 64>(p, stream);
 }
 
 }  // namespace nslg

@@ -227,6 +227,7 @@ int launch_kv8_attention_tc(int dtype, const Kv8AttnParams& p, void* workspace,
 
 // tcgen05 (kv8_prefill_tc.cu): head_dim 128, groups that divide 128.
 bool kv8_prefill_tc_supported(int dtype, const Kv8AttnParams& p);
+bool kv8_prefill_tc_faster(const Kv8AttnParams& p);   // than launch_kv8_attention_tc
 int launch_kv8_prefill_tc(int dtype, const Kv8AttnParams& p, cudaStream_t stream);
 
 }  // namespace nslg

@@ -34,8 +34,21 @@ def rows(shape, dtype, seed, spread=0.0):
     return x.to(dtype)
 
 
+def idle_for_tiles(batch, hq, hkv, max_qo_len, sms=148):
+    """How many sequences without rows and pages make a prefill of ``batch`` large enough for
+    the kernel that works on tiles of 256 query rows (each kv head of a sequence counts as
+    if it had max_qo_len rows); None where none do."""
+    rows = max_qo_len * (hq // hkv)
+    tiles, pairs = -(-rows // 16), -(-rows // 256)
+    for idle in range(400):
+        vs = (batch + idle) * hkv
+        if vs * tiles > 2 * sms * -(-pairs * vs // sms):
+            return idle
+    return None
+
+
 def random_cache(num_pages, hkv, page_size, d, device, seed, power=True):
-    """A pool of random codes (every byte, NaN codes among them, only where ``stale``)."""
+    """A pool of random finite codes, its scales powers of two (any value unless ``power``)."""
     g = torch.Generator().manual_seed(seed)
     out = []
     for _ in range(2):

@@ -297,13 +297,32 @@ PREFILL = [
     # more work items than SMs
     (torch.bfloat16, 16, 4, 128, 16, [170 + 9 * i for i in range(24)], [150 + 5 * i for i in range(24)], True, 0),
     (torch.float16, 8, 8, 128, 16, [400 - 9 * i for i in range(20)], [300 - 9 * i for i in range(20)], True, 0),
+    (torch.bfloat16, 8, 2, 64, 16, [400 - 9 * i for i in range(20)], [300 - 9 * i for i in range(20)], True, 0),
+    (torch.float16, 6, 6, 64, 16, [63, 64, 65, 1, 200], [63, 64, 65, 1, 200], False, 2),
+    (torch.bfloat16, 16, 1, 64, 16, [17, 130, 33], [17, 9, 33], True, 1),
+    (torch.float16, 16, 8, 64, 16, [70, 530], [70, 290], True, 0),
     (torch.float32, 4, 2, 64, 16, [32, 20], [32, 1], True, 0),
     (torch.bfloat16, 6, 3, 96, 5, [12, 6], [5, 6], True, 1),
 ]
 
 
-@pytest.mark.parametrize("dt,hq,hkv,d,ps,lens,counts,causal,left", PREFILL)
-def test_prefill_is_the_definition(dt, hq, hkv, d, ps, lens, counts, causal, left):
+def _with_idle(cases, shape):
+    """Each case as it is and, where it would take another kernel then, in a batch made large
+    by sequences without rows; ``shape``: (dtype, batch, hq, hkv, max_qo_len, page size)."""
+    out = []
+    for case in cases:
+        dt, batch, hq, hkv, new, ps = shape(case)
+        out.append((*case, 0))
+        idle = U.idle_for_tiles(batch, hq, hkv, new)
+        if dt != torch.float32 and ps == 16 and idle and 128 % (hq // hkv) == 0:
+            out.append((*case, idle))
+    return out
+
+
+@pytest.mark.parametrize("dt,hq,hkv,d,ps,lens,counts,causal,left,idle", _with_idle(
+    PREFILL, lambda c: (c[0], len(c[5]), c[1], c[2], max(c[6]), c[4])))
+def test_prefill_is_the_definition(dt, hq, hkv, d, ps, lens, counts, causal, left, idle):
+    lens, counts = lens + [0] * idle, counts + [0] * idle
     pages = sum(-(-n // ps) for n in lens) + 3
     tables = U.page_lists(lens, ps, pages, 21)
     cache = U.random_cache(pages, hkv, ps, d, DEV, 22)
@@ -329,27 +348,32 @@ def test_prefill_is_the_definition(dt, hq, hkv, d, ps, lens, counts, causal, lef
     assert bool((out[~real.to(DEV)] == 5.0).all())
 
 
-@pytest.mark.parametrize("dt,d", [(torch.bfloat16, 128), (torch.float16, 64), (torch.float32, 64)])
-def test_prefill_rows_that_see_nothing_are_zeros(dt, d):
+@pytest.mark.parametrize("dt,d,idle", [(torch.bfloat16, 128, 0), (torch.float16, 64, 0), (torch.float32, 64, 0),
+                                       (torch.bfloat16, 128, 90), (torch.float16, 64, 90)])
+def test_prefill_rows_that_see_nothing_are_zeros(dt, d, idle):
     """More rows than positions (row i sits at kv_len - qo_len + i < 0), and rows of a
     sequence without pages."""
     hq, hkv, ps = 8, 2, 16
     cache = U.random_cache(8, hkv, ps, d, DEV, 2)
-    lens, counts = [3, 0, 20], [5, 4, 2]
+    lens, counts = [3, 0, 20] + [0] * idle, [5, 4, 2] + [0] * idle
+    if idle:                                        # and a second pair of tiles of such rows
+        lens[1], counts[1] = 0, 80
+        lens[2], counts[2] = 20, 150
     tables = U.page_lists(lens, ps, 8, 1)
     q = U.rows((sum(counts), hq, d), dt, 3).to(DEV)
     qo = torch.tensor(np.cumsum([0] + counts), dtype=torch.int32, device=DEV)
     out = torch.full_like(q, 5.0)
     sm = 1 / math.sqrt(d)
-    ops.paged_prefill_kv8(q, qo, 5, *cache, *U.csr(tables, lens, ps, DEV), sm, out=out)
-    _check_attention(out, q, cache, tables, lens, counts, [0, 5, 9], sm, _p_half(dt))
-    assert bool((out[:2] == 0).all()) and bool((out[5:9] == 0).all())
+    ops.paged_prefill_kv8(q, qo, max(counts), *cache, *U.csr(tables, lens, ps, DEV), sm, out=out)
+    starts = [int(x) for x in np.cumsum([0] + counts)[:-1]]
+    _check_attention(out, q, cache, tables, lens, counts, starts, sm, _p_half(dt))
+    assert bool((out[:2] == 0).all()) and bool((out[5:5 + counts[1]] == 0).all())
 
 
-@pytest.mark.parametrize("dt,d,rows", [(torch.bfloat16, 128, 1), (torch.float16, 64, 7),
-                                       (torch.bfloat16, 128, 90), (torch.float16, 128, 150),
-                                       (torch.float32, 64, 5)])
-def test_scales_of_neighbouring_pages_may_differ_by_any_factor(dt, d, rows):
+@pytest.mark.parametrize("dt,d,rows,idle", _with_idle(
+    [(torch.bfloat16, 128, 1), (torch.float16, 64, 7), (torch.bfloat16, 128, 90), (torch.float16, 128, 150),
+     (torch.float16, 64, 90), (torch.float32, 64, 5)], lambda c: (c[0], 1, 8, 2, c[2], 16)))
+def test_scales_of_neighbouring_pages_may_differ_by_any_factor(dt, d, rows, idle):
     """V scales over 40 powers of two, K scales over 8 (zeros and non-powers among them): the
     pages with the large values get next to no weight where K is large."""
     hq, hkv, n = 8, 2, 333
@@ -364,8 +388,9 @@ def test_scales_of_neighbouring_pages_may_differ_by_any_factor(dt, d, rows):
         t.copy_(s)
     q = (U.rows((rows, hq, d), dt, 34) * 2).to(DEV)
     sm = 1 / math.sqrt(d)
-    plan = U.csr(table, [n], 16, DEV)
-    qo = torch.tensor([0, rows], dtype=torch.int32, device=DEV)
+    lens, tables = [n] + [0] * idle, table + [table[0][:0]] * idle
+    plan = U.csr(tables, lens, 16, DEV)
+    qo = torch.tensor([0] + [rows] * (1 + idle), dtype=torch.int32, device=DEV)
     out = ops.paged_prefill_kv8(q, qo, rows, *cache, *plan, sm)
     _check_attention(out, q, cache, table, [n], [rows], [0], sm, _p_half(dt))
     if rows == 1:
@@ -374,9 +399,10 @@ def test_scales_of_neighbouring_pages_may_differ_by_any_factor(dt, d, rows):
 
 
 @pytest.mark.parametrize("which", ["k", "v"])
-@pytest.mark.parametrize("dt,rows", [(torch.bfloat16, 12), (torch.float16, 150), (torch.bfloat16, 260),
-                                     (torch.float32, 40)])
-def test_a_block_that_is_not_finite_in_a_masked_place(dt, rows, which):
+@pytest.mark.parametrize("dt,rows,idle", _with_idle(
+    [(torch.bfloat16, 12), (torch.float16, 150), (torch.bfloat16, 260), (torch.float32, 40)],
+    lambda c: (c[0], 1, 8, 2, c[1], 16)))
+def test_a_block_that_is_not_finite_in_a_masked_place(dt, rows, idle, which):
     """Rows that come before the block see nothing of it; the others are NaN."""
     hq, hkv, d, n = 8, 2, 128, 300
     cache = U.random_cache(22, hkv, 16, d, DEV, 41)
@@ -388,8 +414,9 @@ def test_a_block_that_is_not_finite_in_a_masked_place(dt, rows, which):
     cache[i].view(torch.uint8)[page, 1] = 0          # as the append leaves such a block
     q = U.rows((rows, hq, d), dt, 43).to(DEV)
     sm = 1 / math.sqrt(d)
-    qo = torch.tensor([0, rows], dtype=torch.int32, device=DEV)
-    out = ops.paged_prefill_kv8(q, qo, rows, *cache, *U.csr(table, [n], 16, DEV), sm).cpu()
+    plan = U.csr(table + [table[0][:0]] * idle, [n] + [0] * idle, 16, DEV)
+    qo = torch.tensor([0] + [rows] * (1 + idle), dtype=torch.int32, device=DEV)
+    out = ops.paged_prefill_kv8(q, qo, rows, *cache, *plan, sm).cpu()
     first = bad * 16 - (n - rows)                    # first row that sees the block
     assert 0 <= first < rows or rows == 12
     first = max(first, 0)
@@ -410,6 +437,15 @@ def test_attention_bad_pages_are_reported():
         ops.paged_prefill_kv8(q, qo, 3, *cache, ptr, idx, lpl, 0.1)
         with pytest.raises(RuntimeError, match="page id"):
             ops.check_device_status(DEV)
+        if dt != torch.float32:                     # the kernel of the large batches
+            idle = U.idle_for_tiles(1, hq, hkv, 20)
+            q20 = U.rows((20, hq, d), dt, 3).to(DEV)
+            big = U.csr([np.array([1, 99], np.int32)] + [np.zeros(0, np.int32)] * idle, [20] + [0] * idle, 16, DEV)
+            qo = torch.tensor([0] + [20] * (1 + idle), dtype=torch.int32, device=DEV)
+            out = ops.paged_prefill_kv8(q20, qo, 20, *cache, *big, 0.1)
+            with pytest.raises(RuntimeError, match="page id"):
+                ops.check_device_status(DEV)
+            assert bool(torch.isfinite(out).all())
         ops.kv8_gather(*cache, ptr, idx, lpl, dt)
         with pytest.raises(RuntimeError, match="page id"):
             ops.check_device_status(DEV)
