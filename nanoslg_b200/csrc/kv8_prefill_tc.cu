@@ -40,8 +40,8 @@
 //                   raised; at the end of an item o / l straight to `out`.
 // TMEM per half: two S (and P over it) of 64 + O 128 columns; 512 in all.
 //
-// A block whose scale is NaN (K's or V's) gives NaN to the rows that see it: its F is NaN, and
-// masked positions are left out by selection. Every mbarrier wait is bounded; on a timeout
+// A block whose scale is NaN (K's or V's) gives NaN to the rows that see it: their scores of
+// the page are set to NaN. Every mbarrier wait is bounded; on a timeout
 // the kernel records NSLG_DEV_WAIT_TIMEOUT, waits (bounded) for what it issued, frees its
 // TMEM and returns.
 #include <cuda.h>
@@ -89,11 +89,12 @@ struct PrefillParams : Kv8AttnParams {
 
 // What a tile's pages are.
 struct alignas(16) Factors {
-  float f[kPages];      // scale_k (NaN where the block of K or V is not finite)
+  float f[kPages];      // scale_k sm_scale log2(e), above 0: a masked score, -inf, stays one
   float e[kPages];      // log2 scale_v
   float inv[kPages];    // 2^-e
   int blk[kPages];      // block (page * kv heads + head), -1: none
   uint32_t plain;       // pages with an e of their own
+  uint32_t nan;         // pages whose block of K or V is not finite
   int held;             // positions that exist, maybe more than the tile's; -1: no more tiles
 };
 
@@ -468,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int h = items[s].h, tiles = min(32 / kPages, items[s].ntiles - gr.j0);
         if (gr.j0 == 0) carry = 0.f;
         // ---- the factors of the lane's page
-        const float f = gr.sv != gr.sv ? gr.sv : gr.sk;   // NaN rides on the scores
+        const uint32_t nan = __ballot_sync(0xffffffffu, gr.sk != gr.sk || gr.sv != gr.sv);
         const bool plain = gr.sv > 0.f && gr.sv < INFINITY;
         float e = log2f(gr.sv);
         const uint32_t own = __ballot_sync(0xffffffffu, plain);
@@ -481,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!plain) e = fmaxf((upto != 0u ? last : carry) - kZeroE, -120.f);
         }
         if (own != 0u) carry = __shfl_sync(0xffffffffu, least, 31 - __clz(own));
-        const float inv = exp2f(-e), f_log2 = f * p.scale_log2;
+        const float inv = exp2f(-e), f_log2 = fmaxf(gr.sk * p.scale_log2, 1e-37f);
         const int blk = gr.page >= 0 ? gr.page * p.hkv + h : -1;
         for (int j = 0; j < tiles; ++j, ++n) {
           const int fs = n % kFactors;
@@ -494,6 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             fc.blk[lane % kPages] = blk;
             if (lane % kPages == 0) {
               fc.plain = (own >> lane) & ((1u << kPages) - 1u);
+              fc.nan = (nan >> lane) & ((1u << kPages) - 1u);
               fc.held = items[s].kv_len - (gr.j0 + j) * kBN;
             }
           }
@@ -697,14 +699,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         float s[kBN];
         tmem_ld64(base + 64 * b, s);
         tmem_wait_ld();
-        if (edge) {
+        if (edge || fc.nan != 0u) {
+          const uint32_t nan = fc.nan;
 #pragma unroll
-          for (int c = 0; c < kBN; ++c)
+          for (int c = 0; c < kBN; ++c) {
+            if ((nan >> (c / kPS)) & 1u) s[c] = NAN;
             if (c > gap) s[c] = -INFINITY;
+          }
         }
-        float mt = -INFINITY;
-#pragma unroll
-        for (int g = 0; g < kPages; ++g) {
+        auto page_max = [&](int g) {                   // of t over the page; NaN is ignored
           const float* sg = s + g * 16;
           float a = fmaxf(fmaxf(sg[0], sg[1]), sg[2]), b2 = fmaxf(fmaxf(sg[3], sg[4]), sg[5]);
           a = fmaxf(fmaxf(a, sg[6]), sg[7]);
@@ -712,14 +715,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           a = fmaxf(fmaxf(a, sg[10]), sg[11]);
           b2 = fmaxf(fmaxf(b2, sg[12]), sg[13]);
           a = fmaxf(fmaxf(a, sg[14]), sg[15]);
-          mt = fmaxf(mt, fmaf(fmaxf(a, b2), fc.f[g], fc.e[g]));   // NaN is ignored
-        }
+          return fmaf(fmaxf(a, b2), fc.f[g], fc.e[g]);
+        };
+        float alpha = 1.f;
+        auto raise_to = [&](float mt) {
+          if (m != -INFINITY && mt != -INFINITY) alpha = fast_exp2(m - mt);
+          m = mt;
+        };
         const bool own = fc.plain != 0u, anew = !seen && own;   // anew: O is all zeros so far,
         seen = seen || own;                            // M may go down too
-        const bool raise = (anew && mt > -INFINITY) || mt > m + 8.f;   // and on the first finite maximum
-        const float alpha =
-            raise && m != -INFINITY && mt != -INFINITY ? fast_exp2(m - mt) : 1.f;
-        if (raise) m = mt;
+        float mt = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < kPages; ++g) mt = fmaxf(mt, page_max(g));
+        if ((anew && mt > -INFINITY) || mt > m + 8.f) raise_to(mt);
         const float nb = m == -INFINITY ? 0.f : -m;
         if (!all_wait(&turn[x * 4 + quarter], (t & 1) ^ 1 ^ x)) return false;
 #pragma unroll
@@ -732,11 +740,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             s[c] = fast_exp2(s[c]);
             s[c + 1] = fast_exp2(s[c + 1]);
           }
-        }
-        if (edge) {                                    // F = 0 or NaN times -inf is NaN
-#pragma unroll
-          for (int c = 0; c < kBN; ++c)
-            if (c > gap) s[c] = 0.f;
         }
         float sum = 0.f;
         uint32_t pk[32];
