@@ -372,7 +372,8 @@ int nslg_plan_decode_host(int batch, int page_size, const int32_t* slots, const 
  * value = code * scale of its block (the page_size tokens of one page, one kv head). The
  * append writes the smallest power of two s with amax <= 448 s (0 for a block of zeros, at
  * least 2^-126, NaN for a block that holds a value that is not finite: all of that block
- * then reads as NaN). The readers take any scale. Page lists are the CSR of the other
+ * then reads as NaN). The readers take any scale that is finite and not negative, and NaN (on
+ * the tensor cores a V block of a scale below 2^-100 counts as zeros). Page lists are the CSR of the other
  * entry points; page 0 needs no special contents, and a page that is handed out again
  * needs no clearing. head_dim is a multiple of 32 up to 256; page_size 16 with head_dim 64
  * or 128 and 16-bit activations runs on the tensor cores, the rest on CUDA cores. Pointers
@@ -395,8 +396,8 @@ int nslg_plan_decode_host(int batch, int page_size, const int32_t* slots, const 
  * the same rows again changes nothing. A page written by a call belongs to one sequence of
  * that call (copy a shared page first, codes and scales).
  *
- * max_qo_len bounds qo_len(b). A sequence with more rows than that, more than kv_len(b) or
- * rows outside [0, num_rows) sets NSLG_DEV_BAD_PLAN and is skipped; a page outside the pool
+ * max_qo_len bounds qo_len(b). A sequence with more rows than that, more than kv_len(b),
+ * rows outside [0, num_rows) or a kv_last_page_len outside [1, page_size] sets NSLG_DEV_BAD_PLAN and is skipped; a page outside the pool
  * sets NSLG_DEV_BAD_PAGE (q is still rotated); a position outside the tables sets
  * NSLG_DEV_BAD_POSITION and the part of the page's rows the call writes stays unrotated. */
 int nslg_rope_kv8_append(int dtype, int batch, int num_qo_heads, int num_kv_heads, int head_dim,
@@ -446,7 +447,10 @@ int64_t nslg_prefill_kv8_workspace_bytes(int num_qo_heads, int num_kv_heads, int
 
 /* nslg_paged_prefill over the 8-bit cache: the same rows, mask and head conventions. Rows of
  * no sequence are left as they are; a row that sees no position (qo_len(b) > kv_len(b)) is
- * zeros. */
+ * zeros. In both calls a page outside the pool sets NSLG_DEV_BAD_PAGE (the rows that see it
+ * are finite and otherwise unspecified), and a plan that does not fit, or with 2^31 (page, kv
+ * head, 16 query rows) units or more in one call, sets NSLG_DEV_BAD_PLAN and leaves rows
+ * unwritten. */
 int nslg_paged_prefill_kv8(int dtype, int batch, int num_qo_heads, int num_kv_heads, int head_dim,
                            int page_size, const void* q, int64_t q_stride, int64_t q_rows,
                            void* out, int64_t out_stride, const int32_t* qo_indptr,

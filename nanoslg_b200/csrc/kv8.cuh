@@ -48,6 +48,14 @@ __device__ __forceinline__ float scale_from_amax(uint32_t bits) {
   return __uint_as_float(static_cast<uint32_t>(e < 1 ? 1 : e) << 23);
 }
 
+// The tensor-core readers take V's scale as a power of two in the exponent of a weight, and its
+// inverse in the row's sum, which must not overflow: a V block of a smaller scale than this
+// counts as zeros there (values below 448 * 2^-100).
+constexpr float kLeastE = -100.f;
+__device__ __forceinline__ bool has_exponent(float scale) {
+  return scale >= 7.888609052210118e-31f && scale < INFINITY;   // 2^-100; not NaN
+}
+
 // The larger of two scales; NaN wins.
 __device__ __forceinline__ float scale_max(float a, float b) {
   return (a != a || b != b) ? __uint_as_float(0x7FC00000u) : fmaxf(a, b);

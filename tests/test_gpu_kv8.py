@@ -155,8 +155,10 @@ def test_append_bad_plans_are_reported_and_skipped():
     x = U.rows((12, hkv, d), torch.bfloat16, 1).to(DEV)
     cos, sin = (t.to(DEV) for t in _tables(64, d))
 
-    def run(qo, most, table, length, rows=None, tables=(cos, sin)):
+    def run(qo, most, table, length, rows=None, tables=(cos, sin), last=None):
         ptr, idx, lpl = U.csr([np.array(table, np.int32)], [length], 16, DEV)
+        if last is not None:
+            lpl.fill_(last)
         rs = None if rows is None else torch.tensor([rows], dtype=torch.int32, device=DEV)
         q = torch.full_like(x, 9.0)
         ops.rope_kv8_append(x, x, x, *tables, *cache, torch.tensor([0, qo], dtype=torch.int32, device=DEV),
@@ -165,6 +167,8 @@ def test_append_bad_plans_are_reported_and_skipped():
 
     for args, what in (((12, 12, [1], 5), "plan entry"), ((12, 4, [1], 16), "plan entry"),
                        ((4, 4, [1], 16, 10), "plan entry"), ((4, 4, [1], 16, -1), "plan entry"),
+                       ((1, 1, [1], 16, None, (cos, sin), 17), "plan entry"),
+                       ((4, 4, [1], 16, None, (cos, sin), 0), "plan entry"),
                        ((4, 4, [8], 16), "page id"), ((4, 4, [-1], 16), "page id")):
         q = run(*args)
         with pytest.raises(RuntimeError, match=what):
@@ -396,6 +400,43 @@ def test_scales_of_neighbouring_pages_may_differ_by_any_factor(dt, d, rows, idle
     if rows == 1:
         out = ops.paged_decode_kv8(q, *cache, *plan, sm)
         _check_attention(out, q, cache, table, [n], [1], [0], sm, _p_half(dt))
+
+
+@pytest.mark.parametrize("lo,hi", [(-98, -90), (96, 104)])
+@pytest.mark.parametrize("d,rows,idle", _with_idle([(128, 1), (128, 40), (64, 40)],
+                                                   lambda c: (torch.bfloat16, 1, 8, 2, c[1], 16)))
+def test_scales_far_from_one(d, rows, idle, lo, hi):
+    """V scales whose inverses, summed over a row, come near fp32's limits."""
+    hq, hkv, n = 8, 2, 200
+    cache = U.random_cache(20, hkv, 16, d, DEV, 51)
+    table = U.page_lists([n], 16, 20, 52)
+    g = torch.Generator().manual_seed(53)
+    cache[3].copy_(torch.exp2(torch.randint(lo, hi, cache[3].shape, generator=g).float()))
+    q = U.rows((rows, hq, d), torch.bfloat16, 54).to(DEV)
+    plan = U.csr(table + [table[0][:0]] * idle, [n] + [0] * idle, 16, DEV)
+    qo = torch.tensor([0] + [rows] * (1 + idle), dtype=torch.int32, device=DEV)
+    sm = 1 / math.sqrt(d)
+    out = ops.paged_prefill_kv8(q, qo, rows, *cache, *plan, sm)
+    _check_attention(out, q, cache, table, [n], [rows], [0], sm, _p_half(torch.bfloat16))
+
+
+def test_v_blocks_of_the_smallest_scales():
+    """Scales of 2^-126 .. 2^-101: the outputs are at most the values themselves, never
+    infinite or NaN, and a larger block beside them is exact."""
+    hq, hkv, d, n = 8, 2, 128, 96
+    for rows, idle in ((1, 0), (40, U.idle_for_tiles(1, hq, hkv, 40))):
+        cache = U.random_cache(8, hkv, 16, d, DEV, 61)
+        table = U.page_lists([n], 16, 8, 62)
+        cache[3].copy_(torch.exp2(torch.randint(-126, -100, cache[3].shape,
+                                                generator=torch.Generator().manual_seed(63)).float()))
+        q = U.rows((rows, hq, d), torch.bfloat16, 64).to(DEV)
+        plan = U.csr(table + [table[0][:0]] * idle, [n] + [0] * idle, 16, DEV)
+        qo = torch.tensor([0] + [rows] * (1 + idle), dtype=torch.int32, device=DEV)
+        out = ops.paged_prefill_kv8(q, qo, rows, *cache, *plan, 0.1).float()
+        assert bool((out.abs() <= 448 * 2.0 ** -100).all())
+        cache[3][int(table[0][2])] = 0.5
+        out = ops.paged_prefill_kv8(q, qo, rows, *cache, *plan, 0.1)
+        _check_attention(out, q, cache, table, [n], [rows], [0], 0.1, _p_half(torch.bfloat16))
 
 
 @pytest.mark.parametrize("which", ["k", "v"])
