@@ -59,6 +59,7 @@
 #include <cuda.h>
 
 #include <string>
+#include <type_traits>
 
 #include "kv8.cuh"
 #include "launch.h"
@@ -741,27 +742,36 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
     if (!s_last[k]) continue;
     const Join& jn = s_join[k];
     const int cnt = jn.cnt;
-    for (int e = threadIdx.x; e < per_group; e += kThreads) {
-      const int row = e / DQ, dq = e % DQ;
-      Sum sum;
-      // kBatch partials at a time, every load of a batch in flight at once. Partial i is CTA
-      // cf + i's: the one that begins there for the first, the one that began before else.
-      constexpr int kBatch = 8;
-      for (int i0 = 0; i0 < cnt; i0 += kBatch) {
-        float2 x[kBatch];
-        float4 a[kBatch];
+    // kBatch partials at a time, every load of a batch in flight at once: 4 where that is all (a
+    // batch of sequences; the loads that repeat the last one cost: 12 for all of them took 0.6 us
+    // more on one of 513 tokens), 12 for a few that are spread over many CTAs (5 rows on 4001 tokens
+    // tokens 19.8 us with 8, 18.3 with 12). Partial i is CTA cf + i's: the one that begins there for the
+    // first, the one that began before else.
+    auto join = [&](auto batch) {
+      constexpr int kBatch = decltype(batch)::value;
+      for (int e = threadIdx.x; e < per_group; e += kThreads) {
+        const int row = e / DQ, dq = e % DQ;
+        Sum sum;
+        for (int i0 = 0; i0 < cnt; i0 += kBatch) {
+          float2 x[kBatch];
+          float4 a[kBatch];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int at = min(i0 + i, cnt - 1);
-          const int64_t r = (2ll * (jn.cf + at) + (at == 0 ? 1 : 0)) * p.rows + row;
-          x[i] = __ldcg(reinterpret_cast<const float2*>(p.part_ml + 2 * r));
-          a[i] = __ldcg(reinterpret_cast<const float4*>(p.part_o + r * D + 4 * dq));
+          for (int i = 0; i < kBatch; ++i) {
+            const int at = min(i0 + i, cnt - 1);
+            const int64_t r = (2ll * (jn.cf + at) + (at == 0 ? 1 : 0)) * p.rows + row;
+            x[i] = __ldcg(reinterpret_cast<const float2*>(p.part_ml + 2 * r));
+            a[i] = __ldcg(reinterpret_cast<const float4*>(p.part_o + r * D + 4 * dq));
+          }
+          sum.template add<kBatch>(x, a, cnt - i0);
         }
-        sum.add<kBatch>(x, a, cnt - i0);
+        T* dst = out_row(jn.to, row);
+        if (dst != nullptr) store_out(dst + 4 * dq, sum.acc, sum.l);
       }
-      T* dst = out_row(jn.to, row);
-      if (dst != nullptr) store_out(dst + 4 * dq, sum.acc, sum.l);
-    }
+    };
+    if (cnt <= 4)
+      join(std::integral_constant<int, 4>{});
+    else
+      join(std::integral_constant<int, 12>{});
   }
 }
 
