@@ -373,12 +373,12 @@ int nslg_plan_decode_host(int batch, int page_size, const int32_t* slots, const 
  * append writes the smallest power of two s with amax <= 448 s (0 for a block of zeros, at
  * least 2^-126, NaN for a block that holds a value that is not finite: all of that block
  * then reads as NaN). The readers take any scale that is finite and not negative, and NaN (on
- * the tensor cores a V block of a scale below 2^-100 counts as zeros). Page lists are the CSR of the other
- * entry points; page 0 needs no special contents, and a page that is handed out again
- * needs no clearing. head_dim is a multiple of 32 up to 256; page_size 16 with head_dim 64
- * or 128 and 16-bit activations runs on the tensor cores, the rest on CUDA cores. Pointers
- * are 16-byte aligned (scales 4), row strides are in elements, a multiple of 16 bytes, and
- * cover a row. */
+ * the tensor cores a V block of a scale below 2^-100 counts as zeros). Page lists are the CSR
+ * of the other entry points; page 0 needs no special contents, and a page that is handed out
+ * again needs no clearing. head_dim is a multiple of 32 up to 256, a page of one layer has
+ * fewer than 2^31 elements; page_size 16 with head_dim 64 or 128 and 16-bit activations runs
+ * on the tensor cores, the rest on CUDA cores. Pointers are 16-byte aligned (scales 4), row
+ * strides are in elements, a multiple of 16 bytes, and cover a row. */
 
 /* Rotary embedding of q and k, and k and v quantised into the pages as they are written.
  * Sequence b has qo_len(b) = qo_indptr[b+1] - qo_indptr[b] new rows, rows q_row_start[b] + i
@@ -448,9 +448,9 @@ int64_t nslg_prefill_kv8_workspace_bytes(int num_qo_heads, int num_kv_heads, int
 /* nslg_paged_prefill over the 8-bit cache: the same rows, mask and head conventions. Rows of
  * no sequence are left as they are; a row that sees no position (qo_len(b) > kv_len(b)) is
  * zeros. In both calls a page outside the pool sets NSLG_DEV_BAD_PAGE (the rows that see it
- * are finite and otherwise unspecified), and a plan that does not fit, or with 2^31 (page, kv
- * head, 16 query rows) units or more in one call, sets NSLG_DEV_BAD_PLAN and leaves rows
- * unwritten. */
+ * are finite and otherwise unspecified), and a plan that does not fit (as above), or with
+ * 2^31 (page, kv head, 16 query rows) units or more in one call, sets NSLG_DEV_BAD_PLAN; its
+ * rows are unspecified. */
 int nslg_paged_prefill_kv8(int dtype, int batch, int num_qo_heads, int num_kv_heads, int head_dim,
                            int page_size, const void* q, int64_t q_stride, int64_t q_rows,
                            void* out, int64_t out_stride, const int32_t* qo_indptr,

@@ -4,9 +4,9 @@
 // What bounds it: the bytes of the cache, one per element, read once. So every SM streams
 // an equal share of them whatever the sequences' lengths, and the arithmetic per byte is
 // kept below what an SM can issue in the time its share of the bandwidth takes. Measured
-// (bf16, 32 / 8 heads of 128): 64 sequences of 512 to 8192 tokens 98.7 us, 6.05 TB/s, 0.93 of
-// a copy's rate; 64 of 513 to 768 24.3 us (87 MB: 13.3 at that rate, and about 9 us of launch,
-// plan, first loads and joining, none of which the batch's size changes); one of 513 8.3 us.
+// (bf16, 32 / 8 heads of 128): 64 sequences of 512 to 8192 tokens 98 us, 6.1 TB/s, 0.93 of
+// a copy's rate; 64 of 513 to 768 23.9 us (87 MB: 13.3 at that rate, and about 9 us of launch,
+// plan, first loads and joining, none of which the batch's size changes); one of 513 8.0 us.
 //
 // Work split. A unit is one page of one kv head: 16 tokens, K and V blocks of 16 * head_dim
 // bytes each, contiguous, with one scale each. A "virtual sequence" is (sequence, kv head,
@@ -368,7 +368,12 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
     t.r0 = vs % p.tiles * Shape<NT>::kRows;
     t.qo_len = new_rows(p, t.b, &t.row0);
     t.pages = indptr[t.b + 1] - indptr[t.b];
-    t.kv_len = (t.pages - 1) * kPS + lpl[t.b];
+    int last = lpl[t.b];
+    if (last < 1 || last > kPS) {
+      report(p.status, NSLG_DEV_BAD_PLAN);
+      last = kPS;
+    }
+    t.kv_len = (t.pages - 1) * kPS + last;
     low = 0x7fffffff;
     ev = 0.f;
     seen = false;
@@ -744,9 +749,9 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
     const int cnt = jn.cnt;
     // kBatch partials at a time, every load of a batch in flight at once: 4 where that is all (a
     // batch of sequences; the loads that repeat the last one cost: 12 for all of them took 0.6 us
-    // more on one of 513 tokens), 12 for a few that are spread over many CTAs (5 rows on 4001 tokens
-    // tokens 19.8 us with 8, 18.3 with 12). Partial i is CTA cf + i's: the one that begins there for the
-    // first, the one that began before else.
+    // more on one of 513 tokens), 12 for a few that are spread over many CTAs (5 rows on
+    // 4001 tokens 19.8 us with 8, 18.3 with 12). Partial i is CTA cf + i's: the one that begins
+    // there for the first, the one that began before else.
     auto join = [&](auto batch) {
       constexpr int kBatch = decltype(batch)::value;
       for (int e = threadIdx.x; e < per_group; e += kThreads) {

@@ -1,5 +1,6 @@
 // extern "C" entry points of the 8-bit KV cache (include/nslg_b200.h): argument checks and
 // the choice of kernel. Nothing is thrown across the boundary.
+#include <algorithm>
 #include <string>
 
 #include "launch.h"
@@ -21,6 +22,8 @@ int check_cache(const std::string& what, int dtype, int batch, int hkv, int d, i
     return set_error(NSLG_ERR_UNSUPPORTED, what + ": head_dim must be a multiple of 32, at most 256");
   if (page_size <= 0 || page_size > 65536 || c.num_pages <= 0)
     return set_error(NSLG_ERR_ARG, what + ": page_size and num_pages must be positive");
+  if (static_cast<int64_t>(page_size) * hkv * d >= (int64_t{1} << 31))
+    return set_error(NSLG_ERR_UNSUPPORTED, what + ": a page of 2^31 elements or more");
   if (!c.codes_k || !c.codes_v || !c.scale_k || !c.scale_v)
     return set_error(NSLG_ERR_ARG, what + ": null cache pointer");
   if (!c.kv_indptr || !c.kv_indices || !c.kv_lpl)
@@ -126,8 +129,11 @@ int nslg_rope_kv8_append(int dtype, int batch, int num_qo_heads, int num_kv_head
     p.d = head_dim;
     p.page_size = page_size;
     p.group = num_qo_heads / num_kv_heads;
-    p.max_qo_len = max_qo_len;
-    p.pages_per_seq = static_cast<int>((static_cast<int64_t>(max_qo_len) + page_size - 2) / page_size) + 1;
+    if (static_cast<int64_t>(page_size) * p.group * head_dim >= (int64_t{1} << 31))
+      return set_error(NSLG_ERR_UNSUPPORTED, what + ": a page's query rows of 2^31 elements or more");
+    if (num_rows == 0) return NSLG_OK;
+    p.max_qo_len = static_cast<int>(std::min<int64_t>(max_qo_len, num_rows));   // more never fit
+    p.pages_per_seq = static_cast<int>((static_cast<int64_t>(p.max_qo_len) + page_size - 2) / page_size) + 1;
     p.status = dev_status;
     return launch_kv8_append(dtype, p, static_cast<cudaStream_t>(stream));
   });
@@ -263,7 +269,7 @@ int nslg_paged_prefill_kv8(int dtype, int batch, int num_qo_heads, int num_kv_he
     p.hkv = num_kv_heads;
     p.d = head_dim;
     p.page_size = page_size;
-    p.max_qo_len = max_qo_len;
+    p.max_qo_len = static_cast<int>(std::min<int64_t>(max_qo_len, q_rows));   // more never fit
     p.causal = causal ? 1 : 0;
     p.sm_scale = sm_scale;
     p.status = dev_status;

@@ -138,7 +138,7 @@ __device__ __forceinline__ bool finish_item(const PrefillParams& p, const ItemLo
   it.h = L.h;
   it.qo_len = L.qo1 - L.qo0;
   if (it.qo_len <= 0) return false;
-  if (it.qo_len > p.max_qo_len || L.start < 0 ||
+  if (it.qo_len > p.max_qo_len || L.start < 0 || (L.ip1 > L.ip0 && (L.lpl < 1 || L.lpl > kPS)) ||
       static_cast<int64_t>(L.start) + it.qo_len > p.num_rows) {
     report(p.status, NSLG_DEV_BAD_PLAN);
     return false;

@@ -390,6 +390,8 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (e.type != nullptr) PyErr_SetString(e.type, e.msg.c_str());
   } catch (const std::exception& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (...) {
+    PyErr_SetString(PyExc_RuntimeError, "8-bit KV cache: unknown C++ exception");
   }
   return nullptr;
 }

@@ -504,3 +504,81 @@ def test_a_block_that_is_not_finite_reads_as_nan():
             out = ops.paged_decode_kv8(q, *cache, *plan, 0.1)
             assert bool(torch.isnan(out[0, 4:]).all()) and bool(torch.isfinite(out[0, :4]).all())
             cache[i][2, 1] = keep
+
+
+def test_bad_last_page_lengths_are_reported():
+    hq, hkv, d = 8, 2, 128
+    for dt, rows in ((torch.bfloat16, 1), (torch.bfloat16, 20), (torch.float32, 3)):
+        cache = U.random_cache(4, hkv, 16, d, DEV, 2)
+        idle = U.idle_for_tiles(1, hq, hkv, rows) if rows == 20 else 0
+        ptr, idx, lpl = U.csr([np.array([1, 2], np.int32)] + [np.zeros(0, np.int32)] * idle,
+                              [30] + [0] * idle, 16, DEV)
+        q = U.rows((rows, hq, d), dt, 3).to(DEV)
+        qo = torch.tensor([0] + [rows] * (1 + idle), dtype=torch.int32, device=DEV)
+        for last in (0, 17, 2 ** 31 - 1, -2 ** 31):
+            lpl[0] = last
+            ops.paged_prefill_kv8(q, qo, rows, *cache, ptr, idx, lpl, 0.1)
+            with pytest.raises(RuntimeError, match="plan entry"):
+                ops.check_device_status(DEV)
+
+
+def test_more_sequences_than_shared_memory_holds():
+    """The page list's bounds are read from global memory behind 2048 sequences."""
+    hq, hkv, d, n = 2, 1, 64, 2100
+    lens = [(7 * i) % 41 for i in range(n)]
+    pages = sum(-(-x // 16) for x in lens) + 1
+    tables = U.page_lists(lens, 16, pages, 71)
+    cache = U.random_cache(pages, hkv, 16, d, DEV, 72)
+    q = U.rows((n, hq, d), torch.bfloat16, 73).to(DEV)
+    out = ops.paged_decode_kv8(q, *cache, *U.csr(tables, lens, 16, DEV), 0.125)
+    _check_attention(out, q, cache, tables, lens, [1] * n, list(range(n)), 0.125, U.HALF[torch.bfloat16])
+
+
+def test_max_qo_len_beyond_the_rows():
+    """A bound above the rows there are changes nothing, however large."""
+    hq, hkv, d, lens, counts = 16, 2, 64, [40, 9], [3, 2]
+    cache = U.random_cache(8, hkv, 16, d, DEV, 81)
+    tables = U.page_lists(lens, 16, 8, 82)
+    plan = U.csr(tables, lens, 16, DEV)
+    q = U.rows((5, hq, d), torch.bfloat16, 83).to(DEV)
+    qo = torch.tensor([0, 3, 5], dtype=torch.int32, device=DEV)
+    out = ops.paged_prefill_kv8(q, qo, 2 ** 31 - 1, *cache, *plan, 0.125)
+    _check_attention(out, q, cache, tables, lens, counts, [0, 3], 0.125, U.HALF[torch.bfloat16])
+    k = U.rows((5, hkv, d), torch.bfloat16, 84).to(DEV)
+    got, want = ([t.clone() for t in cache] for _ in range(2))
+    ops.rope_kv8_append(None, k, k, None, None, *got, qo, 2 ** 31 - 1, *plan, rotate=False)
+    ops.rope_kv8_append(None, k, k, None, None, *want, qo, 3, *plan, rotate=False)
+    for a, b in zip(got, want):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_offsets_beyond_32_bits():
+    """The same pages at the end of a pool of 2^32 bytes and more a tensor."""
+    hq, hkv, d, lens, counts = 32, 8, 128, [70, 33, 200], [20, 1, 45]
+    few = sum(-(-n // 16) for n in lens) + 1
+    small = U.random_cache(few, hkv, 16, d, DEV, 91)
+    far = 2 ** 32 // (hkv * 16 * d) + 1
+    big = ops.kv8_pages(far + few, 16, hkv, d, DEV)
+    for b, s in zip(big, small):
+        b[far:].view(torch.uint8).copy_(s.view(torch.uint8))
+    tables = U.page_lists(lens, 16, few, 92)
+    ptr, idx, lpl = U.csr(tables, lens, 16, DEV)
+    q = U.rows((sum(counts), hq, d), torch.bfloat16, 93).to(DEV)
+    k = U.rows((sum(counts), hkv, d), torch.bfloat16, 94).to(DEV)
+    qo = torch.tensor(np.cumsum([0] + counts), dtype=torch.int32, device=DEV)
+    idle = U.idle_for_tiles(3, hq, hkv, 45)
+    results = []
+    for cache, at in ((small, 0), (big, far)):
+        plan = (ptr, idx + at, lpl)
+        ops.rope_kv8_append(None, k, -k, None, None, *cache, qo, 45, *plan, rotate=False)
+        one = (q[:3].contiguous(), *cache, *plan, 0.1)
+        wide = (torch.cat([ptr, ptr[-1:].expand(idle)]), idx + at, torch.cat([lpl, lpl[:1].expand(idle)]))
+        qo_wide = torch.cat([qo, qo[-1:].expand(idle)])
+        results.append([*ops.kv8_gather(*cache, *plan, torch.bfloat16), ops.paged_decode_kv8(*one),
+                        ops.paged_prefill_kv8(q, qo, 45, *cache, *plan, 0.1),
+                        ops.paged_prefill_kv8(q, qo_wide, 45, *cache, *wide, 0.1)])
+    for a, b in zip(*results):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    for b, s in zip(big, small):
+        assert torch.equal(b[far:].view(torch.uint8), s.view(torch.uint8))
+        assert not bool(b[:64].view(torch.uint8).any())
