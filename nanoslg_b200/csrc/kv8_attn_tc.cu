@@ -622,20 +622,22 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
         pb[nt][1] = movmatrix_trans(pack_f16x2(pr[2], pr[3]));
       }
       // ---- o^T += V^T . p^T
-      uint32_t clear[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
-      if (held < kPS || !plain) {   // codes behind the last token, and of a scale of 0 or NaN, count as 0
+      // selectors that pair the bytes of tokens 2tq and 2tq + 1 (+ 8 for the second); codes
+      // behind the last token, and of a scale of 0 or NaN, count as 0 (byte 4)
+      uint32_t sel[2] = {0x3120u, 0x3120u};
+      if (held < kPS || !plain) {
         const int live = plain ? held : 0;
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          clear[e] = (tq * 2 + 8 * e < live ? 0x00FF00FFu : 0u) |
-                     (tq * 2 + 8 * e + 1 < live ? 0xFF00FF00u : 0u);
+          sel[e] = (tq * 2 + 8 * e < live ? 0x0100u : 0x0404u) |
+                   (tq * 2 + 8 * e + 1 < live ? 0x3020u : 0x4040u);
       }
 #pragma unroll
       for (int k = 0; k < KS; k += 2) {
         uint32_t w[4];
         ldmatrix_x4_trans(vb + tile_offset<D>(ltok, k + lch), w[0], w[1], w[2], w[3]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = __byte_perm(w[e], 0u, 0x3120) & clear[e & 1];
+        for (int e = 0; e < 4; ++e) w[e] = __byte_perm(w[e], 0u, sel[e & 1]);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const uint32_t a[4] = {f16x2_from_e4m3x2(static_cast<uint16_t>(w[2 * e])),
