@@ -52,6 +52,15 @@ __device__ __forceinline__ float scale_from_amax(uint32_t bits) {
 // inverse in the row's sum, which must not overflow: a V block of a smaller scale than this
 // counts as zeros there (values below 448 * 2^-100).
 constexpr float kLeastE = -100.f;
+// A block of zeros in V (or of a scale below 2^-100, or NaN) has no exponent, only a part in the
+// row's sum l. Behind blocks that have one it takes one kZeroE below theirs, so that the running
+// maximum M follows it only where it outweighs them by 2^60. Before any it takes 0: M and l are
+// those of the plain scores, and the first block with an exponent sets M anew, whatever its
+// magnitude, but not by more than kMostDown downwards: l, at most 2^8 a position until then, is
+// multiplied by 2^kMostDown at most, and a row whose weights lie further below a block of zeros
+// is less than 448 * 2^-90.
+constexpr float kZeroE = 60.f;
+constexpr float kMostDown = 90.f;
 __device__ __forceinline__ bool has_exponent(float scale) {
   return scale >= 7.888609052210118e-31f && scale < INFINITY;   // 2^-100; not NaN
 }

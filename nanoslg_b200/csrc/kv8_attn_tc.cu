@@ -33,9 +33,8 @@
 // The scales cost nothing per element: K's is a factor the score needs anyway, V's joins the
 // exponent, so p is what multiplies the code and M follows the largest of these weights.
 // p is rounded to f16 (2^-11, whatever the activation type) relative to that, so the scales
-// of neighbouring pages may differ by any factor. A block of zeros in V has no E, only a part
-// in l: it takes one kZeroE below the last page's, so that it raises M only where it outweighs
-// the row's other pages by 2^60, and the first page that has an E sets M anew.
+// of neighbouring pages may differ by any factor. Blocks of zeros in V, which have no E, stand
+// at kZeroE.
 // Against rows-first products (16 query rows, 4 of them in use at a group of 4) this halves
 // the products, the accumulators (32 registers instead of 64 at head_dim 128, so 12 warps
 // fit an SM instead of 8) and the exponentials.
@@ -72,7 +71,6 @@ constexpr int kMaxStages = 8;
 constexpr int kStaticSmem = 2048;     // at least the kernel's __shared__ arrays
 constexpr int kMaxSmem = 232448;      // 227 KiB
 constexpr int kSmemBatch = 2048;      // batches up to this size keep the page list's bounds in smem
-constexpr float kZeroE = 60.f;
 constexpr float kHeadroom = 8.f;      // log2 of the largest probability before m is raised
 
 struct TcParams : Kv8AttnParams {
@@ -540,7 +538,7 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
         ev = eu;
         seen = true;
       } else {
-        eu = fmaxf(ev - kZeroE, kLeastE);
+        eu = seen ? fmaxf(ev - kZeroE, kLeastE) : 0.f;
         iu = fast_exp2(-eu);
       }
       ok = __all_sync(0xffffffffu, mbar_wait(&full[slot], phase));
@@ -597,7 +595,7 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
             // anew: o is all zeros, M may go down (where the row sees the page)
-            const float mn = anew && x > -INFINITY ? x : fmaxf(m[nt][e], x);
+            const float mn = anew && x > -INFINITY ? fmaxf(x, m[nt][e] - kMostDown) : fmaxf(m[nt][e], x);
             const float cf = mn == -INFINITY || m[nt][e] == -INFINITY ? 1.f : fast_exp2(m[nt][e] - mn);
             m[nt][e] = mn;
             nb[nt][e] = mn == -INFINITY ? 0.f : -mn;

@@ -14,11 +14,9 @@
 //   p_j = 2^(t_j - M)        M: running maximum of t, raised when passed by 8
 //   o   = sum_j p_j code_v[j];  l = sum_g 2^-E_g sum_{j in g} p_j;  out = o / l
 // so p is what multiplies the code in the f16 product, M follows the largest of these
-// weights, and no ratio of scales between pages can underflow what matters (a block of zeros
-// in V has no E, only a part in l: it takes one kZeroE below the tile's least, so that it
-// raises M only where it outweighs the row's other pages by 2^60; the first tile with an E of
-// its own sets M anew). F >= 0 makes the
-// maximum of t over a page a function of the maximum of s. p is f16 (2^-11) for both
+// weights, and no ratio of scales between pages can underflow what matters (blocks of zeros in
+// V, which have no E, stand at kZeroE). F > 0 makes the maximum of t over a page a function of
+// the maximum of s. p is f16 (2^-11) for both
 // activation types.
 //
 // Work item: two query tiles of 128 rows ("halves" A and B) of one sequence and kv head, each
@@ -74,7 +72,6 @@ constexpr int kQDimHalf = kBM * 128;  // 16-bit tiles are [64 dims][rows][128 by
 constexpr int kDimHalf = kBN * 128;
 constexpr int kRing = 3;              // K tiles, V tiles
 constexpr int kRawRing = 2;
-constexpr float kZeroE = 60.f;
 constexpr int kFactors = 8;           // ring of the pages' factors
 constexpr int kItems = 4;             // ring of published items
 template <int D>
@@ -408,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         float sk, sv;
       };
       int n = 0;                                       // tiles published
-      float carry = 0.f;                               // least e of this item's last tile that had one
+      float carry = INFINITY;                          // least e of this item's last tile that had one
       int item = blockIdx.x, n_items = 0;              // items with tiles
       int j_next = 0, nt = 0, kv_beg = 0, npages = 0;  // of the item being looked up
       ItemLoads ahead;
@@ -473,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto publish = [&](const Group& gr) -> bool {
         const int s = gr.n % kItems;
         const int h = items[s].h, tiles = min(32 / kPages, items[s].ntiles - gr.j0);
-        if (gr.j0 == 0) carry = 0.f;
+        if (gr.j0 == 0) carry = INFINITY;              // none yet
         // ---- the factors of the lane's page
         const uint32_t nan = __ballot_sync(0xffffffffu, gr.sk != gr.sk || gr.sv != gr.sv);
         const bool plain = has_exponent(gr.sv);
@@ -485,7 +482,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (own != 0xffffffffu) {                      // the last tile, this one included, that has one
           const uint32_t upto = own & ((2u << (lane | (kPages - 1))) - 1u);
           const float last = __shfl_sync(0xffffffffu, least, upto != 0u ? 31 - __clz(upto) : 0);
-          if (!plain) e = fmaxf((upto != 0u ? last : carry) - kZeroE, kLeastE);
+          const float before = upto != 0u ? last : carry;
+          if (!plain) e = before == INFINITY ? 0.f : fmaxf(before - kZeroE, kLeastE);
         }
         if (own != 0u) carry = __shfl_sync(0xffffffffu, least, 31 - __clz(own));
         const float inv = exp2f(-e), f_log2 = fmaxf(gr.sk * p.scale_log2, 1e-37f);
@@ -733,7 +731,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         float mt = -INFINITY;
 #pragma unroll
         for (int g = 0; g < kPages; ++g) mt = fmaxf(mt, page_max(g));
-        if ((anew && mt > -INFINITY) || mt > m + 8.f) raise_to(mt);
+        if (anew && mt > -INFINITY)
+          raise_to(fmaxf(mt, m - kMostDown));
+        else if (mt > m + 8.f)
+          raise_to(mt);
         const float nb = m == -INFINITY ? 0.f : -m;
         if (!all_wait(&turn[x * 4 + quarter], (t & 1) ^ 1 ^ x)) return false;
 #pragma unroll

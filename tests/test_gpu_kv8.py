@@ -218,7 +218,8 @@ def test_gather_saturates_finite_values_to_fp16():
     assert bool((k32[0, 0] == 65536.0).all())
 
 
-def _check_attention(out, q, cache, tables, lens, counts, row_start, sm_scale, p_half, causal=True):
+def _check_attention(out, q, cache, tables, lens, counts, row_start, sm_scale, p_half, causal=True,
+                     more=0.0):
     out = out.cpu()
     for b, (t, n, c) in enumerate(zip(tables, lens, counts)):
         r = slice(row_start[b], row_start[b] + c)
@@ -226,7 +227,7 @@ def _check_attention(out, q, cache, tables, lens, counts, row_start, sm_scale, p
         qd = q[r].cpu().double().numpy()
         want = kv8.attention(qd, k, v, sm_scale, causal)
         vs = U.token_scales(cache[3], t, n, cache[0].shape[2])
-        bound = U.attention_bound(qd, k, v, vs, sm_scale, want, out.dtype, p_half, causal)
+        bound = U.attention_bound(qd, k, v, vs, sm_scale, want, out.dtype, p_half, causal) + more
         got = out[r].double().numpy()
         # an exact value that the bound takes past the type's largest one (fp16: 65504; from
         # 65520 on the nearest value is an infinity) may be the infinity of its sign
@@ -418,6 +419,42 @@ def test_scales_far_from_one(d, rows, idle, lo, hi):
     sm = 1 / math.sqrt(d)
     out = ops.paged_prefill_kv8(q, qo, rows, *cache, *plan, sm)
     _check_attention(out, q, cache, table, [n], [rows], [0], sm, _p_half(torch.bfloat16))
+
+
+@pytest.mark.parametrize("dt,d,rows,idle", _with_idle(
+    [(torch.bfloat16, 128, 1), (torch.float16, 128, 9), (torch.bfloat16, 64, 40), (torch.float16, 128, 90)],
+    lambda c: (c[0], 1, 8, 2, c[2], 16)))
+@pytest.mark.parametrize("seed", range(6))
+def test_zero_v_blocks_beside_large_scores(dt, d, rows, idle, seed):
+    """Scores up to some hundreds, the largest often on blocks of zeros in V: before the first
+    block that has values, between such blocks, and far above or below them.
+
+    On top of attention_bound: a weight that the kernels hold in fp16 is off by at most 2^-25
+    beside M. Where a block of zeros has set M, that is 2^-60 of the zeros' weight times the
+    scale of blocks before it, or 2^-90 of it before any: the row's sum is at least the zeros'
+    weight, so 2^-85 scale_v + 2^-115 times the sum of the codes."""
+    hq, hkv, n = 8, 2, 420
+    pages = -(-n // 16)
+    cache = U.random_cache(pages + 2, hkv, 16, d, DEV, 100 + seed)
+    table = U.page_lists([n], 16, pages + 2, 200 + seed)
+    g = torch.Generator().manual_seed(300 + seed)
+    at = torch.from_numpy(table[0]).long()
+    zero = torch.rand(pages, hkv, generator=g) < 0.4
+    zero[:seed] = True                              # leading ones
+    scale = torch.exp2(torch.randint(-12, 0, (pages, hkv), generator=g).float())
+    scale[zero] = 0.0
+    cache[3][at.to(DEV)] = scale.to(DEV)
+    cache[2][at.to(DEV)] = torch.exp2(torch.randint(-6, 0, (pages, hkv), generator=g).float()).to(DEV)
+    q = U.rows((rows, hq, d), dt, 400 + seed).to(DEV)
+    lens, tables = [n] + [0] * idle, table + [table[0][:0]] * idle
+    qo = torch.tensor([0] + [rows] * (1 + idle), dtype=torch.int32, device=DEV)
+    sm = 1 / math.sqrt(d)
+    out = ops.paged_prefill_kv8(q, qo, rows, *cache, *U.csr(tables, lens, 16, DEV), sm)
+    codes = U.values(cache[1], torch.ones_like(cache[3]), table[0], n)
+    sums = np.repeat(np.abs(codes).sum(0), hq // hkv, 0)[None]
+    most = np.repeat(scale.double().numpy().max(0), hq // hkv)[None, :, None]
+    _check_attention(out, q, cache, table, [n], [rows], [0], sm, _p_half(dt),
+                     more=(2.0 ** -85 * most + 2.0 ** -115) * sums)
 
 
 def test_v_blocks_of_the_smallest_scales():
