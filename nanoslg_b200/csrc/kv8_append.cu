@@ -15,9 +15,12 @@
 //   q_out = rot(q, p), rounded once to the activation type
 //
 // What bounds it: the bytes of the rows, read once, of q_out and of the codes, written once.
-// Measured (bf16, 32 / 8 heads of 128): prompts of 64 x 512 tokens 180 us, 5.2 TB/s, 0.80 of a
-// copy's rate; 16 x 128 behind 1024 20 to 28 us (37 MB; 7 at that rate); one token for each of
-// 64 sequences 3.0 us, most of it the launch and the chain plan, page, scale, codes.
+// Measured (bf16, 32 / 8 heads of 128): prompts of 64 x 512 tokens 180 us with the reading back
+// of what was written, 5.2 TB/s, 0.80 of a copy's rate; 16 x 128 behind 1024 alone 9.0 us
+// (46 MB: 7.0); one token for each of 64 sequences 3.0 us, most of it the launch and the chain
+// plan, page, scale, codes.
+#include <algorithm>
+
 #include "kv8.cuh"
 #include "launch.h"
 
@@ -399,14 +402,12 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8App
   }
 }
 
-// Reading back: one block per listed page, [page_size, hkv, d] values of type T in list
-// order; slots behind the sequence's last token are zeros. Rows of pages behind the last
+// Reading back: the listed pages as [page_size, hkv, d] values of type T in list order; slots behind the sequence's last token are zeros. Rows of pages behind the last
 // listed one are left as they are. A thread takes 16 codes of one head row: 16-byte loads,
 // 16-byte stores, consecutive threads along the output. Bound by its bytes (one read and two
 // or four written per element): 16 sequences of 1152 tokens (8 heads of 128, bf16) 24.4 us,
-// 4.6 TB/s, 2 of it the launch; 1, 2 or 4 chunks a thread at a time take the same within 5 %.
+// 4.6 TB/s, 2 of it the launch; 1, 2 or 4 chunks a thread at a time take the same within 7 %.
 constexpr int kGatherThreads = 256;
-constexpr int kBatch = 2;            // chunks a thread holds at a time
 
 template <typename T>
 __device__ __forceinline__ void store16(T* dst, const uint4& c, float sc) {
@@ -424,7 +425,8 @@ __device__ __forceinline__ void store16(T* dst, const uint4& c, float sc) {
     *reinterpret_cast<uint4*>(dst + i) = *reinterpret_cast<const uint4*>(v + i);
 }
 
-template <typename T>
+// kBatch: chunks a thread holds at a time.
+template <typename T, int kBatch>
 __global__ void __launch_bounds__(kGatherThreads) kv8_gather_kernel(const Kv8GatherParams p) {
   pdl_wait();
   pdl_trigger();
@@ -442,7 +444,8 @@ __global__ void __launch_bounds__(kGatherThreads) kv8_gather_kernel(const Kv8Gat
   const int chunks = p.d / 16, per_slot = p.hkv * chunks, n = p.page_size * per_slot;
   const int64_t blk0 = page * p.hkv;
   bool synced = false;
-  for (int i0 = tid; i0 - tid < n; i0 += kBatch * kGatherThreads) {
+  const int step = kBatch * kGatherThreads * static_cast<int>(gridDim.y);
+  for (int i0 = blockIdx.y * kBatch * kGatherThreads + tid; i0 - tid < n; i0 += step) {
     uint4 ck[kBatch], cv[kBatch];
     float sk[kBatch], sv[kBatch];
     int slot[kBatch];
@@ -517,13 +520,32 @@ int launch_kv8_append(int dtype, const Kv8AppendParams& p, cudaStream_t stream) 
   return launch_pdl("kv8_append", kv8_append_kernel<float>, grid, block, 0, stream, p);
 }
 
+namespace {
+
+// A page is shared by several blocks where the list is short (up to about 8 blocks an SM), down to
+// a chunk a thread for lists of fewer pages than SMs. Us for 19 / 144 / 300 / 1184 pages of 8
+// heads of 128: a block a page 4.4 / 5.1 / 9.3 / 25.5; shared, two chunks a thread 3.2 / 5.1 /
+// 9.9 / 25.5; one chunk 2.6 / 4.9 / 11.2 / 27.4.
+template <typename T, int kBatch>
+int launch_gather(const Kv8GatherParams& p, cudaStream_t stream) {
+  const int64_t chunks = static_cast<int64_t>(p.page_size) * p.hkv * (p.d / 16);
+  const int64_t most = std::min<int64_t>((chunks + kBatch * kGatherThreads - 1) / (kBatch * kGatherThreads), 65535);
+  const int64_t parts = std::max<int64_t>(std::min(8ll * sm_count() / p.num_indices, static_cast<long long>(most)), 1);
+  const dim3 grid(static_cast<unsigned>(p.num_indices), static_cast<unsigned>(parts));
+  return launch_pdl("kv8_gather", kv8_gather_kernel<T, kBatch>, grid, dim3(kGatherThreads), 0, stream, p);
+}
+
+template <typename T>
+int launch_gather_typed(const Kv8GatherParams& p, cudaStream_t stream) {
+  return p.num_indices < sm_count() ? launch_gather<T, 1>(p, stream) : launch_gather<T, 2>(p, stream);
+}
+
+}  // namespace
+
 int launch_kv8_gather(int dtype, const Kv8GatherParams& p, cudaStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(p.num_indices)), block(kGatherThreads);
-  if (dtype == NSLG_DTYPE_BF16)
-    return launch_pdl("kv8_gather", kv8_gather_kernel<__nv_bfloat16>, grid, block, 0, stream, p);
-  if (dtype == NSLG_DTYPE_F16)
-    return launch_pdl("kv8_gather", kv8_gather_kernel<__half>, grid, block, 0, stream, p);
-  return launch_pdl("kv8_gather", kv8_gather_kernel<float>, grid, block, 0, stream, p);
+  if (dtype == NSLG_DTYPE_BF16) return launch_gather_typed<__nv_bfloat16>(p, stream);
+  if (dtype == NSLG_DTYPE_F16) return launch_gather_typed<__half>(p, stream);
+  return launch_gather_typed<float>(p, stream);
 }
 
 }  // namespace nslg
