@@ -6,18 +6,18 @@
 // rows and 64 positions at head_dim 128), so everything else has to stay off the softmax
 // warps. Measured (bf16, 32 / 8 heads of 128): prompts of 64 x 512 tokens 226 us, 16 suffixes
 // of 128 behind 1024 57 us (640 TFLOP/s): 1.1 to 1.2 us for such a tile, the chain of one half's
-// scores, maximum, exponentials and weights, and 2 us at an item's end. The codes are therefore not dequantised: they are
-// only widened, which is exact (K to q's type, V to f16), and the blocks' scales join the
-// exponent, where they cost nothing per element:
+// scores, maximum, exponentials and weights, and 2 us at an item's end.
+//
+// The codes are not dequantised: they are only widened, which is exact (K to q's type, V to
+// f16), and the blocks' scales join the exponent, where they cost nothing per element:
 //   t_j = s_j F_g + E_g      s = q . code_k, F = scale_k sm_scale log2(e), E = log2 scale_v,
 //                            g = j's page (16 positions share F and E)
 //   p_j = 2^(t_j - M)        M: running maximum of t, raised when passed by 8
 //   o   = sum_j p_j code_v[j];  l = sum_g 2^-E_g sum_{j in g} p_j;  out = o / l
-// so p is what multiplies the code in the f16 product, M follows the largest of these
-// weights, and no ratio of scales between pages can underflow what matters (blocks of zeros in
-// V, which have no E, stand at kZeroE). F > 0 makes the maximum of t over a page a function of
-// the maximum of s. p is f16 (2^-11) for both
-// activation types.
+// so p is what multiplies the code in the f16 product, M follows the largest of these weights,
+// and no ratio of scales between pages can underflow what matters (blocks of zeros in V, which
+// have no E, stand at kZeroE). F > 0 makes the maximum of t over a page a function of the
+// maximum of s. p is f16 (2^-11) for both activation types.
 //
 // Work item: two query tiles of 128 rows ("halves" A and B) of one sequence and kv head, each
 // 128 / G new tokens times the G query heads that share the kv head; both read the same K and
@@ -45,9 +45,8 @@
 // TMEM per half: two S (and P over it) of 64 + O 128 columns; 512 in all.
 //
 // A block whose scale is NaN (K's or V's) gives NaN to the rows that see it: their scores of
-// the page are set to NaN. Every mbarrier wait is bounded; on a timeout
-// the kernel records NSLG_DEV_WAIT_TIMEOUT, waits (bounded) for what it issued, frees its
-// TMEM and returns.
+// the page are set to NaN. Every mbarrier wait is bounded; on a timeout the kernel records
+// NSLG_DEV_WAIT_TIMEOUT, waits (bounded) for what it issued, frees its TMEM and returns.
 #include <cuda.h>
 
 #include <string>
