@@ -69,7 +69,8 @@ def _attend(lib, dtype=N.DTYPE_BF16, batch=1, hq=8, hkv=2, d=128, ps=16, q=16, q
     (dict(ps=0), b"page_size"), (dict(pages=0), b"num_pages"), (dict(pool=0), b"null cache"),
     (dict(scale=0), b"null cache"), (dict(plan=0), b"page list"), (dict(pool=24), b"aligned"),
     (dict(q=0), b"null"), (dict(out=0), b"null"), (dict(q=18), b"aligned"), (dict(qs=1020), b"stride"),
-    (dict(qs=512), b"stride"), (dict(sm=0.0), b"sm_scale"), (dict(sm=math.nan), b"sm_scale")])
+    (dict(qs=512), b"stride"), (dict(sm=0.0), b"sm_scale"), (dict(sm=math.nan), b"sm_scale"),
+    (dict(ps=65536, hq=256, hkv=256, qs=32768), b"2^31 elements"), (dict(ps=65537), b"page_size")])
 def test_attention_refusals(lib, bad, what):
     assert _attend(lib, **bad) in (N.ERR_ARG, N.ERR_UNSUPPORTED)
     assert what in lib.nslg_last_error()
