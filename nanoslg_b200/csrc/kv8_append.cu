@@ -295,8 +295,9 @@ __global__ void __launch_bounds__(512) kv8_append_token_kernel(const Kv8AppendPa
           *w = make_uint4(rescale4(x.x, ratio, nan), rescale4(x.y, ratio, nan),
                           rescale4(x.z, ratio, nan), rescale4(x.w, ratio, nan));
         }
-        if (c == 0) *sc = now;
       }
+      // a page that starts here takes its scale even where that is 0: its last owner's is in memory
+      if (c == 0 && (slot == 0 || !(now == was))) *sc = now;
       store_codes<D>(codes + slot * D, c, v, now);
     }
   }

@@ -148,6 +148,32 @@ def test_append_zeros_and_values_that_are_not_finite(n):
         assert bool(torch.isfinite(cache[3][1]).all())
 
 
+@pytest.mark.parametrize("dt,d,ps", [(torch.bfloat16, 128, 16), (torch.float16, 64, 16), (torch.float32, 64, 16),
+                                     (torch.bfloat16, 96, 5)])
+@pytest.mark.parametrize("first", [1, 3])
+@pytest.mark.parametrize("stale", [math.nan, 2.0 ** 20])
+def test_a_page_begun_with_zeros_forgets_its_last_owner(dt, d, ps, first, stale):
+    """Head rows of zeros in the first slots of a page whose scales are left over, alone in their
+    call and together; then small tokens one by one."""
+    hkv, page = 2, 3
+    cache = U.random_cache(5, hkv, ps, d, DEV, 7)
+    cache[2].fill_(stale)
+    cache[3].fill_(stale)
+    oracle = kv8.Cache(5, hkv, ps, d)
+    table = [np.array([page], np.int32)]
+    start = 0
+    for count in (first, 1, 1):
+        k = torch.zeros(count, hkv, d, dtype=dt) if start == 0 else U.rows((count, hkv, d), dt, start) / 16
+        v = k.clone()
+        k[:, 1] = U.rows((count, d), dt, 9)                  # the other kv head has values from the start
+        ptr, idx, lpl = U.csr(table, [start + count], ps, DEV)
+        qo = torch.tensor([0, count], dtype=torch.int32, device=DEV)
+        ops.rope_kv8_append(None, k.to(DEV), v.to(DEV), None, None, *cache, qo, count, ptr, idx, lpl, rotate=False)
+        oracle.append(table[0], start, k.float().numpy(), v.float().numpy())
+        start += count
+        _assert_cache(cache, oracle, table, [start])
+
+
 def test_append_bad_plans_are_reported_and_skipped():
     hkv, d = 2, 64
     cache = U.random_cache(8, hkv, 16, d, DEV, 5)

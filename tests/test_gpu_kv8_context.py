@@ -119,6 +119,41 @@ def test_pages_handed_out_again_start_clean():
         mgr.release_sequence("s")
 
 
+@pytest.mark.parametrize("rope", [True, False])
+def test_a_decode_step_begins_a_page_handed_out_again(rope):
+    """A step planned on the device opens a page whose blocks its last owner left NaN, with rows
+    of zeros; the next step adds a small token."""
+    hq, hkv, d, dt = 8, 2, 64, torch.bfloat16
+    mgr = _manager(hq, hkv, d, dt, 3)
+    cos, sin = (t.to(DEV) for t in rope_table(d, 64, 10000.0))
+
+    def forward(n, make):
+        ctx = mgr.begin_forward(["s"], [n])
+        q, k, v = (make((1, n, h, d), h) for h in (hq, hkv, hkv))
+        out = ctx.attend_rope(0, q, k, v, cos, sin) if rope else ctx.attend(0, q, k, v, hq, hkv)
+        mgr.end_forward(ctx)
+        return out
+
+    def values(shape, seed):
+        return U.rows(shape, dt, seed).to(DEV)
+
+    mgr.allocate_sequence("s", num_tokens=20)
+    forward(20, lambda shape, seed: torch.full(shape, math.nan, dtype=dt, device=DEV))
+    assert bool(torch.isnan(mgr.pool.k_scale[0, 1:]).all())
+    mgr.release_sequence("s")
+    mgr.allocate_sequence("s", num_tokens=16)
+    forward(16, values)
+    out = forward(1, lambda shape, seed: torch.zeros(shape, dtype=dt, device=DEV))
+    page = mgr.seqs["s"].block_table[1]
+    assert bool(torch.isfinite(out).all())
+    for t in (mgr.pool.k_scale, mgr.pool.v_scale):
+        assert bool((t[0, page] == 0).all())
+    out = forward(1, lambda shape, seed: values(shape, seed) / 64)
+    assert bool(torch.isfinite(out).all())
+    for t in (mgr.pool.k_scale, mgr.pool.v_scale):
+        assert bool((t[0, page] > 0).all()) and bool((t[0, page] < 2.0 ** -8).all())
+
+
 def test_a_sequence_twice_in_a_forward_is_refused():
     mgr = _manager(8, 2, 64, torch.bfloat16, 10)
     mgr.allocate_sequence("s", num_tokens=3)
