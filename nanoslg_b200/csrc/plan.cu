@@ -23,6 +23,10 @@
 // zero: a decode step's steady state) skips the staging too: the arrays travel in the
 // launch's parameters, and the kernel reads no host memory (each dependent read of the
 // mapped staging is a PCIe round trip: 23 us per step on B200 for the C2 batch of 64).
+//
+// No kernel here lets its dependents launch early: paged_decode reads the page list before
+// it waits for the kernel in front of it, so the list has to be written, and visible on
+// the whole GPU, before the planner's last block ends.
 #include <cstring>
 #include <mutex>
 #include <string>
@@ -132,6 +136,7 @@ __global__ void __launch_bounds__(128) plan_decode_gather_kernel(const PlanParam
   }
   const int32_t* row = p.bt + s * p.bt_stride;
   for (int j = threadIdx.x; j < end - beg; j += blockDim.x) p.indices[beg + j] = row[j];
+  __threadfence();
 }
 
 // Zeroes `pages` of one or two pool tensors [layers, pages_total, page elements]: block
@@ -193,7 +198,6 @@ __global__ void __launch_bounds__(kFusedThreads) plan_decode_fused_kernel(
   // launched with programmatic dependent launch: nothing is read or written before the
   // previous kernel on the stream (which may still read the plan being replaced) is done
   pdl_wait();
-  pdl_trigger();
   const int t = threadIdx.x;
   const int32_t* slots = use_inline ? in.slots : p.slots;
   const int32_t* starts = use_inline ? in.starts : p.starts;
@@ -258,6 +262,7 @@ __global__ void __launch_bounds__(kFusedThreads) plan_decode_fused_kernel(
   if (!fits) return;
   const int32_t* row = p.bt + s * p.bt_stride;
   for (int j = t; j < n; j += kFusedThreads) p.indices[run + j] = row[j];
+  __threadfence();
 }
 
 // Split-heads plan: sequence b' = b * hkv + h of the split-heads decode is kv head h of
@@ -269,7 +274,6 @@ __global__ void __launch_bounds__(128) split_heads_plan_kernel(
     const int32_t* kv_lpl, int32_t* v_indptr, int32_t* v_indices, int32_t* v_lpl,
     int64_t max_v, uint32_t* status) {
   pdl_wait();
-  pdl_trigger();
   const int bv = blockIdx.x, b = bv / hkv, h = bv % hkv;
   const int beg = kv_indptr[b], n = kv_indptr[b + 1] - beg;
   const int64_t vbeg = static_cast<int64_t>(hkv) * beg + static_cast<int64_t>(h) * n;
@@ -284,6 +288,7 @@ __global__ void __launch_bounds__(128) split_heads_plan_kernel(
   }
   for (int j = threadIdx.x; j < n; j += blockDim.x)
     v_indices[vbeg + j] = kv_indices[beg + j] * hkv + h;
+  __threadfence();
 }
 
 int check_plan_args(int batch, int page_size, int64_t bt_stride, int64_t bt_rows,

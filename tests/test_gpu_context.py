@@ -381,6 +381,51 @@ def test_plan_decode_device_arrays_match_host_arrays(batch):
     assert outs[1][0].numpy().tolist() == want.tolist()
 
 
+@pytest.mark.parametrize("op", ["paged_decode", "split_heads"])
+def test_a_decode_directly_behind_its_plan(op):
+    """nslg_plan_decode_host and the decode with nothing between them, over and over into one
+    plan buffer, short and long sequences in turn: every step's output is the one of a step
+    that waited for its plan."""
+    import numpy as np
+    from nanoslg_b200 import _native as N
+    dev = torch.device("cuda:0")
+    B, ps, hq, hkv, d, stride = 48, 16, 16, 4, 128, 64
+    pages = B * stride + 1
+    g = torch.Generator(device=dev).manual_seed(3)
+    q = torch.randn(B, hq, d, device=dev, generator=g).bfloat16()
+    k, v = (torch.randn(pages, ps, hkv, d, device=dev, generator=g).bfloat16() for _ in range(2))
+    rng = np.random.default_rng(3)
+    bt = torch.from_numpy((rng.permutation(pages - 1)[:B * stride] + 1).reshape(B, stride).astype(np.int32)).to(dev)
+    slots = np.arange(B, dtype=np.int32)
+    starts = [rng.integers(0, 40, B).astype(np.int32), rng.integers(600, 1000, B).astype(np.int32),
+              rng.integers(0, 1000, B).astype(np.int32)]
+    plan = torch.zeros(6 * B + 2 + B * stride, dtype=torch.int32, device=dev)
+    indptr, lpl = plan[2 * B:3 * B + 1], plan[3 * B + 1:4 * B + 1]
+    indices = plan[6 * B + 2:]
+
+    def step(st, wait):
+        N.call("nslg_plan_decode_host", B, ps, slots.ctypes.data, st.ctypes.data, 0, None, 0, None, None, None,
+               1, pages, 16, bt.data_ptr(), stride, B, plan.data_ptr(), B * stride,
+               ops.status_word(dev).data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
+        if wait:
+            torch.cuda.synchronize(dev)
+        if op == "paged_decode":
+            return ops.paged_decode(q, k, v, indptr, indices, lpl, 0.09)
+        split = ops.split_heads_plan(indptr, indices, lpl, hkv, pages)
+        if wait:
+            torch.cuda.synchronize(dev)
+        return ops.paged_decode_split_heads(q, k, v, split, 0.09)
+
+    want = [step(st, True) for st in starts]
+    assert not torch.equal(want[0], want[1])
+    torch.cuda.synchronize(dev)
+    got = [step(starts[i % 3], False) for i in range(120)]
+    torch.cuda.synchronize(dev)
+    for i, o in enumerate(got):
+        assert torch.equal(o, want[i % 3]), i
+    ops.check_device_status(dev)
+
+
 def test_zero_pages_entry_point():
     """nslg_zero_pages zeroes exactly the listed pages of every layer of one pool."""
     from nanoslg_b200 import _native as N
