@@ -430,8 +430,9 @@ int64_t nslg_decode_kv8_workspace_bytes(int batch, int num_qo_heads, int num_kv_
 
 /* nslg_paged_decode over the 8-bit cache: one query row per sequence, the same sequence and
  * head conventions, zeros for a sequence without pages. Launched with programmatic dependent
- * launch under the rule given there (the CSR arrays may be read before the kernel before it
- * on the stream has finished). */
+ * launch, but unlike nslg_paged_decode it reads nothing, the CSR arrays included, before the
+ * kernel in front of it has finished: any work on the stream may write them. The same holds
+ * for the other calls of the 8-bit cache. */
 int nslg_paged_decode_kv8(int dtype, int batch, int num_qo_heads, int num_kv_heads, int head_dim,
                           int page_size, const void* q, int64_t q_stride, void* out,
                           int64_t out_stride, const void* codes_k, const void* codes_v,

@@ -250,6 +250,13 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
       heads + static_cast<size_t>(kWarps) * piece_floats);
   uint64_t* full = bars + warp * stages;
 
+  if (lane < stages) mbar_init(&full[lane], 1);
+  fence_barrier_init();
+  if (threadIdx.x < 2 * kWarps) s_vid[threadIdx.x] = -1;
+  // the kernel before may have written anything this one reads, the page list too
+  pdl_wait();
+  pdl_trigger();
+
   const int32_t* indptr = p.kv_indptr;
   const int32_t* lpl = p.kv_lpl;
   if (p.smem_csr) {
@@ -260,9 +267,6 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
     indptr = s_ip;
     lpl = s_lpl;
   }
-  if (lane < stages) mbar_init(&full[lane], 1);
-  fence_barrier_init();
-  if (threadIdx.x < 2 * kWarps) s_vid[threadIdx.x] = -1;
   __syncthreads();
 
   const int hm = p.hkv * p.tiles;        // virtual sequences per sequence
@@ -272,8 +276,6 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
   const int n = min((total + kWarps - 1) / kWarps, p.grid);
   const int c = blockIdx.x;
   if (c >= n) {
-    pdl_wait();
-    pdl_trigger();
     if (!fits && threadIdx.x == 0) report(p.status, NSLG_DEV_BAD_PLAN);
     zero_empty<T, kThreads>(p, indptr);
     return;
@@ -299,7 +301,7 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
     vid = b * hm + vs;
     return loc - vs * np;
   };
-  auto look_up = [&](int i, Meta& m) {    // page list only: may run before the PDL wait
+  auto look_up = [&](int i, Meta& m) {
     m.blk = -1;
     m.vid = -1;
     m.j = 0;
@@ -336,8 +338,6 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
 
   Meta cur, nxt;
   look_up(lane, nxt);
-  pdl_wait();      // the kernel before may have written q, the codes and the scales
-  pdl_trigger();
   load_scales(nxt);   // before the bulk loads, which would queue in front of them
   if (lane < stages && lane < units) issue(nxt, lane);
   zero_empty<T, kThreads>(p, indptr);

@@ -176,7 +176,12 @@ def rope_kv_append(q, k, v, positions, cos, sin, write_loc, pool_k, pool_v, q_ou
 
 def paged_decode(q, pool_k, pool_v, kv_indptr, kv_indices, kv_last_page_len, sm_scale,
                  out=None):
-    """Decode attention, one query per sequence. q: [B, Hq, D] -> out [B, Hq, D]."""
+    """Decode attention, one query per sequence. q: [B, Hq, D] -> out [B, Hq, D].
+
+    The kernel may read the page list (kv_indptr, kv_indices, kv_last_page_len) while the
+    kernel in front of it on the stream is still running, where that one lets its dependents
+    start early (the append, RMSNorm, SwiGLU and linear kernels of this library): write the
+    list before that kernel. Directly behind the planner's kernels the call is safe."""
     _need_cuda(q, pool_k, pool_v, kv_indptr, kv_indices, kv_last_page_len)
     dt = _dtype_code(q)
     nb, qs = _rows(q, "q")
@@ -466,7 +471,8 @@ def argmax_rows(x, index_offset=0, values=False):
 # ---------------------------------------------------------------- 8-bit KV cache
 # One layer of the cache: e4m3 codes [num_pages, Hkv, page_size, D] and a fp32 scale per
 # (page, kv head) for K and for V (kv8_pages allocates them); value = code * scale. The
-# checks, outputs, scratch and streams of these ops are csrc/kv8_torch.cpp.
+# checks, outputs, scratch and streams of these ops are csrc/kv8_torch.cpp. All of them are
+# ordered behind everything in front of them on the stream, the page list's writers too.
 KV8_DTYPE = torch.float8_e4m3fn
 
 

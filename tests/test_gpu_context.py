@@ -381,7 +381,7 @@ def test_plan_decode_device_arrays_match_host_arrays(batch):
     assert outs[1][0].numpy().tolist() == want.tolist()
 
 
-@pytest.mark.parametrize("op", ["paged_decode", "split_heads"])
+@pytest.mark.parametrize("op", ["paged_decode", "split_heads", "kv8"])
 def test_a_decode_directly_behind_its_plan(op):
     """nslg_plan_decode_host and the decode with nothing between them, over and over into one
     plan buffer, short and long sequences in turn: every step's output is the one of a step
@@ -394,6 +394,9 @@ def test_a_decode_directly_behind_its_plan(op):
     g = torch.Generator(device=dev).manual_seed(3)
     q = torch.randn(B, hq, d, device=dev, generator=g).bfloat16()
     k, v = (torch.randn(pages, ps, hkv, d, device=dev, generator=g).bfloat16() for _ in range(2))
+    if op == "kv8":
+        k, v = (t.transpose(1, 2).contiguous().to(torch.float8_e4m3fn) for t in (k, v))
+        scale = torch.ones(pages, hkv, device=dev)
     rng = np.random.default_rng(3)
     bt = torch.from_numpy((rng.permutation(pages - 1)[:B * stride] + 1).reshape(B, stride).astype(np.int32)).to(dev)
     slots = np.arange(B, dtype=np.int32)
@@ -409,6 +412,8 @@ def test_a_decode_directly_behind_its_plan(op):
                ops.status_word(dev).data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
         if wait:
             torch.cuda.synchronize(dev)
+        if op == "kv8":
+            return ops.paged_decode_kv8(q, k, v, scale, scale, indptr, indices, lpl, 0.09)
         if op == "paged_decode":
             return ops.paged_decode(q, k, v, indptr, indices, lpl, 0.09)
         split = ops.split_heads_plan(indptr, indices, lpl, hkv, pages)

@@ -201,6 +201,59 @@ def test_graphs_and_streams_do_not_share_scratch():
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("behind", ["copy", "rmsnorm"])
+@pytest.mark.parametrize("rows", [1, 6, 200])
+def test_attention_directly_behind_the_work_that_writes_its_list(rows, behind, graph):
+    """The page list and the scales are copied into place right before the call, or right before
+    a kernel that lets its dependents start early: every route of decode and prefill takes the
+    list that was written last, eager and replayed."""
+    hq, hkv, d, dt = 8, 2, 128, torch.bfloat16
+    lens = [[900, 40, 700, 260], [230, 1000, 201, 800]]
+    tables = [U.page_lists([1024] * 4, 16, 300, 7 + i) for i in range(2)]
+    cache = U.random_cache(300, hkv, 16, d, DEV, 8)
+    lists = []
+    for ln, tab in zip(lens, tables):
+        ln = [max(n, rows) for n in ln]
+        lists.append(U.csr([t[:-(-n // 16)] for t, n in zip(tab, ln)], ln, 16, DEV))
+    room = max(x[1].numel() for x in lists)
+    now = [torch.zeros_like(lists[0][0]), torch.zeros(room, dtype=torch.int32, device=DEV),
+           torch.ones_like(lists[0][2])]
+    q = U.rows((4 * rows, hq, d), dt, 11).to(DEV)
+    qo = torch.arange(5, dtype=torch.int32, device=DEV) * rows
+    x, w = torch.ones(64, 4096, dtype=dt, device=DEV), torch.ones(4096, dtype=dt, device=DEV)
+
+    def call(src):
+        for a, b in zip(now, src):
+            torch.add(b, 0, out=a[:b.numel()])
+        if behind == "rmsnorm":
+            ops.rmsnorm_residual(x, w, 1e-5)
+        if rows == 1:
+            return ops.paged_decode_kv8(q, *cache, *now, 0.09)
+        return ops.paged_prefill_kv8(q, qo, rows, *cache, *now, 0.09)
+
+    def alone(src):
+        torch.cuda.synchronize()
+        if rows == 1:
+            return ops.paged_decode_kv8(q, *cache, *src, 0.09)
+        return ops.paged_prefill_kv8(q, qo, rows, *cache, *src, 0.09)
+    want = [alone(src) for src in lists]
+    assert not torch.equal(*want)
+    call(lists[0])
+    torch.cuda.synchronize()
+    if graph:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = [call(lists[i % 2]) for i in range(20)]
+        for _ in range(3):
+            g.replay()
+    else:
+        got = [call(lists[i % 2]) for i in range(60)]
+    torch.cuda.synchronize()
+    for i, o in enumerate(got):
+        assert torch.equal(o, want[i % 2]), i
+
+
 def test_append_and_attention_in_a_graph_follow_the_plan():
     """A captured append + decode replayed over plans written into the same buffers."""
     hq, hkv, d, dt = 16, 4, 128, torch.bfloat16
