@@ -374,7 +374,8 @@ int nslg_plan_decode_host(int batch, int page_size, const int32_t* slots, const 
  * least 2^-126, NaN for a block that holds a value that is not finite: all of that block
  * then reads as NaN). The readers take any scale that is finite and not negative, and NaN (on
  * the tensor cores a V block of a scale below 2^-100 counts as zeros). Page lists are the CSR
- * of the other entry points; page 0 needs no special contents, and a page that is handed out
+ * of the other entry points; kv_indptr may be a part of a longer batch's (kv_indptr[0] > 0,
+ * kv_indices the whole list). Page 0 needs no special contents, and a page that is handed out
  * again needs no clearing. head_dim is a multiple of 32 up to 256, a page of one layer has
  * fewer than 2^31 elements; page_size 16 with head_dim 64 or 128 and 16-bit activations runs
  * on the tensor cores, the rest on CUDA cores. Pointers are 16-byte aligned (scales 4), row
@@ -411,9 +412,10 @@ int nslg_rope_kv8_append(int dtype, int batch, int num_qo_heads, int num_kv_head
                          uint32_t* dev_status, void* stream);
 
 /* Pages read back as values of the activation type `dtype`: out_k and out_v are
- * [num_indices, page_size, num_kv_heads, head_dim], page j of the list (j < kv_indptr[batch]
- * <= num_indices) at out[j]; slots behind a sequence's last token and pages outside the pool
- * (NSLG_DEV_BAD_PAGE) read as zeros, the pages of out behind the list are left as they are.
+ * [num_indices, page_size, num_kv_heads, head_dim], page j of the list (kv_indptr[0] <= j <
+ * kv_indptr[batch] <= num_indices) at out[j]; slots behind a sequence's last token and pages
+ * outside the pool (NSLG_DEV_BAD_PAGE) read as zeros, the pages of out of no sequence are left
+ * as they are.
  * A finite value beyond fp16's range reads as +-65504 there. */
 int nslg_kv8_gather(int dtype, int batch, int num_kv_heads, int head_dim, int page_size,
                     const void* codes_k, const void* codes_v, const float* scale_k,

@@ -403,8 +403,8 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8App
   }
 }
 
-// Reading back: the listed pages as [page_size, hkv, d] values of type T in list order; slots behind the sequence's last token are zeros. Rows of pages behind the last
-// listed one are left as they are. A thread takes 16 codes of one head row: 16-byte loads,
+// Reading back: the listed pages as [page_size, hkv, d] values of type T in list order; slots
+// behind the sequence's last token are zeros. Rows of list entries of no sequence are left as they are. A thread takes 16 codes of one head row: 16-byte loads,
 // 16-byte stores, consecutive threads along the output. Bound by its bytes (one read and two
 // or four written per element): 16 sequences of 1152 tokens (8 heads of 128, bf16) 24.4 us,
 // 4.6 TB/s, 2 of it the launch; 1, 2 or 4 chunks a thread at a time take the same within 7 %.
@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(kGatherThreads) kv8_gather_kernel(const Kv8Gat
   __shared__ int s_fill;
   const int64_t j = blockIdx.x;
   const int tid = threadIdx.x;
-  if (j >= p.kv_indptr[p.batch]) return;
+  if (j < p.kv_indptr[0] || j >= p.kv_indptr[p.batch]) return;
   const int64_t page = p.kv_indices[j];
   for (int b = tid; b < p.batch; b += kGatherThreads) {
     const int lo = p.kv_indptr[b], hi = p.kv_indptr[b + 1];

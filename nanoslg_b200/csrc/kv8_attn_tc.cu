@@ -270,9 +270,11 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
   __syncthreads();
 
   const int hm = p.hkv * p.tiles;        // virtual sequences per sequence
-  const int64_t all = static_cast<int64_t>(indptr[p.batch]) * hm;
-  const bool fits = all >= 0 && all < (int64_t{1} << 31) - kWarps;
-  const int total = fits ? static_cast<int>(all) : 0;
+  // units are numbered from the list's first entry on, which may be one of a longer list
+  const int64_t from = static_cast<int64_t>(indptr[0]) * hm, to = static_cast<int64_t>(indptr[p.batch]) * hm;
+  const bool fits = from >= 0 && to >= from && to < (int64_t{1} << 31) - kWarps;
+  const int ufirst = fits ? static_cast<int>(from) : 0;
+  const int total = fits ? static_cast<int>(to - from) : 0;
   const int n = min((total + kWarps - 1) / kWarps, p.grid);
   const int c = blockIdx.x;
   if (c >= n) {
@@ -281,7 +283,7 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
     return;
   }
   const Split ctas(total, n);
-  const int u0 = ctas.begin(c), u1 = ctas.begin(c + 1);
+  const int u0 = ufirst + ctas.begin(c), u1 = ufirst + ctas.begin(c + 1);
   const Split parts(u1 - u0, kWarps);
   const int ua = u0 + parts.begin(warp), ub = u0 + parts.begin(warp + 1);
   const int units = ub - ua;
@@ -463,8 +465,8 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
     int beg, end;
     segment(jn.vid, beg, end);
     if (warp == 0 ? beg < u0 : (beg >= u0 && end > u1)) {
-      jn.cf = ctas.part_of(beg);
-      jn.cnt = ctas.part_of(end - 1) - jn.cf + 1;
+      jn.cf = ctas.part_of(beg - ufirst);
+      jn.cnt = ctas.part_of(end - 1 - ufirst) - jn.cf + 1;
       jn.to = group_of(jn.vid);
     } else {
       jn.vid = -1;

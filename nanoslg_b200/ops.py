@@ -473,6 +473,7 @@ def argmax_rows(x, index_offset=0, values=False):
 # (page, kv head) for K and for V (kv8_pages allocates them); value = code * scale. The
 # checks, outputs, scratch and streams of these ops are csrc/kv8_torch.cpp. All of them are
 # ordered behind everything in front of them on the stream, the page list's writers too.
+# kv_indptr and kv_last_page_len may be slices of a longer batch's, over its whole kv_indices.
 KV8_DTYPE = torch.float8_e4m3fn
 
 
@@ -509,7 +510,7 @@ def kv8_gather(pool_k, pool_v, scale_k, scale_v, kv_indptr, kv_indices, kv_last_
                out=None):
     """The listed pages read back as values: (k, v), each [kv_indices.numel(), page_size,
     Hkv, D] of ``dtype``, page j of the list at row j, zeros behind a sequence's last token.
-    Rows behind the list (kv_indptr[-1]) are left as they are."""
+    Rows of no sequence (before kv_indptr[0], from kv_indptr[-1] on) are left as they are."""
     k, v = (None, None) if out is None else out
     return N.kv8().gather(pool_k, pool_v, scale_k, scale_v, kv_indptr, kv_indices,
                           kv_last_page_len, dtype, k, v)

@@ -615,6 +615,41 @@ def test_max_qo_len_beyond_the_rows():
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
 
 
+@pytest.mark.parametrize("dt,hq,hkv,d,ps", [(torch.bfloat16, 32, 8, 128, 16), (torch.float16, 6, 2, 64, 16),
+                                            (torch.float32, 4, 2, 64, 16), (torch.bfloat16, 6, 3, 96, 5)])
+@pytest.mark.parametrize("first,last", [(2, 6), (5, 6), (0, 3), (3, 3)])
+def test_a_part_of_a_longer_batch(dt, hq, hkv, d, ps, first, last):
+    """Bounds sliced out of a batch of seven, over its whole list: the results of the sequences'
+    own list."""
+    lens, counts = [60, 900, 33, 0, 700, 18, 45], [7, 5, 1, 0, 6, 2, 3]
+    pages = sum(-(-n // ps) for n in lens) + 1
+    tables = U.page_lists(lens, ps, pages, 61)
+    caches = [U.random_cache(pages, hkv, ps, d, DEV, 62) for _ in range(2)]
+    ptr, idx, lpl = U.csr(tables, lens, ps, DEV)
+    part = (ptr[first:last + 1], idx, lpl[first:last])
+    own = U.csr(tables[first:last], lens[first:last], ps, DEV)
+    q = U.rows((sum(counts), hq, d), dt, 63).to(DEV)
+    k = U.rows((sum(counts), hkv, d), dt, 64).to(DEV)
+    qo = torch.tensor(np.cumsum([0] + counts), dtype=torch.int32, device=DEV)[first:last + 1]
+    r0, r1 = int(sum(counts[:first])), int(sum(counts[:last]))
+    got = []
+    for cache, plan in zip(caches, (part, own)):
+        ops.rope_kv8_append(None, k, -k, None, None, *cache, qo, 7, *plan, rotate=False)
+        out = torch.full_like(q, 3.0)
+        ops.paged_prefill_kv8(q, qo, 7, *cache, *plan, 0.1, out=out)
+        dec = ops.paged_decode_kv8(q[:last - first], *cache, *plan, 0.1)
+        at = int(ptr[first]) if plan is part else 0
+        n = int(ptr[last] - ptr[first])
+        back = tuple(torch.full((plan[1].numel(), ps, hkv, d), 7.0, dtype=dt, device=DEV) for _ in range(2))
+        ops.kv8_gather(*cache, *plan, dt, out=back)
+        for t in back:
+            assert bool((t[:at] == 7.0).all()) and bool((t[at + n:] == 7.0).all())
+        assert bool((out[:r0] == 3.0).all()) and bool((out[r1:] == 3.0).all())
+        got.append([out, dec, *(t[at:at + n] for t in back), *(t.view(torch.uint8) for t in cache)])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
 def test_offsets_beyond_32_bits():
     """The same pages at the end of a pool of 2^32 bytes and more a tensor."""
     hq, hkv, d, lens, counts = 32, 8, 128, [70, 33, 200], [20, 1, 45]
