@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
   const uint64_t policy = p.tiles > 1 ? l2_policy_evict_last() : l2_policy_evict_first();
   auto issue = [&](const Meta& m, int i) {   // by the lane that holds unit i
     const int s = i % stages;
-    const int row = max(m.blk, 0) * kBoxRows;   // a bad page: page 0's codes, scale 0
+    const int row = m.blk * kBoxRows;   // a bad page: a box before the first row, which reads as zeros
     mbar_arrive_expect_tx(&full[s], kSlot);
     tma_load_2d(ring + s * kSlot, &tmap_k, &full[s], 0, row, policy);
     tma_load_2d(ring + s * kSlot + kBlock, &tmap_v, &full[s], 0, row, policy);

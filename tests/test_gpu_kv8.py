@@ -555,6 +555,31 @@ def test_attention_bad_pages_are_reported():
             ops.check_device_status(DEV)
 
 
+@pytest.mark.parametrize("dt,d", [(torch.bfloat16, 128), (torch.float16, 64), (torch.float32, 64)])
+@pytest.mark.parametrize("rows,idle", [(1, 0), (3, 0), (20, True)])
+@pytest.mark.parametrize("bad", [99, -1, 4])
+def test_rows_that_see_a_bad_page_are_finite(dt, d, rows, idle, bad):
+    """Whatever page 0 holds: NaN codes, NaN scales."""
+    hq, hkv = 8, 2
+    cache = U.random_cache(4, hkv, 16, d, DEV, 2)
+    for t in cache[:2]:
+        t.view(torch.uint8)[0] = 0x7F
+    for t in cache[2:]:
+        t[0] = math.nan
+    idle = U.idle_for_tiles(1, hq, hkv, rows) if idle else 0
+    none = [np.zeros(0, np.int32)] * idle
+    plan = U.csr([np.array([1, bad, 2], np.int32)] + none, [40] + [0] * idle, 16, DEV)
+    q = U.rows((rows, hq, d), dt, 3).to(DEV)
+    qo = torch.tensor([0] + [rows] * (1 + idle), dtype=torch.int32, device=DEV)
+    outs = [ops.paged_prefill_kv8(q, qo, rows, *cache, *plan, 0.1)]
+    if rows == 1:
+        outs.append(ops.paged_decode_kv8(q, *cache, *plan, 0.1))
+    with pytest.raises(RuntimeError, match="page id"):
+        ops.check_device_status(DEV)
+    for out in outs:
+        assert bool(torch.isfinite(out).all())
+
+
 def test_a_block_that_is_not_finite_reads_as_nan():
     hq, hkv, d = 8, 2, 128
     for dt in (torch.bfloat16, torch.float32):
