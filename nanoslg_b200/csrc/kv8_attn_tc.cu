@@ -698,7 +698,8 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
   }
   __syncthreads();
   const int ngroups = s_ngroups;
-  if (ngroups == 0) return;
+  // a CTA that others wait to count arrives even where its warps gave up before they had a piece
+  if (ngroups == 0 && s_join[0].vid < 0 && s_join[1].vid < 0) return;
   constexpr int DQ = D / 4;
   const float* pieces = reinterpret_cast<const float*>(smem);
   const int ml = p.rows * kPR;           // (m, l) of a piece's rows lie behind its values

@@ -2,6 +2,8 @@
 points refuse."""
 import ctypes
 import math
+import os
+import re
 
 import numpy as np
 import pytest
@@ -185,6 +187,67 @@ def test_ops_refuse(lib, names, bad, error, what):
     for n in names:
         with pytest.raises(error, match=what):
             calls[n]()
+
+
+def _split(total, n):
+    """Bounds of n contiguous parts of [0, total), the first total % n one longer."""
+    q, r = divmod(total, n)
+    return [q * c + min(c, r) for c in range(n + 1)]
+
+
+def _leaves_early():
+    """The condition under which a CTA of the split kernel ends before it arrives, from the source."""
+    path = os.path.join(os.path.dirname(N.__file__), "csrc", "kv8_attn_tc.cu")
+    with open(path) as f:
+        body = f.read().split("const int ngroups = s_ngroups;")[1].split("atom_add_acq_rel_u32")[0]
+    found = re.findall(r"if \((.*)\) return;", body)
+    assert len(found) == 1
+    text = found[0].replace("&&", "and").replace("s_join[0].vid", "vid0").replace("s_join[1].vid", "vid1")
+    return compile(text, path, "eval")
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_split_attention_counts_return_to_zero_when_warps_give_up(seed):
+    """A model of the split kernel's bookkeeping: every CTA over which a virtual sequence is spread
+    arrives at the count of its first one, wherever the waits of any warps ran out (a warp that
+    gives up leaves a piece of the sequence it was at and none of those behind it)."""
+    rng = np.random.default_rng(seed)
+    leaves = _leaves_early()
+    hm, warps, sms = int(rng.integers(1, 9)), 12, int(rng.integers(2, 20))
+    pages = rng.integers(0, 40, int(rng.integers(1, 6)))
+    if seed % 2:                                    # many sequences of a page before a long one
+        pages = np.array([1] * int(rng.integers(20, 60)) + [400])
+    starts = np.cumsum([0] + [n for n in pages for _ in range(hm)])       # first unit of each sequence
+    total = int(starts[-1])
+    vid_of = [v for v in range(len(starts) - 1) for _ in range(starts[v + 1] - starts[v])]
+    n = min(-(-total // warps), sms)
+    if n == 0:
+        return
+    ctas = _split(total, n)
+    cta_of = [c for c in range(n) for _ in range(ctas[c + 1] - ctas[c])]
+    arrived, expected = [0] * n, [0] * n
+    for v in range(len(starts) - 1):
+        if starts[v] < starts[v + 1]:
+            first, last = cta_of[starts[v]], cta_of[starts[v + 1] - 1]
+            expected[first] += last - first + 1 if last > first else 0
+    for c in range(n):
+        u0, u1 = ctas[c], ctas[c + 1]
+        head, tail = vid_of[u0], vid_of[u1 - 1]
+        joins = [head if starts[head] < u0 else -1,
+                 tail if starts[tail] >= u0 and starts[tail + 1] > u1 else -1]
+        groups = set()
+        for a, b in zip(*(lambda w: (w, w[1:]))([u0 + x for x in _split(u1 - u0, warps)])):
+            # units it got through
+            stop = a if seed % 2 else int(rng.integers(a, b + 1)) if rng.random() < 0.7 else b
+            for v in set(vid_of[a:min(stop + 1, b)]):
+                if starts[v] < a or starts[v + 1] > b:                       # not whole: a piece
+                    groups.add(v)
+        if eval(leaves, {}, {"ngroups": len(groups), "vid0": joins[0], "vid1": joins[1]}):
+            continue
+        for v in joins:
+            if v >= 0:
+                arrived[cta_of[starts[v]]] += 1
+    assert arrived == expected
 
 
 def test_manager_bookkeeping_does_not_depend_on_the_cache_type():
