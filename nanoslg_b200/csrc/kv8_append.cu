@@ -265,7 +265,6 @@ __global__ void __launch_bounds__(512) kv8_append_token_kernel(const Kv8AppendPa
     const int64_t blk = static_cast<int64_t>(page) * p.hkv + h;
     float* sc = (kv ? p.scale_v : p.scale_k) + blk;
     const bool writes = live && !is_q && paged;
-    // read before the shuffles, which every lane of the row passes before one of them writes it
     const float was = writes && slot > 0 ? *sc : 0.f;
     float v[16];
 #pragma unroll
@@ -280,6 +279,7 @@ __global__ void __launch_bounds__(512) kv8_append_token_kernel(const Kv8AppendPa
     uint32_t top = top_of(v);
 #pragma unroll
     for (int o = 1; o < kRow; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    __syncwarp();                  // every lane of the row has read the old scale
     if (live && is_q) {
       store_row<T, D>(static_cast<T*>(p.q_out) + (r.row0 * p.hq + h) * D, c, v);
     } else if (writes) {
