@@ -88,13 +88,18 @@ def build_torch(force=False, verbose=False):
 
     import torch
     src = os.path.join(CSRC, "kv8_torch.cpp")
-    stamp = os.path.join(BUILD, "kv8_torch." + torch.__version__)      # another torch: again
+    # what the built file was made against; anything else there: again
+    stamp = os.path.join(BUILD, "kv8_torch.key")
+    abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    key = f"torch {torch.__version__} abi {abi} {sysconfig.get_config_var('SOABI')}"
     if not force and os.path.exists(stamp) and not _stale(KV8, [src, *_headers()]):
-        return KV8
+        with open(stamp) as f:
+            if f.read() == key:
+                return KV8
     t = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(nvcc()))
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", src, "-o", KV8]
+           f"-D_GLIBCXX_USE_CXX11_ABI={abi}", src, "-o", KV8]
     for d in (INCLUDE, os.path.join(t, "include"),
               os.path.join(t, "include", "torch", "csrc", "api", "include"),
               os.path.join(cuda, "include"), sysconfig.get_paths()["include"]):
@@ -106,7 +111,8 @@ def build_torch(force=False, verbose=False):
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed on kv8_torch.cpp:\n{r.stdout}\n{r.stderr}")
-    open(stamp, "w").close()
+    with open(stamp, "w") as f:
+        f.write(key)
     return KV8
 
 

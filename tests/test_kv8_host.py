@@ -4,6 +4,8 @@ import ctypes
 import math
 import os
 import re
+import sysconfig
+from types import SimpleNamespace
 
 import numpy as np
 import pytest
@@ -248,6 +250,27 @@ def test_split_attention_counts_return_to_zero_when_warps_give_up(seed):
             if v >= 0:
                 arrived[cta_of[starts[v]]] += 1
     assert arrived == expected
+
+
+def test_the_torch_side_is_built_again_for_another_torch_or_python(monkeypatch, tmp_path):
+    """Version A, B and A again: three compilations, none while nothing changes."""
+    runs = []
+
+    def compile_(cmd, **_):
+        runs.append(cmd)
+        (tmp_path / "_kv8.so").write_text("built")
+        return SimpleNamespace(returncode=0)
+    monkeypatch.setattr(build, "KV8", str(tmp_path / "_kv8.so"))
+    monkeypatch.setattr(build, "BUILD", str(tmp_path))
+    monkeypatch.setattr(build.subprocess, "run", compile_)
+    for version in ("2.0", "2.0", "2.1", "2.1", "2.0", "2.0"):
+        monkeypatch.setattr(torch, "__version__", version)
+        build.build_torch()
+    assert len(runs) == 3
+    monkeypatch.setattr(sysconfig, "get_config_var", lambda name: "another python")
+    build.build_torch()
+    build.build_torch()
+    assert len(runs) == 4
 
 
 def test_manager_bookkeeping_does_not_depend_on_the_cache_type():
