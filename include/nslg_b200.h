@@ -372,8 +372,8 @@ int nslg_plan_decode_host(int batch, int page_size, const int32_t* slots, const 
  * value = code * scale of its block (the page_size tokens of one page, one kv head). The
  * append writes the smallest power of two s with amax <= 448 s (0 for a block of zeros, at
  * least 2^-126, NaN for a block that holds a value that is not finite: all of that block
- * then reads as NaN). The readers take any scale that is finite and not negative, and NaN (on
- * the tensor cores a V block of a scale below 2^-100 counts as zeros). Page lists are the CSR
+ * then reads as NaN). The readers take any scale from 0 to 2^120, the largest the append
+ * writes, and NaN (on the tensor cores a V block of a scale below 2^-100 counts as zeros). Page lists are the CSR
  * of the other entry points; kv_indptr may be a part of a longer batch's (kv_indptr[0] > 0,
  * kv_indices the whole list). Page 0 needs no special contents, and a page that is handed out
  * again needs no clearing. head_dim is a multiple of 32 up to 256, a page of one layer has
@@ -395,12 +395,16 @@ int nslg_plan_decode_host(int batch, int page_size, const int32_t* slots, const 
  * and where it grows their codes are rounded again for the new scale (exact but for codes
  * that become e4m3 subnormals). A page whose first slot is written starts afresh. Writing
  * the same rows again changes nothing. A page written by a call belongs to one sequence of
- * that call (copy a shared page first, codes and scales).
+ * that call and stands in its list once (copy a shared page first, codes and scales).
+ * What a token did to its block outlives the token: writing other rows over it neither takes
+ * back a scale that it raised nor the rounding of the older codes, and after one that was not
+ * finite the block is NaN, its older tokens lost, until its page is begun again.
  *
  * max_qo_len bounds qo_len(b). A sequence with more rows than that, more than kv_len(b),
- * rows outside [0, num_rows) or a kv_last_page_len outside [1, page_size] sets NSLG_DEV_BAD_PLAN and is skipped; a page outside the pool
- * sets NSLG_DEV_BAD_PAGE (q is still rotated); a position outside the tables sets
- * NSLG_DEV_BAD_POSITION and the part of the page's rows the call writes stays unrotated. */
+ * rows outside [0, num_rows) or a kv_last_page_len outside [1, page_size] sets
+ * NSLG_DEV_BAD_PLAN and is skipped; a page outside the pool sets NSLG_DEV_BAD_PAGE (q is
+ * still rotated); a position outside the tables sets NSLG_DEV_BAD_POSITION and the part of
+ * the page's rows the call writes stays unrotated. */
 int nslg_rope_kv8_append(int dtype, int batch, int num_qo_heads, int num_kv_heads, int head_dim,
                          int page_size, const void* q, int64_t q_stride, const void* k,
                          int64_t k_stride, const void* v, int64_t v_stride, int64_t num_rows,
@@ -415,8 +419,7 @@ int nslg_rope_kv8_append(int dtype, int batch, int num_qo_heads, int num_kv_head
  * [num_indices, page_size, num_kv_heads, head_dim], page j of the list (kv_indptr[0] <= j <
  * kv_indptr[batch] <= num_indices) at out[j]; slots behind a sequence's last token and pages
  * outside the pool (NSLG_DEV_BAD_PAGE) read as zeros, the pages of out of no sequence are left
- * as they are.
- * A finite value beyond fp16's range reads as +-65504 there. */
+ * as they are. A finite value beyond fp16's range reads as +-65504 there. */
 int nslg_kv8_gather(int dtype, int batch, int num_kv_heads, int head_dim, int page_size,
                     const void* codes_k, const void* codes_v, const float* scale_k,
                     const float* scale_v, int64_t num_pages, const int32_t* kv_indptr,

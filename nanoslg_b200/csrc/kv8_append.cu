@@ -15,10 +15,10 @@
 //   q_out = rot(q, p), rounded once to the activation type
 //
 // What bounds it: the bytes of the rows, read once, of q_out and of the codes, written once.
-// Measured (bf16, 32 / 8 heads of 128): prompts of 64 x 512 tokens 180 us with the reading back
-// of what was written, 5.2 TB/s, 0.80 of a copy's rate; 16 x 128 behind 1024 alone 9.0 us
-// (46 MB: 7.0); one token for each of 64 sequences 3.0 us, most of it the launch and the chain
-// plan, page, scale, codes.
+// Measured (bf16, 32 / 8 heads of 128, graphs of 60 calls): prompts of 64 x 512 tokens 139 us,
+// 5.3 TB/s, 0.81 of a copy's rate (181 with the reading back of what was written); 16 x 128
+// behind 1024 11.4 us (46 MB: 7.0); one token for each of 64 sequences 2.9 us, most of it the
+// launch and the chain plan, page, scale, codes.
 #include <algorithm>
 
 #include "kv8.cuh"
@@ -304,6 +304,9 @@ __global__ void __launch_bounds__(512) kv8_append_token_kernel(const Kv8AppendPa
 }
 
 // ---------------------------------------------------------------- any shape and type
+// A block a page and kv head, two codes a store, every element of K rotated twice (for the
+// block's largest magnitude and for the codes): there to be right. 16 x 128 rows behind 1024, 32 / 8
+// heads: 55 us for fp32, 47 at head_dim 96, 92 in pages of 32 (11 by the kernel above).
 constexpr int kAppendThreads = 128;
 
 template <typename T>
@@ -404,10 +407,12 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8App
 }
 
 // Reading back: the listed pages as [page_size, hkv, d] values of type T in list order; slots
-// behind the sequence's last token are zeros. Rows of list entries of no sequence are left as they are. A thread takes 16 codes of one head row: 16-byte loads,
-// 16-byte stores, consecutive threads along the output. Bound by its bytes (one read and two
-// or four written per element): 16 sequences of 1152 tokens (8 heads of 128, bf16) 24.4 us,
-// 4.6 TB/s, 2 of it the launch; 1, 2 or 4 chunks a thread at a time take the same within 7 %.
+// behind the sequence's last token are zeros. Rows of list entries of no sequence are left as
+// they are. A thread takes 16 codes of one head row: 16-byte loads, 16-byte stores, consecutive
+// threads along the output. Bound by its bytes (one read and two or four written per element):
+// 16 sequences of 1152 tokens (8 heads of 128, bf16) 24.4 us, 4.6 TB/s, 2 of it the launch, fp32
+// output 45 us; 1, 2 or 4 chunks a thread at a time take the same within 7 %. What holds it below a copy's rate is likely the stores: a thread's chunk is
+// 32 bytes of output in two stores, so a warp's store touches 32 sectors by halves (counted).
 constexpr int kGatherThreads = 256;
 
 template <typename T>

@@ -4,9 +4,12 @@
 // What bounds it: the bytes of the cache, one per element, read once. So every SM streams
 // an equal share of them whatever the sequences' lengths, and the arithmetic per byte is
 // kept below what an SM can issue in the time its share of the bandwidth takes. Measured
-// (bf16, 32 / 8 heads of 128): 64 sequences of 512 to 8192 tokens 98 us, 6.1 TB/s, 0.93 of
-// a copy's rate; 64 of 513 to 768 23.9 us (87 MB: 13.3 at that rate, and about 9 us of launch,
-// plan, first loads and joining, none of which the batch's size changes); one of 513 8.0 us.
+// (bf16, 32 / 8 heads of 128, graphs of 60 calls): 64 sequences of 512 to 8192 tokens 103 us,
+// 5.8 TB/s, 0.89 of a copy's rate (110 us over seconds); 64 of 513 to 768 24.4 us (87 MB: 13.3
+// at that rate, and about 10 us of launch, plan, first loads and joining, none of which the
+// batch's size changes); one of 513 9.0 us. The page list is read behind the kernel in front,
+// like all else: reading it ahead of that saved 0.7 to 1.4 us a call and took a list that the
+// kernel in front had yet to write.
 //
 // Work split. A unit is one page of one kv head: 16 tokens, K and V blocks of 16 * head_dim
 // bytes each, contiguous, with one scale each. A "virtual sequence" is (sequence, kv head,
@@ -81,8 +84,8 @@ struct TcParams : Kv8AttnParams {
   float scale_log2;
 };
 
-// W warps a CTA, one CTA an SM. With 12 the rings of a full SM are 192 KiB in 4 stages; at 8 query
-// rows a warp 8 / 12 / 16 warps took 119 / 98.7 / 100 us for 64 sequences of up to 8192 tokens
+// W warps a CTA, one CTA an SM. With 12 the rings of a full SM are 192 KiB in 4 stages; at 8
+// query rows a warp (times of short bursts) 8 / 12 / 16 warps took 119 / 98.7 / 100 us for 64 sequences of up to 8192 tokens
 // (8 kv heads of 128), 16.9 / 16.2 / 17.2 for 32 of up to 4096 (2 kv heads). The 16 rows of two
 // column tiles need more than the 168 registers of 12 warps.
 template <int NT>

@@ -4,9 +4,11 @@
 // What bounds it: 4 * head_dim flop and one exponential per (query row, head, position). At 16
 // exponentials a clock and SM they take as long as the products at full rate (0.55 us for 256
 // rows and 64 positions at head_dim 128), so everything else has to stay off the softmax
-// warps. Measured (bf16, 32 / 8 heads of 128): prompts of 64 x 512 tokens 226 us, 16 suffixes
-// of 128 behind 1024 57 us (640 TFLOP/s): 1.1 to 1.2 us for such a tile, the chain of one half's
-// scores, maximum, exponentials and weights, and 2 us at an item's end.
+// warps. Measured (bf16, 32 / 8 heads of 128, graphs of 60 calls): prompts of 64 x 512 tokens
+// 256 us (540 TFLOP/s; 182 us at head_dim 64), 16 suffixes of 128 behind 1024 57 us (640): 1.1 to
+// 1.2 us for such a tile, the chain of one half's scores, maximum, exponentials and weights, and
+// 2 us at an item's end. The steps quoted below were measured in bursts of a few calls, before
+// the power limit lowers the clocks; there the prompts take 226 us.
 //
 // The codes are not dequantised: they are only widened, which is exact (K to q's type, V to
 // f16), and the blocks' scales join the exponent, where they cost nothing per element:

@@ -219,13 +219,14 @@ struct Kv8AttnParams : Kv8Cache {
 // CUDA cores: any page size, head_dim a multiple of 32 up to 256, all three types.
 int launch_kv8_attention_simt(int dtype, const Kv8AttnParams& p, cudaStream_t stream);
 
-// Tensor cores, split over the cache (kv8_attn_tc.cu): decode, and a few rows a sequence.
+// Tensor cores, split over the cache (kv8_attn_tc.cu): decode, a few rows a sequence, and any
+// number of rows in the groups that the kernel below does not take.
 bool kv8_attn_tc_supported(int dtype, const Kv8AttnParams& p);
 int64_t kv8_attn_tc_workspace_bytes(int group, int max_qo_len, int d);
 int launch_kv8_attention_tc(int dtype, const Kv8AttnParams& p, void* workspace,
                             int64_t workspace_bytes, cudaStream_t stream);
 
-// tcgen05 (kv8_prefill_tc.cu): head_dim 128, groups that divide 128.
+// tcgen05 (kv8_prefill_tc.cu): head_dim 64 and 128, groups of 1, 2, 4, 8 and 16.
 bool kv8_prefill_tc_supported(int dtype, const Kv8AttnParams& p);
 bool kv8_prefill_tc_faster(const Kv8AttnParams& p);   // than launch_kv8_attention_tc
 int launch_kv8_prefill_tc(int dtype, const Kv8AttnParams& p, cudaStream_t stream);

@@ -497,7 +497,8 @@ def rope_kv8_append(q, k, v, cos, sin, pool_k, pool_v, scale_k, scale_v, qo_indp
     them. The position is the row of the cos / sin tables (fp32 [rows, D]). A block's scale
     is the smallest power of two that brings its largest magnitude to 448 or less; in a
     page with older tokens it never shrinks, and where it grows their codes are rounded
-    again. Returns q_out ([rows, Hq, D], rotated q; rows of no sequence are left as they
+    again; a value that is not finite makes its block NaN, the older tokens included. Neither
+    is taken back by writing other rows over the token, only by beginning the page again. Returns q_out ([rows, Hq, D], rotated q; rows of no sequence are left as they
     are), or None when q is None. With ``rotate=False`` q and k are taken as already
     rotated, cos and sin are ignored.
     """
