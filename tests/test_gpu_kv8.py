@@ -207,6 +207,25 @@ def test_append_bad_plans_are_reported_and_skipped():
         ops.check_device_status(DEV)
 
 
+@pytest.mark.parametrize("dt,hq,hkv,d,ps", [(torch.bfloat16, 32, 8, 128, 16), (torch.float16, 12, 2, 64, 16),
+                                            (torch.float32, 4, 2, 64, 16), (torch.bfloat16, 6, 3, 96, 5)])
+@pytest.mark.parametrize("counts", [[1, 1, 1], [40, 3, 1]])
+def test_append_turns_q_in_place(dt, hq, hkv, d, ps, counts):
+    lens = [n + s for n, s in zip(counts, (7, 0, 30))]
+    tables = U.page_lists(lens, ps, 40, 4)
+    cos, sin = (t.to(DEV) for t in _tables(max(lens), d))
+    plan = U.csr(tables, lens, ps, DEV)
+    qo = torch.tensor(np.cumsum([0] + counts), dtype=torch.int32, device=DEV)
+    q, k, v = (U.rows((sum(counts), h, d), dt, 5 + h).to(DEV) for h in (hq, hkv, hkv))
+    first, second = (U.random_cache(40, hkv, ps, d, DEV, 6) for _ in range(2))
+    want = ops.rope_kv8_append(q, k, v, cos, sin, *first, qo, max(counts), *plan)
+    assert not torch.equal(want, q)
+    assert ops.rope_kv8_append(q, k, v, cos, sin, *second, qo, max(counts), *plan, q_out=q) is q
+    assert torch.equal(q, want)
+    for a, b in zip(first, second):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("hkv,d,ps,lens", [(8, 128, 16, [1, 0, 33, 512]), (2, 64, 16, [300]),
                                            (3, 96, 5, [7, 5, 1]), (1, 256, 64, [65])])
